@@ -480,6 +480,126 @@ int64_t vl_knn_metric_workspace_bytes(int64_t n_queries, int64_t n_vectors, int6
 int64_t vl_knn_left_offset(int64_t n_queries, int64_t n_vectors, int64_t dim, int64_t k, int32_t metric,
                            int64_t workspace_bytes);
 
+/* ---- attention over a key/value cache in 4 bits ------------------------- */
+/* No counterpart in the reference.  A program that answers with a language
+ * model keeps, per layer, the keys and values of all tokens so far.  They are
+ * held here as the vectors of an index are looked at through its sketch: few
+ * bits, cheap bounds that decide what is fetched, and exact sums over what is.
+ *
+ * The cache is a pool of pages of 64 tokens; device memory of the caller's.  32
+ * dimensions of a token's key or value are a group: 32 codes of 4 bits (sign,
+ * two bits of exponent, one of mantissa, standing for 0 0.5 1 1.5 2 3 4 6) and a
+ * byte, the exponent + 127 of a power of two (the OCP microscaling format
+ * MXFP4).
+ *   keys          [pages, heads, 64, dim / 2]       dimensions 2 j and 2 j + 1 in the low and high bits of byte j
+ *   values        [pages, heads, 16, dim / 8, 4, 4] token / 4, dim / 8, token % 4, the four bytes of 8 dimensions
+ *   key_scales, value_scales [pages, heads, dim / 32, 64]
+ *   bounds        [pages, heads, 2, dim]            of a page's keys: the largest and the smallest in each
+ *                                                   dimension, rounded outwards to 8 bits
+ *   bound_scales  [pages, heads]                    exponent of the power of two that they are multiplied with
+ * Writing rounds to the nearest code, of two as near to the even one; the scale
+ * of a group is 2^max(floor(log2(largest magnitude)) - 2, -124), and magnitudes
+ * over 6 times it become 6.  A token with an element that is not finite gets
+ * scale bytes 255 and reads as NaN, and its page has bound_scale 127.  dim: 32,
+ * 64, 96, 128, 192 or 256.  All pointers on 16-byte boundaries. */
+typedef struct vl_cache {
+    int64_t pages, heads, dim;
+    uint8_t *keys, *key_scales, *values, *value_scales;
+    int8_t *bounds, *bound_scales;
+} vl_cache;
+
+/* The tokens of a call.  Rows [offsets[b], offsets[b + 1]) belong to sequence b;
+ * offsets NULL: rows == sequences and row b belongs to sequence b.  table[b, :]
+ * names the page of each block of 64 tokens of the sequence; a page outside
+ * [0, pages) holds nothing: what is written there is dropped, and it takes no
+ * part in attention.  lengths[b]: tokens in the sequence, see each call. */
+typedef struct vl_tokens {
+    int64_t rows, sequences, blocks, table_stride;
+    const int32_t *table;   /* [sequences, blocks] */
+    const int32_t *lengths; /* [sequences] */
+    const int32_t *offsets; /* [sequences + 1] or NULL */
+} vl_tokens;
+
+#define VL_BF16 1
+#define VL_F16 2
+#define VL_F32 3
+
+/* Quantises keys and values [rows, heads, dim] (strides in elements, rows of dim
+ * contiguous) to the places lengths[b], lengths[b] + 1, ... of their sequences:
+ * lengths is what the sequences hold BEFORE the call.  The bounds of every block
+ * written into are made anew from all of its tokens up to the last one written.
+ * Two sequences must not share a page that is written into. */
+int vl_cache_write(const vl_cache *cache, const vl_tokens *tokens, int type,
+                   const void *keys, int64_t key_row, int64_t key_head,
+                   const void *values, int64_t value_row, int64_t value_head,
+                   void *stream);
+/* The reverse: the keys and values [rows, heads, dim] that the cache holds at
+ * these places; zeros at places without a page. */
+int vl_cache_read(const vl_cache *cache, const vl_tokens *tokens, int type,
+                  void *keys, void *values, void *stream);
+/* out [n, heads, 2, dim]: the bounds of pages[0 .. n) as the values they stand
+ * for; -inf and inf the other way round (no bounds) where bound_scale is 127,
+ * zeros for a page outside the cache. */
+int vl_cache_read_bounds(const vl_cache *cache, const int32_t *pages, int64_t n,
+                         float *out, void *stream);
+
+/* Queries [rows, heads, dim] of a call, heads a multiple of the cache's: heads
+ * [h * heads / cache.heads, ...) attend to its head h.  The rows of sequence b
+ * stand at its last places: row i of n at lengths[b] - n + i.  out: [rows,
+ * heads, dim] of the queries' type, contiguous.  lse: NULL, or [rows, heads]
+ * logarithms of the sums of exponentials.  A row that sees no token gives zeros
+ * (and -inf). */
+typedef struct vl_queries {
+    int64_t heads, row_stride, head_stride;
+    const void *queries;
+    void *out;
+    float *lse;
+    double scale; /* scores are scale * <query, key> */
+    int32_t type; /* VL_BF16, VL_F16, VL_F32 */
+    int32_t causal; /* 0: every row sees all lengths[b] tokens; else those up to its own place */
+} vl_queries;
+
+/* Softmax attention over everything the cache holds of the sequences.  Sums and
+ * softmax are held in 32 bits; keys, values and queries enter the products
+ * exactly, the weights rounded to the queries' type or finer. */
+int64_t vl_attend_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries);
+int vl_attend(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
+              void *workspace, int64_t workspace_bytes, void *stream);
+/* The form that takes such a call: VL_ATTEND_FEW splits the tokens over
+ * workgroups, VL_ATTEND_MANY shares them among the rows of a workgroup. */
+#define VL_ATTEND_FEW 0
+#define VL_ATTEND_MANY 1
+int vl_attend_form(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries);
+
+/* blocks [rows, cache.heads, count]: for every row and head of the cache the
+ * block of the row's own token and the others up to it with the best scores,
+ * ascending, then VL_MAXINT.  The score of a block is an upper bound of the
+ * largest <query, key> in it: with u the queries of the row that share the head
+ * rounded to 8 bits with one power of two (largest magnitude in [64, 128), cut
+ * to 127), the largest over these queries of sum_j max(u_j, 0) hi_j +
+ * min(u_j, 0) lo_j, hi and lo the block's bounds; whole numbers times a power
+ * of two, so that no order of the sum changes one.  Blocks without bounds (127)
+ * come before all others, ties go to the lower block; queries that are not
+ * finite count as zeros.  A row before the first token has no blocks.
+ * queries->out, lse, scale and causal are not looked at. */
+int64_t vl_select_blocks_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
+                                         int64_t count);
+int vl_select_blocks(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries, int64_t count,
+                     int32_t *blocks, void *workspace, int64_t workspace_bytes, void *stream);
+/* Softmax attention of every row over the tokens of its blocks [rows,
+ * cache.heads, count] up to its own place (causal is not looked at).  Blocks
+ * outside the table are skipped; a block named twice counts twice. */
+int64_t vl_attend_blocks_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
+                                         int64_t count);
+int vl_attend_blocks(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
+                     const int32_t *blocks, int64_t count,
+                     void *workspace, int64_t workspace_bytes, void *stream);
+/* vl_select_blocks, then vl_attend_blocks on its choice, which it leaves in blocks. */
+int64_t vl_attend_selected_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
+                                           int64_t count);
+int vl_attend_selected(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries, int64_t count,
+                       int32_t *blocks, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

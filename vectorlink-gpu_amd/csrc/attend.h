@@ -1,0 +1,29 @@
+// Attention over the cache: what its kernels and their launchers share.
+#pragma once
+#include "cache.h"
+
+// S = scale <query, key>, P = softmax of S over the tokens that a row sees, out = P values.
+struct AttendArgs {
+    CacheView c;
+    Tokens t;
+    const void *queries;
+    int64_t q_row, q_head;  // strides in elements
+    void *out;              // [rows, heads_q, D]
+    float *lse;             // [rows, heads_q] or null
+    const int32_t *list;    // [rows, c.heads, count] blocks of every row and head, or null: all blocks
+    int count;
+    int group, heads_q;     // queries that share a head of the cache; c.heads * group
+    int causal, aligned;
+    float scale;            // |scale| log2(e): exponentials are powers of two here
+    uint32_t sign;          // 0x80000000 where the scale is negative: turns the queries' sign
+    int splits;
+    float *part;            // splits > 1: [rows * heads_q, splits, D] sums, then [rows * heads_q, splits, 2] maxima and sums of weights
+};
+constexpr int kMaxSplits = 64;
+
+// 16 rows at a time, the tokens split over wavefronts and workgroups
+template <int NS>
+int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream);
+extern template int launch_attend_few<1>(const AttendArgs &, int64_t, hipStream_t);
+extern template int launch_attend_few<2>(const AttendArgs &, int64_t, hipStream_t);
+extern template int launch_attend_few<3>(const AttendArgs &, int64_t, hipStream_t);

@@ -1,0 +1,181 @@
+// Attention over the cache: entry points, their checks, and how a call is cut into workgroups.
+#include "attend.h"
+
+#include <math.h>
+
+#include "select.h"
+
+namespace {
+
+int attend_args(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *q, bool data, AttendArgs *a) {
+    *a = {};
+    int rc = vl_cache_of(cache, &a->c);
+    if (rc == VL_OK) rc = vl_tokens_of(tokens, &a->t);
+    if (rc != VL_OK) return rc;
+    VL_REQUIRE(q != nullptr, "queries is null");
+    VL_REQUIRE(q->type >= VL_BF16 && q->type <= VL_F32, "type: %d", q->type);
+    VL_REQUIRE(q->heads >= 1 && q->heads <= (1 << 24) && q->heads % a->c.heads == 0, "%lld heads of queries for %d of the cache",
+               (long long)q->heads, a->c.heads);
+    const int size = q->type == VL_F32 ? 4 : 2;
+    if (data && a->t.rows) {
+        VL_REQUIRE(q->queries && q->out, "queries or out is null");
+        VL_REQUIRE((uintptr_t)q->queries % size == 0, "queries not aligned to their type");
+        VL_REQUIRE(((uintptr_t)q->out & 15) == 0, "out not on a 16-byte boundary");
+        VL_REQUIRE(isfinite(q->scale), "scale is not finite");
+    }
+    a->queries = q->queries;
+    a->q_row = q->row_stride;
+    a->q_head = q->head_stride;
+    a->out = q->out;
+    a->lse = q->lse;
+    a->heads_q = (int)q->heads;
+    a->group = (int)(q->heads / a->c.heads);
+    a->causal = q->causal != 0;
+    a->aligned = ((uintptr_t)q->queries & 15) == 0 && q->row_stride * size % 16 == 0 && q->head_stride * size % 16 == 0;
+    a->scale = (float)(fabs(q->scale) * 1.4426950408889634);
+    a->sign = q->scale < 0 ? 0x80000000u : 0;
+    a->splits = 1;
+    return VL_OK;
+}
+
+// Tiles of 16 rows: rows of a sequence and a head come one after the other, and every sequence may end inside a tile.
+int64_t few_tiles(const AttendArgs &a) {
+    const int64_t per = (a.group + 15) / 16;
+    if (a.count || !a.t.offsets) return a.t.rows * per;
+    return (int64_t)a.t.rows * a.group / 16 + a.t.sequences;
+}
+
+// Workgroups that the tokens of a tile are split over: enough for four on every compute unit, but a page for every wavefront.
+int splits_for(const AttendArgs &a, int64_t tiles) {
+    const int64_t entries = a.count ? a.count : a.t.blocks;
+    const int64_t items = tiles * a.c.heads;
+    if (items == 0) return 1;
+    int64_t s = (4 * kComputeUnits + items - 1) / items;
+    s = s < (entries + 3) / 4 ? s : (entries + 3) / 4;
+    return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+}
+
+int64_t part_bytes(const AttendArgs &a, int splits) {
+    if (splits <= 1) return 0;
+    return ((int64_t)a.t.rows * a.heads_q * splits * (a.c.dim + 2) * 4 + 255) / 256 * 256;
+}
+
+int attend_few(AttendArgs &a, int type, void *workspace, int64_t bytes, hipStream_t stream) {
+    const int64_t tiles = few_tiles(a);
+    a.splits = splits_for(a, tiles);
+    const int64_t need = part_bytes(a, a.splits);
+    if (need > bytes || (need && !workspace)) {
+        vl_set_error("workspace too small: %lld bytes needed, %lld given", (long long)need, (long long)bytes);
+        return VL_ERR_WORKSPACE;
+    }
+    VL_REQUIRE(((uintptr_t)workspace & 15) == 0, "workspace not on a 16-byte boundary");
+    a.part = (float *)workspace;
+    return type == VL_BF16 ? launch_attend_few<1>(a, tiles, stream) : type == VL_F16 ? launch_attend_few<2>(a, tiles, stream) : launch_attend_few<3>(a, tiles, stream);
+}
+
+int check_count(int64_t count) {
+    VL_REQUIRE(count >= 1 && count < (1 << 24), "count: %lld", (long long)count);
+    return VL_OK;
+}
+
+SelectArgs select_args(const AttendArgs &a, int64_t count) {
+    return {a.c, a.t, a.queries, a.q_row, a.q_head, a.group, a.aligned, (int)count, nullptr, nullptr};
+}
+
+int choose(const AttendArgs &a, int type, int64_t count, int32_t *blocks, void *workspace, int64_t bytes, hipStream_t stream) {
+    SelectArgs s = select_args(a, count);
+    const int64_t need = select_workspace_bytes(s);
+    if (need > bytes || (need && !workspace)) {
+        vl_set_error("workspace too small: %lld bytes needed, %lld given", (long long)need, (long long)bytes);
+        return VL_ERR_WORKSPACE;
+    }
+    VL_REQUIRE(blocks, "blocks is null");
+    s.out = blocks;
+    s.keys = (uint32_t *)workspace;
+    return launch_select(s, type, stream);
+}
+
+}  // namespace
+
+VL_EXPORT int vl_attend_form(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries) {
+    AttendArgs a;
+    const int rc = attend_args(cache, tokens, queries, false, &a);
+    return rc != VL_OK ? rc : VL_ATTEND_FEW;
+}
+
+VL_EXPORT int64_t vl_attend_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries) {
+    AttendArgs a;
+    const int rc = attend_args(cache, tokens, queries, false, &a);
+    return rc != VL_OK ? rc : part_bytes(a, splits_for(a, few_tiles(a)));
+}
+
+VL_EXPORT int vl_attend(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries, void *workspace,
+                        int64_t workspace_bytes, void *stream) {
+    AttendArgs a;
+    const int rc = attend_args(cache, tokens, queries, true, &a);
+    if (rc != VL_OK || a.t.rows == 0) return rc;
+    return attend_few(a, queries->type, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+VL_EXPORT int64_t vl_select_blocks_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
+                                                   int64_t count) {
+    AttendArgs a;
+    int rc = attend_args(cache, tokens, queries, false, &a);
+    if (rc == VL_OK) rc = check_count(count);
+    return rc != VL_OK ? rc : select_workspace_bytes(select_args(a, count));
+}
+
+VL_EXPORT int vl_select_blocks(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries, int64_t count,
+                               int32_t *blocks, void *workspace, int64_t workspace_bytes, void *stream) {
+    AttendArgs a;
+    int rc = attend_args(cache, tokens, queries, false, &a);
+    if (rc == VL_OK) rc = check_count(count);
+    if (rc != VL_OK || a.t.rows == 0) return rc;
+    VL_REQUIRE(a.queries && (uintptr_t)a.queries % (queries->type == VL_F32 ? 4 : 2) == 0, "queries is null or not aligned to its type");
+    return choose(a, queries->type, count, blocks, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+VL_EXPORT int64_t vl_attend_blocks_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
+                                                   int64_t count) {
+    AttendArgs a;
+    int rc = attend_args(cache, tokens, queries, false, &a);
+    if (rc == VL_OK) rc = check_count(count);
+    a.count = (int)count;
+    return rc != VL_OK ? rc : part_bytes(a, splits_for(a, few_tiles(a)));
+}
+
+VL_EXPORT int vl_attend_blocks(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries, const int32_t *blocks,
+                               int64_t count, void *workspace, int64_t workspace_bytes, void *stream) {
+    AttendArgs a;
+    int rc = attend_args(cache, tokens, queries, true, &a);
+    if (rc == VL_OK) rc = check_count(count);
+    if (rc != VL_OK || a.t.rows == 0) return rc;
+    VL_REQUIRE(blocks, "blocks is null");
+    a.list = blocks;
+    a.count = (int)count;
+    return attend_few(a, queries->type, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+VL_EXPORT int64_t vl_attend_selected_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
+                                                     int64_t count) {
+    AttendArgs a;
+    int rc = attend_args(cache, tokens, queries, false, &a);
+    if (rc == VL_OK) rc = check_count(count);
+    if (rc != VL_OK) return rc;
+    a.count = (int)count;
+    return select_workspace_bytes(select_args(a, count)) + part_bytes(a, splits_for(a, few_tiles(a)));
+}
+
+VL_EXPORT int vl_attend_selected(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries, int64_t count,
+                                 int32_t *blocks, void *workspace, int64_t workspace_bytes, void *stream) {
+    AttendArgs a;
+    int rc = attend_args(cache, tokens, queries, true, &a);
+    if (rc == VL_OK) rc = check_count(count);
+    if (rc != VL_OK || a.t.rows == 0) return rc;
+    rc = choose(a, queries->type, count, blocks, workspace, workspace_bytes, (hipStream_t)stream);
+    if (rc != VL_OK) return rc;
+    const int64_t used = select_workspace_bytes(select_args(a, count));
+    a.list = blocks;
+    a.count = (int)count;
+    return attend_few(a, queries->type, workspace ? (uint8_t *)workspace + used : nullptr, workspace_bytes - used, (hipStream_t)stream);
+}

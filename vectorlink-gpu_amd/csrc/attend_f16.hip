@@ -1,0 +1,4 @@
+// Attention of a few rows: queries of type f16.
+#include "attend_few.h"
+
+template int launch_attend_few<2>(const AttendArgs &, int64_t, hipStream_t);

@@ -1,0 +1,416 @@
+// Attention of a few rows over many tokens: single tokens of a batch of answers, a handful of proposed tokens, and rows with
+// blocks of their own.
+//
+// What bounds it is the cache's bytes: D + D / 16 a token and head, against 4 D operations for each of the queries that share
+// the head.  So a wavefront takes whole pages, 64 tokens at a time, every byte read once in 16-byte pieces, and keeps the
+// rest in registers; a maximum and a sum that run along (x -> exp2(x - max), both rescaled where the maximum grows) make one
+// pass of it.
+//
+// S^T = K Q^T: A = 16 tokens x 32 dimensions, B = 32 dimensions x 16 rows (row = lane % 16 = r, quad = lane / 16 = c).  Which
+// token stands in which row of A and which dimension at which place of the sum is free, as long as both operands agree:
+//   token of tile m, row 4 c' + e of A:  c' * 16 + m * 4 + e,  so the results of a lane are 16 tokens in a row, c * 16 ...
+//   dimensions of lane (c, .):           a quarter of a part of 128 (or 64, 32), so that its 16 (8, 4) bytes have one scale.
+// out^T = V^T P^T then takes P^T as it lies in the registers: B = 32 tokens x 16 rows, of quad c the tokens c * 16 + 8 s ...,
+// and A = 16 dimensions x the same tokens.  A byte of the cache holds two dimensions of a token, so two tokens' bytes turn
+// into two dimensions' pairs of tokens by two permutations.  Row i of tile k of a part: dimension 8 i + k (4 i + k, 2 i + k).
+//
+// Queries enter as NS bfloat16 values that add up to them exactly (bfloat16 1, half 2, float32 3: 24 bits), weights as two that
+// hold 16 bits of them (float32: three, 24 bits), keys and values are exact.  Weights of one part would halve the matrix
+// instructions of the second product, which are not what bounds this, and their error would be as large as a bfloat16
+// result's own rounding.
+#pragma once
+#include "attend.h"
+
+template <int D>
+struct Parts {  // D = parts of 128, then 64, then 32
+    static constexpr int k128 = D / 128, k64 = D % 128 / 64, k32 = D % 64 / 32, kCount = k128 + k64 + k32;
+    static constexpr int width(int p) { return p < k128 ? 128 : p == k128 && k64 ? 64 : 32; }
+    static constexpr int base(int p) { return p <= k128 ? 128 * p : 128 * k128 + 64; }
+};
+
+// one page of a head, as a lane holds it
+template <int D>
+struct PageRegs {
+    static constexpr int P = Parts<D>::kCount;
+    uint32_t k[P][4][4];  // [part][tile m][word]
+    u32x4 ks[P];          // scales of tiles 0 .. 3: byte r % 4 of word m
+    u32x4 v[P][4];        // [part][4 tokens m], a word a token
+    u32x4 vs[P];          // scales of tokens c * 16 + 4 m + byte
+};
+
+template <int D>
+__device__ inline void load_page(PageRegs<D> &g, const CacheView &c, int64_t page, int h) {
+    typedef Parts<D> PT;
+    const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
+    const int64_t unit = page * c.heads + h;
+    const uint8_t *const kc = c.keys + unit * (kPage * D / 2), *const vc = c.values + unit * (kPage * D / 2);
+    const uint8_t *const ks = c.key_scales + unit * (kPage * D / 32), *const vs = c.value_scales + unit * (kPage * D / 32);
+    const int token = (r >> 2) * 16 + (r & 3);
+#pragma unroll
+    for (int p = 0; p < PT::kCount; p++) {
+        const int W = PT::width(p), base = PT::base(p);
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            const uint8_t *const at = kc + (token + m * 4) * (D / 2) + base / 2 + q * (W / 8);
+            if (W == 128) {
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(at);
+                g.k[p][m][0] = x[0], g.k[p][m][1] = x[1], g.k[p][m][2] = x[2], g.k[p][m][3] = x[3];
+            } else if (W == 64) {
+                const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
+                g.k[p][m][0] = x[0], g.k[p][m][1] = x[1];
+            } else {
+                g.k[p][m][0] = *reinterpret_cast<const uint32_t *>(at);
+            }
+        }
+        g.ks[p] = *reinterpret_cast<const u32x4 *>(ks + (base / 32 + q * W / 128) * kPage + (r >> 2) * 16);
+    }
+#pragma unroll
+    for (int p = 0; p < PT::kCount; p++) {
+        const int W = PT::width(p), base = PT::base(p);
+        const int seg = base / 8 + r * W / 128;
+#pragma unroll
+        for (int m = 0; m < 4; m++) g.v[p][m] = *reinterpret_cast<const u32x4 *>(vc + ((q * 4 + m) * (D / 8) + seg) * 16);
+        g.vs[p] = *reinterpret_cast<const u32x4 *>(vs + (seg >> 2) * kPage + q * 16);
+    }
+}
+
+// NS bfloat16 values that add up to x (to 8 NS bits of it): the first NS - 1 cut off, so that what is left is exact.
+template <int NS>
+__device__ inline void split_into(float x, __bf16 (&out)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS; n++) {
+        if (n == NS - 1) {
+            out[n] = (__bf16)x;
+        } else {
+            const float cut = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xFFFF0000u);
+            out[n] = (__bf16)cut;
+            x -= cut;
+        }
+    }
+}
+
+// The state of 16 rows: lane (q, r) holds row r, of every part of W dimensions the W / 4 from q * W / 4 on, as [place e][tile k]:
+// dimension base + (W / 16) * (4 q + e) + k.
+template <int D>
+struct RowState {
+    f32x4 acc[D / 16];  // tiles of all parts, one after the other
+    float top, sum;     // maximum so far (of all lanes of the row), sum of this lane's weights
+};
+
+// The queries of lane (q, r): those of row r, the dimensions as the keys' words hold them.
+template <int D, int NS>
+struct QueryRegs {
+    bf16x8 x[NS][D / 32];
+};
+
+template <int D, int NS>
+__device__ inline void load_queries(QueryRegs<D, NS> &f, const AttendArgs &a, bool real, int64_t row, int head) {
+    typedef Parts<D> PT;
+    typedef typename ElementOf<NS>::type E;
+    const int q = (threadIdx.x & 63) >> 4;
+    const E *const at = (const E *)a.queries + (real ? row * a.q_row + head * a.q_head : 0);
+#pragma unroll
+    for (int p = 0; p < PT::kCount; p++) {
+        const int W = PT::width(p), base = PT::base(p);
+#pragma unroll
+        for (int j = 0; j < W / 32; j++) {
+            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (real) load8<NS>(at + base + q * (W / 4) + j * 8, a.aligned, x);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                __bf16 s[NS];
+                split_into<NS>(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[i]) ^ a.sign), s);
+#pragma unroll
+                for (int n = 0; n < NS; n++) f.x[n][base / 32 + j][i] = s[n];
+            }
+        }
+    }
+}
+
+// Tokens of a page: see(token) says whether this lane's row sees the token's place in the page; edge: some row does not see
+// some token, or some token may not be finite.  spoilt tokens (scale 255) turn the rows that see them into NaN, and no others.
+template <int D, int NS>
+__device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryRegs<D, NS> &f, float scale, bool edge, int sees,
+                                 int written) {
+    typedef Parts<D> PT;
+    constexpr int NW = NS < 2 ? 2 : NS;  // parts of a weight
+    const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
+    f32x4 s[4];
+    const int turn = (8 * (r & 3) + 9) & 31;
+#pragma unroll
+    for (int m = 0; m < 4; m++) {
+        s[m] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int p = 0; p < PT::kCount; p++) {
+            const float ks = __builtin_bit_cast(float, __builtin_amdgcn_alignbit(g.ks[p][m], g.ks[p][m], turn));
+#pragma unroll
+            for (int j = 0; j < PT::width(p) / 32; j++) {
+                const bf16x8 k = eight_values(g.k[p][m][j], ks);
+#pragma unroll
+                for (int n = 0; n < NS; n++)
+                    s[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, f.x[n][PT::base(p) / 32 + j], s[m], 0, 0, 0);
+            }
+        }
+        s[m] *= scale;
+    }
+    if (edge) {
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int token = q * 16 + m * 4 + e;
+                const uint32_t byte = g.vs[0][m] >> (8 * e) & 255;
+                if (byte == kNotFinite) s[m][e] = NAN;
+                if (token >= sees) s[m][e] = -INFINITY;
+                if (byte == kNotFinite || token >= written) {
+                    // its weight is 0 or NaN whatever it holds: any finite value will do
+#pragma unroll
+                    for (int p = 0; p < PT::kCount; p++) g.vs[p][m] = g.vs[p][m] & ~(255u << (8 * e)) | (127u << (8 * e));
+                }
+            }
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 16; i++) top = fmaxf(top, s[i >> 2][i & 3]);
+    top = fmaxf(max_over_quads(top), st.top);
+    if (__ballot(top > st.top)) {
+        const float less = top > -INFINITY ? __builtin_amdgcn_exp2f(st.top - top) : 1.0f;
+        st.top = top;
+        st.sum *= less;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) st.acc[k] *= less;
+    }
+    const float from = st.top > -INFINITY ? st.top : 0.0f;  // a row that has seen nothing yet: all weights 0
+#pragma unroll
+    for (int m = 0; m < 4; m++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[m][e] = __builtin_amdgcn_exp2f(s[m][e] - from);
+        st.sum += (s[m][0] + s[m][1]) + (s[m][2] + s[m][3]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {  // 32 tokens a step: of every quad 8
+        bf16x8 w[NW];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            __bf16 x[NW];
+            split_into<NW>(s[2 * h + (i >> 2)][i & 3], x);
+#pragma unroll
+            for (int n = 0; n < NW; n++) w[n][i] = x[n];
+        }
+        auto product = [&](int tile, u32x4 a) {
+#pragma unroll
+            for (int n = 0; n < NW; n++)
+                st.acc[tile] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), w[n], st.acc[tile], 0, 0, 0);
+        };
+#pragma unroll
+        for (int p = 0; p < PT::kCount; p++) {
+            const int W = PT::width(p), t0 = PT::base(p) / 16;
+            uint32_t word[8];
+            float vs[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int m = 2 * h + (u >> 2);
+                word[u] = g.v[p][m][u & 3];
+                if (W == 64) word[u] >>= 16 * (r & 1);
+                if (W == 32) word[u] >>= 8 * (r & 3);
+                vs[u] = scale_at(g.vs[p][m], u & 3);
+            }
+#define VL_TWO_TILES(B)                                                                     \
+    if (B < W / 32) {                                                                       \
+        u32x4 even, odd;                                                                    \
+        _Pragma("unroll") for (int i = 0; i < 4; i++) {                                     \
+            const uint32_t x = two_values<B>(word[2 * i], vs[2 * i]);                       \
+            const uint32_t y = two_values<B>(word[2 * i + 1], vs[2 * i + 1]);               \
+            even[i] = __builtin_amdgcn_perm(y, x, 0x05040100);                              \
+            odd[i] = __builtin_amdgcn_perm(y, x, 0x07060302);                               \
+        }                                                                                   \
+        product(t0 + 2 * B, even);                                                          \
+        product(t0 + 2 * B + 1, odd);                                                       \
+    }
+            VL_TWO_TILES(0)
+            VL_TWO_TILES(1)
+            VL_TWO_TILES(2)
+            VL_TWO_TILES(3)
+#undef VL_TWO_TILES
+        }
+    }
+}
+
+// A workgroup has 16 rows of one head and a share of their blocks; its four wavefronts take pages in turn.
+template <int D, int NS>
+__global__ __launch_bounds__(256) void attend_few_kernel(AttendArgs a) {
+    typedef Parts<D> PT;
+    typedef typename ElementOf<NS>::type E;
+    constexpr int kPad = 132;  // a row of 128 sums in LDS: 16 lanes x 4 words of a store lie in 64 banks
+    __shared__ float s_sum[4][16 * kPad];
+    __shared__ float s_top[4][16], s_all[4][16];
+
+    const int h = blockIdx.y, split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits;
+    const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // with a list, a tile is 16 of the queries of one token; without, of all tokens of the sequence
+    Piece w;
+    int token0 = 0, tokens;
+    if (a.list) {
+        const int per = (a.group + 15) / 16, row = tile / per;
+        w = {sequence_of(a.t, row), tile % per};
+        w.sequence = __builtin_amdgcn_readfirstlane(w.sequence);
+        token0 = row - first_row(a.t, w.sequence);
+        tokens = 1;
+    } else if (!a.t.offsets) {
+        const int per = (a.group + 15) / 16;
+        w = {tile / per, tile % per};
+        tokens = 1;
+    } else {
+        w = find_piece(a.t.sequences, tile, [&](int b) { return (int)(((int64_t)row_count(a.t, b) * a.group + 15) / 16); });
+        if (w.sequence < 0) return;
+        tokens = row_count(a.t, w.sequence);
+    }
+    const int b = w.sequence, length = length_of(a.t, b), all = row_count(a.t, b);
+    const int index = w.piece * 16 + r;
+    const bool real = index < tokens * a.group;
+    const int token = token0 + index / a.group, head = h * a.group + index % a.group;
+    const int64_t row = first_row(a.t, b) + (int64_t)token;
+    // tokens that the row sees, and the most that any of the tile does
+    const bool causal = a.causal || a.list;
+    int sees = causal ? min(max((int)min((int64_t)a.t.lengths[b], (int64_t)1 << 30) - all + token + 1, 0), length) : length;
+    if (!real) sees = 0;
+    int most = sees, least = real ? sees : length;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+        most = max(most, __shfl_xor(most, d));
+        least = min(least, __shfl_xor(least, d));
+    }
+    most = __builtin_amdgcn_readfirstlane(most);
+    least = __builtin_amdgcn_readfirstlane(least);
+
+    QueryRegs<D, NS> f;
+    load_queries<D, NS>(f, a, real, row, head);
+    RowState<D> st;
+#pragma unroll
+    for (int k = 0; k < D / 16; k++) st.acc[k] = f32x4{0, 0, 0, 0};
+    st.top = -INFINITY;
+    st.sum = 0;
+
+    const int entries = a.list ? a.count : (most + kPage - 1) / kPage;
+    const int from = (int)((int64_t)entries * split / a.splits), to = (int)((int64_t)entries * (split + 1) / a.splits);
+    const int32_t *const list = a.list ? a.list + ((first_row(a.t, b) + (int64_t)token0) * a.c.heads + h) * a.count : nullptr;
+    for (int i = from + wave; i < to; i += 4) {
+        const int block = list ? list[i] : i;
+        const int64_t page = page_of(a.t, a.c, b, block);
+        if (page < 0 || block * kPage >= most) continue;
+        PageRegs<D> g;
+        load_page<D>(g, a.c, page, h);
+        const bool edge = (block + 1) * kPage > least || a.c.bound_scales[page * a.c.heads + h] == kBoundless;
+        take_page<D, NS>(st, g, f, a.scale, edge, sees - block * kPage, length - block * kPage);
+    }
+
+    // join the four wavefronts, 128 dimensions at a time
+    const float sum = sum_over_quads(st.sum);
+    if (q == 0) {
+        s_top[wave][r] = st.top;
+        s_all[wave][r] = sum;
+    }
+    __syncthreads();
+    const int jr = threadIdx.x >> 4, js = threadIdx.x & 15;  // a thread joins 8 dimensions of row jr
+    float top = s_top[0][jr], weight[4], total = 0;
+#pragma unroll
+    for (int i = 1; i < 4; i++) top = fmaxf(top, s_top[i][jr]);
+    const float base_top = top > -INFINITY ? top : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        weight[i] = __builtin_amdgcn_exp2f(s_top[i][jr] - base_top);
+        total += weight[i] * s_all[i][jr];
+    }
+    const int jindex = w.piece * 16 + jr;
+    const bool jreal = jindex < tokens * a.group;
+    const int64_t out_row = (first_row(a.t, b) + (int64_t)(token0 + jindex / a.group)) * a.heads_q + h * a.group + jindex % a.group;
+#pragma unroll
+    for (int p = 0; p < PT::kCount; p++) {
+        const int W = PT::width(p), t0 = PT::base(p) / 16;
+        if (p) __syncthreads();
+        // lane (q, r) has dimensions q * W / 4 + e * W / 16 + k
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int k = 0; k < W / 16; k++) s_sum[wave][r * kPad + q * (W / 4) + e * (W / 16) + k] = st.acc[t0 + k][e];
+        __syncthreads();
+        if (js * 8 < W && jreal) {
+            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] += weight[i] * s_sum[i][jr * kPad + js * 8 + k];
+            if (a.splits > 1) {
+                float *const to = a.part + (out_row * a.splits + split) * D + PT::base(p) + js * 8;
+#pragma unroll
+                for (int k = 0; k < 8; k++) to[k] = x[k];
+            } else {
+                const float by = total == 0 ? 0.0f : 1.0f / total;
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] *= by;
+                store8<NS>((E *)a.out + out_row * D + PT::base(p) + js * 8, x);
+            }
+        }
+    }
+    if (js == 0 && jreal) {
+        if (a.splits > 1) {
+            float *const to = a.part + (int64_t)a.t.rows * a.heads_q * a.splits * D + (out_row * a.splits + split) * 2;
+            to[0] = top;
+            to[1] = total;
+        } else if (a.lse) {
+            a.lse[out_row] = (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+        }
+    }
+}
+
+// A wavefront joins the splits of one row and head: at most 64, a lane for each one's maximum and sum.
+template <int D, int NS>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
+    typedef typename ElementOf<NS>::type E;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= (int64_t)a.t.rows * a.heads_q) return;
+    const float *const ends = a.part + (int64_t)a.t.rows * a.heads_q * a.splits * D + row * a.splits * 2;
+    float top = lane < a.splits ? ends[lane * 2] : -INFINITY;
+    float sum = lane < a.splits ? ends[lane * 2 + 1] : 0;
+    float most = top;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+    const float weight = __builtin_amdgcn_exp2f(top - (most > -INFINITY ? most : 0.0f));
+    float total = sum * weight;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+    constexpr int kEach = D >= 128 ? D / 64 : 2;  // elements of a lane: 2, 3 or 4
+    const int at = lane * kEach;
+    float x[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; k++) x[k] = 0;
+    for (int s = 0; s < a.splits; s++) {
+        const float by = __shfl(weight, s);
+        if (at < D) {
+#pragma unroll
+            for (int k = 0; k < kEach; k++) x[k] += by * a.part[(row * a.splits + s) * D + at + k];
+        }
+    }
+    const float by = total == 0 ? 0.0f : 1.0f / total;
+    if (at < D) {
+#pragma unroll
+        for (int k = 0; k < kEach; k++) ((E *)a.out)[row * D + at + k] = (E)(x[k] * by);
+    }
+    if (lane == 0 && a.lse) a.lse[row] = (most + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+}
+
+template <int NS>
+int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
+    VL_REQUIRE(tiles * a.splits <= 4 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)(tiles * a.splits));
+    for_dim(a.c.dim, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        attend_few_kernel<D, NS><<<dim3((unsigned)(tiles * a.splits), (unsigned)a.c.heads), 256, 0, stream>>>(a);
+        if (a.splits > 1)
+            attend_join_kernel<D, NS><<<(unsigned)(((int64_t)a.t.rows * a.heads_q + 3) / 4), 256, 0, stream>>>(a);
+    });
+    VL_LAUNCH_CHECK("attend_few_kernel");
+    return VL_OK;
+}

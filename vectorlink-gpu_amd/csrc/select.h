@@ -1,0 +1,16 @@
+// The choice of blocks for every row and head of the cache.
+#pragma once
+#include "cache.h"
+
+struct SelectArgs {
+    CacheView c;
+    Tokens t;
+    const void *queries;
+    int64_t q_row, q_head;
+    int group, aligned;
+    int count;
+    int32_t *out;    // [rows, c.heads, count]
+    uint32_t *keys;  // [rows, c.heads, t.blocks]: scores, in an order that unsigned numbers have
+};
+int64_t select_workspace_bytes(const SelectArgs &a);
+int launch_select(const SelectArgs &a, int type, hipStream_t stream);

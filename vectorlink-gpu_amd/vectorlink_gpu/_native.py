@@ -23,6 +23,23 @@ class BeamParams(C.Structure):
         "flags", "metric")]
 
 
+class Cache(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("pages", "heads", "dim")] + [(n, C.c_void_p) for n in (
+        "keys", "key_scales", "values", "value_scales", "bounds", "bound_scales")]
+
+
+class Tokens(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("rows", "sequences", "blocks", "table_stride")] + [
+        (n, C.c_void_p) for n in ("table", "lengths", "offsets")]
+
+
+class Queries(C.Structure):
+    _fields_ = [("heads", C.c_int64), ("row_stride", C.c_int64), ("head_stride", C.c_int64), ("queries", C.c_void_p),
+                ("out", C.c_void_p), ("lse", C.c_void_p), ("scale", C.c_double), ("type", C.c_int32), ("causal", C.c_int32)]
+
+
+TYPES = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}  # VL_BF16, VL_F16, VL_F32
+ATTEND_FORMS = {"few": 0, "many": 1}  # VL_ATTEND_FEW, VL_ATTEND_MANY
 METRICS = {"cosine": 0, "l2": 1}  # include/vlgpu.h: VL_METRIC_COSINE, VL_METRIC_L2
 KNN_FORMS = {"tiles": 0, "few": 1, "filter": 2}  # VL_KNN_TILES, VL_KNN_FEW, VL_KNN_FILTER
 KNN_ANY_SIZE = 256  # VL_KNN_ANY_SIZE
@@ -76,6 +93,18 @@ _SIGNATURES = {
     "vl_knn_left_offset": (C.c_int64, [_i64, _i64, _i64, _i64, C.c_int32, _i64]),
     "vl_knn_exact": (C.c_int, [_ptr, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _i64, _ptr]),
     "vl_knn_exact_metric": (C.c_int, [_ptr, _i64, _ptr, _i64, _i64, _i64, C.c_int32, _ptr, _ptr, _ptr, _i64, _ptr]),
+    "vl_cache_write": (C.c_int, [_ptr, _ptr, C.c_int, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr]),
+    "vl_cache_read": (C.c_int, [_ptr, _ptr, C.c_int, _ptr, _ptr, _ptr]),
+    "vl_cache_read_bounds": (C.c_int, [_ptr, _ptr, _i64, _ptr, _ptr]),
+    "vl_attend_workspace_bytes": (C.c_int64, [_ptr, _ptr, _ptr]),
+    "vl_attend_form": (C.c_int, [_ptr, _ptr, _ptr]),
+    "vl_attend": (C.c_int, [_ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
+    "vl_select_blocks_workspace_bytes": (C.c_int64, [_ptr, _ptr, _ptr, _i64]),
+    "vl_select_blocks": (C.c_int, [_ptr, _ptr, _ptr, _i64, _ptr, _ptr, _i64, _ptr]),
+    "vl_attend_blocks_workspace_bytes": (C.c_int64, [_ptr, _ptr, _ptr, _i64]),
+    "vl_attend_blocks": (C.c_int, [_ptr, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _ptr]),
+    "vl_attend_selected_workspace_bytes": (C.c_int64, [_ptr, _ptr, _ptr, _i64]),
+    "vl_attend_selected": (C.c_int, [_ptr, _ptr, _ptr, _i64, _ptr, _ptr, _i64, _ptr]),
     "vl_prune": (C.c_int, [_ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr]),
 }
 
