@@ -24,6 +24,13 @@ constexpr int kMaxSplits = 64;
 // 16 rows at a time, the tokens split over wavefronts and workgroups
 template <int NS>
 int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream);
+// 32 rows a wavefront, all of a workgroup's on the same pages: 8 wavefronts, or 4 where a row's registers are many
+constexpr int many_waves(int dim, int parts) { return dim <= 128 && dim * parts <= 256 ? 8 : 4; }
+template <int NS>
+int launch_attend_many(const AttendArgs &a, int64_t tiles, hipStream_t stream);
 extern template int launch_attend_few<1>(const AttendArgs &, int64_t, hipStream_t);
 extern template int launch_attend_few<2>(const AttendArgs &, int64_t, hipStream_t);
 extern template int launch_attend_few<3>(const AttendArgs &, int64_t, hipStream_t);
+extern template int launch_attend_many<1>(const AttendArgs &, int64_t, hipStream_t);
+extern template int launch_attend_many<2>(const AttendArgs &, int64_t, hipStream_t);
+extern template int launch_attend_many<3>(const AttendArgs &, int64_t, hipStream_t);

@@ -7,6 +7,9 @@
 
 namespace {
 
+// From so many rows a sequence on (queries that share a head counted each) the form that shares a page among them is the faster.
+constexpr int kManyRows = 256;
+
 int attend_args(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *q, bool data, AttendArgs *a) {
     *a = {};
     int rc = vl_cache_of(cache, &a->c);
@@ -32,7 +35,8 @@ int attend_args(const vl_cache *cache, const vl_tokens *tokens, const vl_queries
     a->group = (int)(q->heads / a->c.heads);
     a->causal = q->causal != 0;
     a->aligned = ((uintptr_t)q->queries & 15) == 0 && q->row_stride * size % 16 == 0 && q->head_stride * size % 16 == 0;
-    a->scale = (float)(fabs(q->scale) * 1.4426950408889634);
+    // 0 becomes a scale that leaves all scores 0 after rounding but for those that a mask sets to -inf
+    a->scale = (float)fmax(fabs(q->scale) * 1.4426950408889634, 1e-37);
     a->sign = q->scale < 0 ? 0x80000000u : 0;
     a->splits = 1;
     return VL_OK;
@@ -60,17 +64,48 @@ int64_t part_bytes(const AttendArgs &a, int splits) {
     return ((int64_t)a.t.rows * a.heads_q * splits * (a.c.dim + 2) * 4 + 255) / 256 * 256;
 }
 
-int attend_few(AttendArgs &a, int type, void *workspace, int64_t bytes, hipStream_t stream) {
-    const int64_t tiles = few_tiles(a);
-    a.splits = splits_for(a, tiles);
-    const int64_t need = part_bytes(a, a.splits);
+// Tiles of the rows of a workgroup of attend_many_kernel
+int many_rows(const AttendArgs &a, int type) { return 32 * many_waves(a.c.dim, type); }
+int64_t many_tiles(const AttendArgs &a, int type) { return (int64_t)a.t.rows * a.group / many_rows(a, type) + a.t.sequences; }
+
+bool takes_many(const AttendArgs &a, int type) {
+    return a.t.offsets && (int64_t)a.t.rows * a.group >= (int64_t)kManyRows * a.t.sequences;
+}
+
+// Workgroups that share a tile's tokens: enough for one on every compute unit, but eight pages for each.
+int many_splits(const AttendArgs &a, int64_t tiles) {
+    const int64_t items = tiles * a.c.heads;
+    if (items == 0) return 1;
+    int64_t s = kComputeUnits / items;
+    s = s < a.t.blocks / 8 ? s : a.t.blocks / 8;
+    return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+}
+
+int check_workspace(int64_t need, const void *workspace, int64_t bytes) {
     if (need > bytes || (need && !workspace)) {
         vl_set_error("workspace too small: %lld bytes needed, %lld given", (long long)need, (long long)bytes);
         return VL_ERR_WORKSPACE;
     }
     VL_REQUIRE(((uintptr_t)workspace & 15) == 0, "workspace not on a 16-byte boundary");
+    return VL_OK;
+}
+
+int attend_few(AttendArgs &a, int type, void *workspace, int64_t bytes, hipStream_t stream) {
+    const int64_t tiles = few_tiles(a);
+    a.splits = splits_for(a, tiles);
+    const int rc = check_workspace(part_bytes(a, a.splits), workspace, bytes);
+    if (rc != VL_OK) return rc;
     a.part = (float *)workspace;
     return type == VL_BF16 ? launch_attend_few<1>(a, tiles, stream) : type == VL_F16 ? launch_attend_few<2>(a, tiles, stream) : launch_attend_few<3>(a, tiles, stream);
+}
+
+int attend_many(AttendArgs &a, int type, void *workspace, int64_t bytes, hipStream_t stream) {
+    const int64_t tiles = many_tiles(a, type);
+    a.splits = many_splits(a, tiles);
+    const int rc = check_workspace(part_bytes(a, a.splits), workspace, bytes);
+    if (rc != VL_OK) return rc;
+    a.part = (float *)workspace;
+    return type == VL_BF16 ? launch_attend_many<1>(a, tiles, stream) : type == VL_F16 ? launch_attend_many<2>(a, tiles, stream) : launch_attend_many<3>(a, tiles, stream);
 }
 
 int check_count(int64_t count) {
@@ -84,11 +119,8 @@ SelectArgs select_args(const AttendArgs &a, int64_t count) {
 
 int choose(const AttendArgs &a, int type, int64_t count, int32_t *blocks, void *workspace, int64_t bytes, hipStream_t stream) {
     SelectArgs s = select_args(a, count);
-    const int64_t need = select_workspace_bytes(s);
-    if (need > bytes || (need && !workspace)) {
-        vl_set_error("workspace too small: %lld bytes needed, %lld given", (long long)need, (long long)bytes);
-        return VL_ERR_WORKSPACE;
-    }
+    const int rc = check_workspace(select_workspace_bytes(s), workspace, bytes);
+    if (rc != VL_OK) return rc;
     VL_REQUIRE(blocks, "blocks is null");
     s.out = blocks;
     s.keys = (uint32_t *)workspace;
@@ -100,13 +132,15 @@ int choose(const AttendArgs &a, int type, int64_t count, int32_t *blocks, void *
 VL_EXPORT int vl_attend_form(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries) {
     AttendArgs a;
     const int rc = attend_args(cache, tokens, queries, false, &a);
-    return rc != VL_OK ? rc : VL_ATTEND_FEW;
+    return rc != VL_OK ? rc : takes_many(a, queries->type) ? VL_ATTEND_MANY : VL_ATTEND_FEW;
 }
 
 VL_EXPORT int64_t vl_attend_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries) {
     AttendArgs a;
     const int rc = attend_args(cache, tokens, queries, false, &a);
-    return rc != VL_OK ? rc : part_bytes(a, splits_for(a, few_tiles(a)));
+    if (rc != VL_OK) return rc;
+    if (takes_many(a, queries->type)) return part_bytes(a, many_splits(a, many_tiles(a, queries->type)));
+    return part_bytes(a, splits_for(a, few_tiles(a)));
 }
 
 VL_EXPORT int vl_attend(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries, void *workspace,
@@ -114,7 +148,8 @@ VL_EXPORT int vl_attend(const vl_cache *cache, const vl_tokens *tokens, const vl
     AttendArgs a;
     const int rc = attend_args(cache, tokens, queries, true, &a);
     if (rc != VL_OK || a.t.rows == 0) return rc;
-    return attend_few(a, queries->type, workspace, workspace_bytes, (hipStream_t)stream);
+    return takes_many(a, queries->type) ? attend_many(a, queries->type, workspace, workspace_bytes, (hipStream_t)stream)
+                                        : attend_few(a, queries->type, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 VL_EXPORT int64_t vl_select_blocks_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,

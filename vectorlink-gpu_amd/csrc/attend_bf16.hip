@@ -1,4 +1,5 @@
-// Attention of a few rows: queries of type bf16.
-#include "attend_few.h"
+// Attention with queries of type bf16.
+#include "attend_launch.h"
 
 template int launch_attend_few<1>(const AttendArgs &, int64_t, hipStream_t);
+template int launch_attend_many<1>(const AttendArgs &, int64_t, hipStream_t);

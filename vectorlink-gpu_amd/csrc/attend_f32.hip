@@ -1,4 +1,5 @@
-// Attention of a few rows: queries of type f32.
-#include "attend_few.h"
+// Attention with queries of type f32.
+#include "attend_launch.h"
 
 template int launch_attend_few<3>(const AttendArgs &, int64_t, hipStream_t);
+template int launch_attend_many<3>(const AttendArgs &, int64_t, hipStream_t);

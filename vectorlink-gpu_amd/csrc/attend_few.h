@@ -401,16 +401,3 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
     }
     if (lane == 0 && a.lse) a.lse[row] = (most + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
 }
-
-template <int NS>
-int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
-    VL_REQUIRE(tiles * a.splits <= 4 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)(tiles * a.splits));
-    for_dim(a.c.dim, [&](auto d) {
-        constexpr int D = decltype(d)::value;
-        attend_few_kernel<D, NS><<<dim3((unsigned)(tiles * a.splits), (unsigned)a.c.heads), 256, 0, stream>>>(a);
-        if (a.splits > 1)
-            attend_join_kernel<D, NS><<<(unsigned)(((int64_t)a.t.rows * a.heads_q + 3) / 4), 256, 0, stream>>>(a);
-    });
-    VL_LAUNCH_CHECK("attend_few_kernel");
-    return VL_OK;
-}

@@ -1,0 +1,39 @@
+// Launchers of the kernels of one type of queries.
+#pragma once
+#include "attend_few.h"
+#include "attend_many.h"
+
+template <int D, int NS>
+void launch_join(const AttendArgs &a, hipStream_t stream) {
+    if (a.splits > 1) attend_join_kernel<D, NS><<<(unsigned)(((int64_t)a.t.rows * a.heads_q + 3) / 4), 256, 0, stream>>>(a);
+}
+
+template <int NS>
+int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
+    VL_REQUIRE(tiles * a.splits <= 4 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)(tiles * a.splits));
+    for_dim(a.c.dim, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        attend_few_kernel<D, NS><<<dim3((unsigned)(tiles * a.splits), (unsigned)a.c.heads), 256, 0, stream>>>(a);
+        launch_join<D, NS>(a, stream);
+    });
+    VL_LAUNCH_CHECK("attend_few_kernel");
+    return VL_OK;
+}
+
+template <int NS>
+int launch_attend_many(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
+    const int64_t groups = tiles * a.splits * a.c.heads;
+    VL_REQUIRE(groups <= 2 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)groups);
+    hipError_t e = hipSuccess;
+    for_dim(a.c.dim, [&](auto d) {
+        constexpr int D = decltype(d)::value, W = many_waves(D, NS);
+        constexpr size_t lds = 2 * (Images<D>::kBytes + kPage);
+        e = vl_allow_lds(attend_many_kernel<D, NS, W>, lds);
+        if (e != hipSuccess) return;
+        attend_many_kernel<D, NS, W><<<(unsigned)groups, W * 64, lds, stream>>>(a, (int)tiles);
+        launch_join<D, NS>(a, stream);
+    });
+    VL_HIP(e);
+    VL_LAUNCH_CHECK("attend_many_kernel");
+    return VL_OK;
+}

@@ -142,7 +142,8 @@ def ptr(t) -> C.c_void_p:
 
 def stream() -> C.c_void_p:
     """The current torch stream as a hipStream_t (kernels.py:14-16 does the same for Numba)."""
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # what torch.cuda.current_stream().cuda_stream is, without making two objects of it (0.2 us, not 2.5)
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 def require_gpu(*tensors):

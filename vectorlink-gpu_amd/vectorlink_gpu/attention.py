@@ -22,28 +22,25 @@ PAGE = 64  # tokens
 DIMS = (32, 64, 96, 128, 192, 256)
 
 
-def _check_int32(t: Tensor, name: str, size: int):
-    assert t.dtype == torch.int32, f"{name} must be int32"
-    assert t.dim() == 1 and t.numel() == size and (size < 2 or t.stride(0) == 1), f"{name} must be a contiguous tensor of {size}"
-
-
 def _tokens(rows: int, table: Tensor, lengths: Tensor, offsets: Optional[Tensor]) -> nv.Tokens:
     assert table.dtype == torch.int32 and table.dim() == 2, "table must be int32 [sequences, blocks]"
-    (sequences, blocks) = table.size()
-    assert blocks < 2 or table.stride(1) == 1, "rows of table must be contiguous"
-    _check_int32(lengths, "lengths", sequences)
+    (sequences, blocks) = table.shape
+    (stride, one) = table.stride()
+    assert one == 1 or blocks < 2, "rows of table must be contiguous"
+    assert lengths.dtype == torch.int32 and lengths.shape == (sequences,) and lengths.is_contiguous(), \
+        f"lengths must be a contiguous int32 tensor of {sequences}"
     if offsets is None:
         assert rows == sequences, f"without offsets every sequence has one row: {rows} rows, {sequences} sequences"
-        nv.require_gpu(table, lengths)
+        at = None
     else:
-        _check_int32(offsets, "offsets", sequences + 1)
-        nv.require_gpu(table, lengths, offsets)
-    return nv.Tokens(rows, sequences, blocks, table.stride(0) if sequences > 1 else blocks, table.data_ptr(), lengths.data_ptr(),
-                     None if offsets is None else offsets.data_ptr())
+        assert offsets.dtype == torch.int32 and offsets.shape == (sequences + 1,) and offsets.is_contiguous(), \
+            f"offsets must be a contiguous int32 tensor of {sequences + 1}"
+        at = offsets.data_ptr()
+    return nv.Tokens(rows, sequences, blocks, stride if sequences > 1 else blocks, table.data_ptr(), lengths.data_ptr(), at)
 
 
 def _check_rows(t: Tensor, name: str, dim: int) -> int:
-    assert t.dim() == 3 and t.size(2) == dim, f"{name} must be [rows, heads, {dim}]"
+    assert t.dim() == 3 and t.shape[2] == dim, f"{name} must be [rows, heads, {dim}]"
     assert t.stride(2) == 1, f"the last dimension of {name} must be contiguous"
     assert t.dtype in nv.TYPES, f"{name} must be bfloat16, float16 or float32"
     return nv.TYPES[t.dtype]
@@ -89,10 +86,10 @@ class KVCache:
         """Quantise keys and values [rows, heads, dim] behind the `starts` [sequences] tokens that the sequences hold, and make
         the bounds of the blocks written into anew.  Writing again at an earlier place is allowed and takes back what was behind."""
         kind = _check_rows(keys, "keys", self.dim)
-        assert _check_rows(values, "values", self.dim) == kind and values.size() == keys.size(), "keys and values differ in type or size"
-        assert keys.size(1) == self.heads, f"keys have {keys.size(1)} heads, the cache {self.heads}"
-        tokens = _tokens(keys.size(0), table, starts, offsets)
-        nv.require_gpu(keys, values)
+        assert _check_rows(values, "values", self.dim) == kind and values.shape == keys.shape, "keys and values differ in type or size"
+        assert keys.shape[1] == self.heads, f"keys have {keys.shape[1]} heads, the cache {self.heads}"
+        tokens = _tokens(keys.shape[0], table, starts, offsets)
+        nv.require_gpu(keys, values, table, starts, offsets)
         nv.check(nv.lib().vl_cache_write(self._ref, C.byref(tokens), kind, keys.data_ptr(), keys.stride(0), keys.stride(1),
                                          values.data_ptr(), values.stride(0), values.stride(1), nv.stream()))
 
@@ -102,6 +99,7 @@ class KVCache:
         there, rounded.  rows is the last of offsets, or the number of sequences."""
         assert dtype in nv.TYPES, "dtype must be bfloat16, float16 or float32"
         tokens = _tokens(rows, table, starts, offsets)
+        nv.require_gpu(table, starts, offsets)
         keys = torch.empty((rows, self.heads, self.dim), dtype=dtype, device=self.keys.device)
         values = torch.empty_like(keys)
         nv.check(nv.lib().vl_cache_read(self._ref, C.byref(tokens), nv.TYPES[dtype], keys.data_ptr(), values.data_ptr(), nv.stream()))
@@ -117,38 +115,22 @@ class KVCache:
         return out
 
 
-class _Call:
-    """The checked arguments of a call with queries, as the library takes them."""
+def _queries(queries: Tensor, cache: KVCache, scale: Optional[float], causal: bool, out: Optional[Tensor],
+             lse: Optional[Tensor]) -> nv.Queries:
+    (row, head, _) = queries.stride()
+    return nv.Queries(queries.shape[1], row, head, queries.data_ptr(), None if out is None else out.data_ptr(),
+                      None if lse is None else lse.data_ptr(), cache.dim ** -0.5 if scale is None else scale,
+                      nv.TYPES[queries.dtype], causal)
 
-    def __init__(self, queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, offsets: Optional[Tensor],
-                 scale: Optional[float] = None, causal: bool = True, output: bool = True, lse: bool = False):
-        kind = _check_rows(queries, "queries", cache.dim)
-        (rows, heads, dim) = queries.size()
-        assert heads > 0 and heads % cache.heads == 0, f"{heads} heads of queries for {cache.heads} of the cache"
-        self.tokens = _tokens(rows, table, lengths, offsets)
-        nv.require_gpu(queries)
-        self.out = torch.empty((rows, heads, dim), dtype=queries.dtype, device=queries.device) if output else None
-        self.lse = torch.empty((rows, heads), dtype=torch.float32, device=queries.device) if lse else None
-        self.native = nv.Queries(heads, queries.stride(0), queries.stride(1), queries.data_ptr(),
-                                 self.out.data_ptr() if output else None, self.lse.data_ptr() if lse else None,
-                                 dim ** -0.5 if scale is None else scale, kind, int(causal))
-        self.args = (cache._ref, C.byref(self.tokens), C.byref(self.native))
-        self.device = queries.device
 
-    def workspace(self, need: int):
-        """(pointer, bytes), kept with the call"""
-        need = nv.check(need)
-        if need == 0:
-            return (None, 0)
-        self.scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
-        return (self.scratch.data_ptr(), need)
+def _check_queries(queries: Tensor, cache: KVCache):
+    _check_rows(queries, "queries", cache.dim)
+    heads = queries.shape[1]
+    assert heads > 0 and heads % cache.heads == 0, f"{heads} heads of queries for {cache.heads} of the cache"
 
-    def blocks(self, cache: KVCache, count: int) -> Tensor:
-        assert count >= 1, f"count: {count}"
-        return torch.empty((self.tokens.rows, cache.heads, count), dtype=torch.int32, device=self.device)
 
-    def result(self):
-        return self.out if self.lse is None else (self.out, self.lse)
+def _workspace(need: int, beside: Tensor) -> Optional[Tensor]:
+    return beside.new_empty(nv.check(need), dtype=torch.uint8) if need else None
 
 
 def attend(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, offsets: Optional[Tensor] = None,
@@ -157,46 +139,69 @@ def attend(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, offs
     dim], heads a multiple of the cache's; scale defaults to dim ** -0.5.  The rows of a sequence are its last tokens and see
     what stands before them and themselves, or with causal=False everything.  A row that sees nothing gives zeros.  With
     return_lse also the logarithms of the sums of exponentials [rows, heads], by which parts of an attention are joined."""
-    call = _Call(queries, cache, table, lengths, offsets, scale, causal, lse=return_lse)
+    tokens = C.byref(_tokens(queries.shape[0], table, lengths, offsets))
+    _check_queries(queries, cache)
+    nv.require_gpu(queries, table, lengths, offsets)
+    out = queries.new_empty(queries.shape)
+    lse = queries.new_empty(queries.shape[:2], dtype=torch.float32) if return_lse else None
+    q = C.byref(_queries(queries, cache, scale, causal, out, lse))
     lib = nv.lib()
-    ws = call.workspace(lib.vl_attend_workspace_bytes(*call.args))
-    nv.check(lib.vl_attend(*call.args, *ws, nv.stream()))
-    return call.result()
+    need = lib.vl_attend_workspace_bytes(cache._ref, tokens, q)
+    ws = _workspace(need, queries)
+    nv.check(lib.vl_attend(cache._ref, tokens, q, nv.ptr(ws), need, nv.stream()))
+    return (out, lse) if return_lse else out
 
 
 def select_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, count: int,
                   offsets: Optional[Tensor] = None) -> Tensor:
     """For every row and head of the cache `count` blocks of its sequence, ascending: the row's own and those with the highest
     upper bound on a score in them, by queries and bounds of 8 bits; MAXINT where there are no more.  [rows, cache.heads, count]"""
-    call = _Call(queries, cache, table, lengths, offsets, output=False)
+    assert count >= 1, f"count: {count}"
+    tokens = C.byref(_tokens(queries.shape[0], table, lengths, offsets))
+    _check_queries(queries, cache)
+    nv.require_gpu(queries, table, lengths, offsets)
+    blocks = table.new_empty((queries.shape[0], cache.heads, count))
+    q = C.byref(_queries(queries, cache, None, True, None, None))
     lib = nv.lib()
-    blocks = call.blocks(cache, count)
-    ws = call.workspace(lib.vl_select_blocks_workspace_bytes(*call.args, count))
-    nv.check(lib.vl_select_blocks(*call.args, count, blocks.data_ptr(), *ws, nv.stream()))
+    need = lib.vl_select_blocks_workspace_bytes(cache._ref, tokens, q, count)
+    ws = _workspace(need, queries)
+    nv.check(lib.vl_select_blocks(cache._ref, tokens, q, count, blocks.data_ptr(), nv.ptr(ws), need, nv.stream()))
     return blocks
 
 
 def attend_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, blocks: Tensor,
                   offsets: Optional[Tensor] = None, scale: Optional[float] = None, return_lse: bool = False):
     """attend over the tokens of blocks [rows, cache.heads, count] alone, up to the row's own place."""
-    call = _Call(queries, cache, table, lengths, offsets, scale, lse=return_lse)
+    tokens = C.byref(_tokens(queries.shape[0], table, lengths, offsets))
+    _check_queries(queries, cache)
+    nv.require_gpu(queries, table, lengths, offsets)
     assert blocks.dtype == torch.int32 and blocks.is_contiguous(), "blocks must be contiguous int32"
-    assert blocks.dim() == 3 and blocks.size(0) == queries.size(0) and blocks.size(1) == cache.heads and blocks.size(2) > 0, \
+    assert blocks.dim() == 3 and blocks.shape[:2] == (queries.shape[0], cache.heads) and blocks.shape[2] > 0, \
         "blocks must be [rows, cache.heads, count]"
     nv.require_gpu(blocks)
+    count = blocks.shape[2]
+    out = queries.new_empty(queries.shape)
+    lse = queries.new_empty(queries.shape[:2], dtype=torch.float32) if return_lse else None
+    q = C.byref(_queries(queries, cache, scale, True, out, lse))
     lib = nv.lib()
-    count = blocks.size(2)
-    ws = call.workspace(lib.vl_attend_blocks_workspace_bytes(*call.args, count))
-    nv.check(lib.vl_attend_blocks(*call.args, blocks.data_ptr(), count, *ws, nv.stream()))
-    return call.result()
+    need = lib.vl_attend_blocks_workspace_bytes(cache._ref, tokens, q, count)
+    ws = _workspace(need, queries)
+    nv.check(lib.vl_attend_blocks(cache._ref, tokens, q, blocks.data_ptr(), count, nv.ptr(ws), need, nv.stream()))
+    return (out, lse) if return_lse else out
 
 
 def attend_selected(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, count: int,
                     offsets: Optional[Tensor] = None, scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
     """(attend_blocks(...), blocks) with the blocks of select_blocks, in one call."""
-    call = _Call(queries, cache, table, lengths, offsets, scale)
+    assert count >= 1, f"count: {count}"
+    tokens = C.byref(_tokens(queries.shape[0], table, lengths, offsets))
+    _check_queries(queries, cache)
+    nv.require_gpu(queries, table, lengths, offsets)
+    blocks = table.new_empty((queries.shape[0], cache.heads, count))
+    out = queries.new_empty(queries.shape)
+    q = C.byref(_queries(queries, cache, scale, True, out, None))
     lib = nv.lib()
-    blocks = call.blocks(cache, count)
-    ws = call.workspace(lib.vl_attend_selected_workspace_bytes(*call.args, count))
-    nv.check(lib.vl_attend_selected(*call.args, count, blocks.data_ptr(), *ws, nv.stream()))
-    return (call.out, blocks)
+    need = lib.vl_attend_selected_workspace_bytes(cache._ref, tokens, q, count)
+    ws = _workspace(need, queries)
+    nv.check(lib.vl_attend_selected(cache._ref, tokens, q, count, blocks.data_ptr(), nv.ptr(ws), need, nv.stream()))
+    return (out, blocks)
