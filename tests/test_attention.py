@@ -77,7 +77,7 @@ def test_rows_that_are_written_or_read_are_checked(lib):
 
 
 def test_workspaces_are_checked(lib):
-    t = tokens(blocks=400, table_stride=400)
+    t = tokens(blocks=40_000, table_stride=40_000)
     sizes = [(lib.vl_attend_workspace_bytes(cache(), t, queries()), lambda n: lib.vl_attend(cache(), t, queries(), 256, n, None)),
              (lib.vl_select_blocks_workspace_bytes(cache(), t, queries(), 4),
               lambda n: lib.vl_select_blocks(cache(), t, queries(), 4, 256, 256, n, None)),

@@ -1,6 +1,6 @@
 // Attention over the cache: what its kernels and their launchers share.
 #pragma once
-#include "cache.h"
+#include "select.h"
 
 // S = scale <query, key>, P = softmax of S over the tokens that a row sees, out = P values.
 struct AttendArgs {
@@ -13,10 +13,10 @@ struct AttendArgs {
     const int32_t *list;    // [rows, c.heads, count] blocks of every row and head, or null: all blocks
     int count;
     int group, heads_q;     // queries that share a head of the cache; c.heads * group
-    int causal, aligned;
+    int causal;
     float scale;            // |scale| log2(e): exponentials are powers of two here
     uint32_t sign;          // 0x80000000 where the scale is negative: turns the queries' sign
-    int splits;
+    int splits;             // workgroups that share a tile of attend_few_kernel; 0: a wavefront has a tile
     float *part;            // splits > 1: [rows * heads_q, splits, D] sums, then [rows * heads_q, splits, 2] maxima and sums of weights
 };
 constexpr int kMaxSplits = 64;
@@ -28,9 +28,15 @@ int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream);
 constexpr int many_waves(int dim, int parts) { return dim <= 128 && dim * parts <= 256 ? 8 : 4; }
 template <int NS>
 int launch_attend_many(const AttendArgs &a, int64_t tiles, hipStream_t stream);
+// a choice of blocks and attention over it, a workgroup for a token and head
+template <int NS>
+int launch_attend_step(const AttendArgs &a, const SelectArgs &s, hipStream_t stream);
 extern template int launch_attend_few<1>(const AttendArgs &, int64_t, hipStream_t);
 extern template int launch_attend_few<2>(const AttendArgs &, int64_t, hipStream_t);
 extern template int launch_attend_few<3>(const AttendArgs &, int64_t, hipStream_t);
 extern template int launch_attend_many<1>(const AttendArgs &, int64_t, hipStream_t);
 extern template int launch_attend_many<2>(const AttendArgs &, int64_t, hipStream_t);
 extern template int launch_attend_many<3>(const AttendArgs &, int64_t, hipStream_t);
+extern template int launch_attend_step<1>(const AttendArgs &, const SelectArgs &, hipStream_t);
+extern template int launch_attend_step<2>(const AttendArgs &, const SelectArgs &, hipStream_t);
+extern template int launch_attend_step<3>(const AttendArgs &, const SelectArgs &, hipStream_t);

@@ -3,12 +3,16 @@
 
 #include <math.h>
 
-#include "select.h"
 
 namespace {
 
 // From so many rows a sequence on (queries that share a head counted each) the form that shares a page among them is the faster.
 constexpr int kManyRows = 256;
+// Tokens times heads up to which one launch for a choice and its attention is the faster: a workgroup for each compute unit (512
+// workgroups over 8,192 tokens each: 56 us, in several launches 45; 128 over 131,072: 46 and 57).  A compute unit alone reads about
+// 25 GB/s, so few workgroups take it for few bytes each (8 over 32,768 tokens, 0.4 MB each: 24 and 29 us; over 131,072, 0.8
+// MB: 39 and 28).
+constexpr int64_t kStepItems = 256, kStepBytes = 1 << 19, kStepFull = 64;
 
 int attend_args(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *q, bool data, AttendArgs *a) {
     *a = {};
@@ -34,7 +38,6 @@ int attend_args(const vl_cache *cache, const vl_tokens *tokens, const vl_queries
     a->heads_q = (int)q->heads;
     a->group = (int)(q->heads / a->c.heads);
     a->causal = q->causal != 0;
-    a->aligned = ((uintptr_t)q->queries & 15) == 0 && q->row_stride * size % 16 == 0 && q->head_stride * size % 16 == 0;
     // 0 becomes a scale that leaves all scores 0 after rounding but for those that a mask sets to -inf
     a->scale = (float)fmax(fabs(q->scale) * 1.4426950408889634, 1e-37);
     a->sign = q->scale < 0 ? 0x80000000u : 0;
@@ -49,12 +52,15 @@ int64_t few_tiles(const AttendArgs &a) {
     return (int64_t)a.t.rows * a.group / 16 + a.t.sequences;
 }
 
-// Workgroups that the tokens of a tile are split over: enough for four on every compute unit, but a page for every wavefront.
+// Workgroups that the tokens of a tile are split over: enough for the two that a compute unit holds at once, but a page for every
+// wavefront.  More cost their starts and ends (64 tokens over 4,096 to 8,192: 92 us with 512 workgroups, 98 with 1,024, 123 with
+// 4,096).  0, a tile for every wavefront, where that alone gives every SIMD two.
 int splits_for(const AttendArgs &a, int64_t tiles) {
     const int64_t entries = a.count ? a.count : a.t.blocks;
     const int64_t items = tiles * a.c.heads;
     if (items == 0) return 1;
-    int64_t s = (4 * kComputeUnits + items - 1) / items;
+    if (items >= 8 * kComputeUnits) return 0;
+    int64_t s = (2 * kComputeUnits + items - 1) / items;
     s = s < (entries + 3) / 4 ? s : (entries + 3) / 4;
     return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
 }
@@ -114,7 +120,7 @@ int check_count(int64_t count) {
 }
 
 SelectArgs select_args(const AttendArgs &a, int64_t count) {
-    return {a.c, a.t, a.queries, a.q_row, a.q_head, a.group, a.aligned, (int)count, nullptr, nullptr};
+    return {a.c, a.t, a.queries, a.q_row, a.q_head, a.group, (int)count, nullptr, nullptr};
 }
 
 int choose(const AttendArgs &a, int type, int64_t count, int32_t *blocks, void *workspace, int64_t bytes, hipStream_t stream) {
@@ -125,6 +131,13 @@ int choose(const AttendArgs &a, int type, int64_t count, int32_t *blocks, void *
     s.out = blocks;
     s.keys = (uint32_t *)workspace;
     return launch_select(s, type, stream);
+}
+
+// Whether attend_step_kernel takes a choice and the attention over it: few tokens, and for one workgroup not too many bytes.
+bool in_one_step(const AttendArgs &a, int64_t count) {
+    const int64_t items = (int64_t)a.t.rows * a.c.heads, bytes = (int64_t)a.t.blocks * 2 * a.c.dim + count * kPage * (a.c.dim + a.c.dim / 16);
+    return a.group <= 16 && a.t.blocks <= 16384 && count <= 2048 && items <= kStepItems &&
+           (bytes <= kStepBytes || items >= kStepFull);
 }
 
 }  // namespace
@@ -197,6 +210,7 @@ VL_EXPORT int64_t vl_attend_selected_workspace_bytes(const vl_cache *cache, cons
     int rc = attend_args(cache, tokens, queries, false, &a);
     if (rc == VL_OK) rc = check_count(count);
     if (rc != VL_OK) return rc;
+    if (in_one_step(a, count)) return 0;
     a.count = (int)count;
     return select_workspace_bytes(select_args(a, count)) + part_bytes(a, splits_for(a, few_tiles(a)));
 }
@@ -207,6 +221,13 @@ VL_EXPORT int vl_attend_selected(const vl_cache *cache, const vl_tokens *tokens,
     int rc = attend_args(cache, tokens, queries, true, &a);
     if (rc == VL_OK) rc = check_count(count);
     if (rc != VL_OK || a.t.rows == 0) return rc;
+    if (in_one_step(a, count)) {
+        VL_REQUIRE(blocks, "blocks is null");
+        SelectArgs s = select_args(a, count);
+        s.out = blocks;
+        const hipStream_t at = (hipStream_t)stream;
+        return queries->type == VL_BF16 ? launch_attend_step<1>(a, s, at) : queries->type == VL_F16 ? launch_attend_step<2>(a, s, at) : launch_attend_step<3>(a, s, at);
+    }
     rc = choose(a, queries->type, count, blocks, workspace, workspace_bytes, (hipStream_t)stream);
     if (rc != VL_OK) return rc;
     const int64_t used = select_workspace_bytes(select_args(a, count));

@@ -109,20 +109,21 @@ __device__ inline void load_queries(QueryRegs<D, NS> &f, const AttendArgs &a, bo
     typedef typename ElementOf<NS>::type E;
     const int q = (threadIdx.x & 63) >> 4;
     const E *const at = (const E *)a.queries + (real ? row * a.q_row + head * a.q_head : 0);
+    Eight<NS> x[D / 32];
 #pragma unroll
     for (int p = 0; p < PT::kCount; p++) {
         const int W = PT::width(p), base = PT::base(p);
 #pragma unroll
-        for (int j = 0; j < W / 32; j++) {
-            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (real) load8<NS>(at + base + q * (W / 4) + j * 8, a.aligned, x);
+        for (int j = 0; j < W / 32; j++) x[base / 32 + j] = load8<NS>(at + base + q * (W / 4) + j * 8, real);
+    }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                __bf16 s[NS];
-                split_into<NS>(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[i]) ^ a.sign), s);
+    for (int k = 0; k < D / 32; k++) {
 #pragma unroll
-                for (int n = 0; n < NS; n++) f.x[n][base / 32 + j][i] = s[n];
-            }
+        for (int i = 0; i < 8; i++) {
+            __bf16 s[NS];
+            split_into<NS>(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)x[k][i]) ^ a.sign), s);
+#pragma unroll
+            for (int n = 0; n < NS; n++) f.x[n][k][i] = s[n];
         }
     }
 }
@@ -237,42 +238,184 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryReg
     }
 }
 
-// A workgroup has 16 rows of one head and a share of their blocks; its four wavefronts take pages in turn.
-template <int D, int NS>
-__global__ __launch_bounds__(256) void attend_few_kernel(AttendArgs a) {
-    typedef Parts<D> PT;
-    typedef typename ElementOf<NS>::type E;
-    constexpr int kPad = 132;  // a row of 128 sums in LDS: 16 lanes x 4 words of a store lie in 64 banks
-    __shared__ float s_sum[4][16 * kPad];
-    __shared__ float s_top[4][16], s_all[4][16];
+// The blocks i = from, from + step, ... < to of a wavefront, as entries of a list or themselves; pages that do not exist and
+// blocks behind the last place that a row sees are passed over.
+struct Blocks {
+    const int32_t *list;
+    int from, step, to;
+};
 
-    const int h = blockIdx.y, split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits;
+// All of a wavefront's blocks.  64 blocks' pages are looked up at once, a lane each, and handed out as scalars: a lookup in the
+// loop would wait, in order, for the page's bytes that were asked for before it.  Where two pages fit the registers of two
+// wavefronts a SIMD, the next page's bytes are loaded before a page is worked on (64 dimensions: 61 us with one, 54 with two, 64
+// tokens over 4,096 to 8,192 and 8 heads; 128: 94 and 92; 96 spills); behind the last one the same page is loaded once more instead
+// of a branch, over which the compiler would have to wait for all loads.
+template <int D, int NS>
+__device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const QueryRegs<D, NS> &f, Blocks l, int b, int h, int sees,
+                                   int least, int most, int length) {
+    const int lane = threadIdx.x & 63;
+    for (int i0 = l.from; i0 < l.to; i0 += 64 * l.step) {
+        const int i = i0 + lane * l.step;
+        int block = 0, page = -1;
+        bool edge = false;
+        if (i < l.to) {
+            block = l.list ? l.list[i] : i;
+            page = (int)page_of(a.t, a.c, b, block);
+            if (page >= 0 && block * kPage >= most) page = -1;
+            if (page >= 0) edge = (block + 1) * kPage > least || a.c.bound_scales[(int64_t)page * a.c.heads + h] == kBoundless;
+        }
+        uint64_t left = __ballot(page >= 0);
+        const uint64_t edges = __ballot(edge);
+        if (!left) continue;
+        int at = 0;
+        auto next = [&](PageRegs<D> &g) {  // the next page's loads
+            if (left) {
+                at = __builtin_ctzll(left);
+                left &= left - 1;
+            }
+            load_page<D>(g, a.c, __builtin_amdgcn_readlane(page, at), h);
+        };
+        auto take = [&](PageRegs<D> &g, int at) {
+            const int first = __builtin_amdgcn_readlane(block, at) * kPage;
+            take_page<D, NS>(st, g, f, a.scale, edges >> at & 1, sees - first, length - first);
+        };
+        PageRegs<D> x;
+        if constexpr (D == 64 || D == 128) {
+            PageRegs<D> y;
+            next(x);
+            for (;;) {
+                int here = at;
+                bool last = !left;
+                next(y);
+                take(x, here);
+                if (last) break;
+                here = at;
+                last = !left;
+                next(x);
+                take(y, here);
+                if (last) break;
+            }
+        } else {
+            while (left) {
+                next(x);
+                take(x, at);
+            }
+        }
+    }
+}
+
+template <int D>
+__device__ inline void start_rows(RowState<D> &st) {
+#pragma unroll
+    for (int k = 0; k < D / 16; k++) st.acc[k] = f32x4{0, 0, 0, 0};
+    st.top = -INFINITY;
+    st.sum = 0;
+}
+
+// Result of a row and head: sums x of dimensions d ..., the maximum and the sum of weights, either whole or one split's.
+template <int NS>
+__device__ inline void put8(const AttendArgs &a, int64_t out_row, int split, int D, int d, float (&x)[8], float total) {
+    typedef typename ElementOf<NS>::type E;
+    if (a.splits > 1) {
+        float *const to = a.part + (out_row * a.splits + split) * D + d;
+        *reinterpret_cast<f32x4 *>(to) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4 *>(to + 4) = f32x4{x[4], x[5], x[6], x[7]};
+    } else {
+        const float by = total == 0 ? 0.0f : 1.0f / total;
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] *= by;
+        store8<NS>((E *)a.out + out_row * D + d, x);
+    }
+}
+__device__ inline void put_sums(const AttendArgs &a, int64_t out_row, int split, int D, float top, float total) {
+    if (a.splits > 1) {
+        float *const to = a.part + (int64_t)a.t.rows * a.heads_q * a.splits * D + (out_row * a.splits + split) * 2;
+        to[0] = top;
+        to[1] = total;
+    } else if (a.lse) {
+        a.lse[out_row] = (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+    }
+}
+
+// Joins what WAVES wavefronts have of the same 16 rows, 128 dimensions at a time: thread t the 8 dimensions 8 (t % 16) of row
+// t / 16.  out_row(r): where row r belongs, negative if it is none.
+constexpr int kJoinPad = 132;  // a row of 128 sums in LDS: 16 lanes x 4 words of a store lie in 64 banks
+template <int WAVES>
+struct JoinLds {
+    float sum[WAVES][16 * kJoinPad];
+    float top[WAVES][16], all[WAVES][16];
+};
+template <int D, int NS, int WAVES, class F>
+__device__ inline void join_waves(const RowState<D> &st, JoinLds<WAVES> &s, const AttendArgs &a, int split, F out_row) {
+    typedef Parts<D> PT;
+    const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15, wave = threadIdx.x >> 6;
+    const float sum = sum_over_quads(st.sum);
+    if (q == 0) {
+        s.top[wave][r] = st.top;
+        s.all[wave][r] = sum;
+    }
+    __syncthreads();
+    const int jr = threadIdx.x >> 4 & 15, js = threadIdx.x & 15;
+    float top = s.top[0][jr], weight[WAVES], total = 0;
+#pragma unroll
+    for (int i = 1; i < WAVES; i++) top = fmaxf(top, s.top[i][jr]);
+    const float base = top > -INFINITY ? top : 0.0f;
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) {
+        weight[i] = __builtin_amdgcn_exp2f(s.top[i][jr] - base);
+        total += weight[i] * s.all[i][jr];
+    }
+    const int64_t to = threadIdx.x < 256 ? out_row(jr) : -1;
+#pragma unroll
+    for (int p = 0; p < PT::kCount; p++) {
+        const int W = PT::width(p), t0 = PT::base(p) / 16;
+        if (p) __syncthreads();
+        // lane (q, r) has dimensions q * W / 4 + e * W / 16 + k
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int k = 0; k < W / 16; k++) s.sum[wave][r * kJoinPad + q * (W / 4) + e * (W / 16) + k] = st.acc[t0 + k][e];
+        __syncthreads();
+        if (js * 8 < W && to >= 0) {
+            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < WAVES; i++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] += weight[i] * s.sum[i][jr * kJoinPad + js * 8 + k];
+            put8<NS>(a, to, split, D, PT::base(p) + js * 8, x, total);
+        }
+    }
+    if (js == 0 && to >= 0) put_sums(a, to, split, D, top, total);
+}
+
+// A tile is 16 rows of one head: of the queries of one token where there is a list, of all tokens of a sequence otherwise.
+// JOIN: the four wavefronts of a workgroup share a tile's blocks and are joined; else each has a tile of its own.
+template <int D, int NS, bool JOIN>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_few_kernel(AttendArgs a, int tiles) {
+    typedef Parts<D> PT;
     const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // with a list, a tile is 16 of the queries of one token; without, of all tokens of the sequence
+    const int h = blockIdx.y, split = JOIN ? blockIdx.x % a.splits : 0, tile = JOIN ? blockIdx.x / a.splits : blockIdx.x * 4 + wave;
+    if (tile >= tiles) return;
     Piece w;
-    int token0 = 0, tokens;
+    int token0 = 0, tokens = 1;
+    const int per = (a.group + 15) / 16;
     if (a.list) {
-        const int per = (a.group + 15) / 16, row = tile / per;
-        w = {sequence_of(a.t, row), tile % per};
-        w.sequence = __builtin_amdgcn_readfirstlane(w.sequence);
-        token0 = row - first_row(a.t, w.sequence);
-        tokens = 1;
+        w = {__builtin_amdgcn_readfirstlane(sequence_of(a.t, tile / per)), tile % per};
+        token0 = tile / per - first_row(a.t, w.sequence);
     } else if (!a.t.offsets) {
-        const int per = (a.group + 15) / 16;
         w = {tile / per, tile % per};
-        tokens = 1;
     } else {
         w = find_piece(a.t.sequences, tile, [&](int b) { return (int)(((int64_t)row_count(a.t, b) * a.group + 15) / 16); });
         if (w.sequence < 0) return;
         tokens = row_count(a.t, w.sequence);
     }
     const int b = w.sequence, length = length_of(a.t, b), all = row_count(a.t, b);
+    const int row0 = first_row(a.t, b);
     const int index = w.piece * 16 + r;
     const bool real = index < tokens * a.group;
     const int token = token0 + index / a.group, head = h * a.group + index % a.group;
-    const int64_t row = first_row(a.t, b) + (int64_t)token;
-    // tokens that the row sees, and the most that any of the tile does
+    // tokens that the row sees, and the least and the most that any of the tile does
     const bool causal = a.causal || a.list;
     int sees = causal ? min(max((int)min((int64_t)a.t.lengths[b], (int64_t)1 << 30) - all + token + 1, 0), length) : length;
     if (!real) sees = 0;
@@ -286,82 +429,37 @@ __global__ __launch_bounds__(256) void attend_few_kernel(AttendArgs a) {
     least = __builtin_amdgcn_readfirstlane(least);
 
     QueryRegs<D, NS> f;
-    load_queries<D, NS>(f, a, real, row, head);
+    load_queries<D, NS>(f, a, real, row0 + (int64_t)token, head);
     RowState<D> st;
-#pragma unroll
-    for (int k = 0; k < D / 16; k++) st.acc[k] = f32x4{0, 0, 0, 0};
-    st.top = -INFINITY;
-    st.sum = 0;
-
+    start_rows<D>(st);
     const int entries = a.list ? a.count : (most + kPage - 1) / kPage;
     const int from = (int)((int64_t)entries * split / a.splits), to = (int)((int64_t)entries * (split + 1) / a.splits);
-    const int32_t *const list = a.list ? a.list + ((first_row(a.t, b) + (int64_t)token0) * a.c.heads + h) * a.count : nullptr;
-    for (int i = from + wave; i < to; i += 4) {
-        const int block = list ? list[i] : i;
-        const int64_t page = page_of(a.t, a.c, b, block);
-        if (page < 0 || block * kPage >= most) continue;
-        PageRegs<D> g;
-        load_page<D>(g, a.c, page, h);
-        const bool edge = (block + 1) * kPage > least || a.c.bound_scales[page * a.c.heads + h] == kBoundless;
-        take_page<D, NS>(st, g, f, a.scale, edge, sees - block * kPage, length - block * kPage);
-    }
+    const int32_t *const list = a.list ? a.list + ((row0 + (int64_t)token0) * a.c.heads + h) * a.count : nullptr;
+    take_blocks<D, NS>(st, a, f, {list, JOIN ? from + wave : from, JOIN ? 4 : 1, to}, b, h, sees, least, most, length);
 
-    // join the four wavefronts, 128 dimensions at a time
-    const float sum = sum_over_quads(st.sum);
-    if (q == 0) {
-        s_top[wave][r] = st.top;
-        s_all[wave][r] = sum;
-    }
-    __syncthreads();
-    const int jr = threadIdx.x >> 4, js = threadIdx.x & 15;  // a thread joins 8 dimensions of row jr
-    float top = s_top[0][jr], weight[4], total = 0;
+    auto out_row = [&](int r) {
+        const int i = w.piece * 16 + r;
+        return i < tokens * a.group ? (row0 + (int64_t)(token0 + i / a.group)) * a.heads_q + h * a.group + i % a.group : -1;
+    };
+    if constexpr (JOIN) {
+        __shared__ JoinLds<4> s_join;
+        join_waves<D, NS, 4>(st, s_join, a, split, out_row);
+    } else {
+        const float total = sum_over_quads(st.sum);
+        const int64_t to = out_row(r);
+        if (to < 0) return;
 #pragma unroll
-    for (int i = 1; i < 4; i++) top = fmaxf(top, s_top[i][jr]);
-    const float base_top = top > -INFINITY ? top : 0.0f;
+        for (int p = 0; p < PT::kCount; p++) {
+            const int W = PT::width(p), t0 = PT::base(p) / 16;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        weight[i] = __builtin_amdgcn_exp2f(s_top[i][jr] - base_top);
-        total += weight[i] * s_all[i][jr];
-    }
-    const int jindex = w.piece * 16 + jr;
-    const bool jreal = jindex < tokens * a.group;
-    const int64_t out_row = (first_row(a.t, b) + (int64_t)(token0 + jindex / a.group)) * a.heads_q + h * a.group + jindex % a.group;
+            for (int d = 0; d < W / 4; d += 8) {
+                float x[8];
 #pragma unroll
-    for (int p = 0; p < PT::kCount; p++) {
-        const int W = PT::width(p), t0 = PT::base(p) / 16;
-        if (p) __syncthreads();
-        // lane (q, r) has dimensions q * W / 4 + e * W / 16 + k
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-            for (int k = 0; k < W / 16; k++) s_sum[wave][r * kPad + q * (W / 4) + e * (W / 16) + k] = st.acc[t0 + k][e];
-        __syncthreads();
-        if (js * 8 < W && jreal) {
-            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int k = 0; k < 8; k++) x[k] += weight[i] * s_sum[i][jr * kPad + js * 8 + k];
-            if (a.splits > 1) {
-                float *const to = a.part + (out_row * a.splits + split) * D + PT::base(p) + js * 8;
-#pragma unroll
-                for (int k = 0; k < 8; k++) to[k] = x[k];
-            } else {
-                const float by = total == 0 ? 0.0f : 1.0f / total;
-#pragma unroll
-                for (int k = 0; k < 8; k++) x[k] *= by;
-                store8<NS>((E *)a.out + out_row * D + PT::base(p) + js * 8, x);
+                for (int k = 0; k < 8; k++) x[k] = st.acc[t0 + (d + k) % (W / 16)][(d + k) / (W / 16)];
+                put8<NS>(a, to, 0, D, PT::base(p) + q * (W / 4) + d, x, total);
             }
         }
-    }
-    if (js == 0 && jreal) {
-        if (a.splits > 1) {
-            float *const to = a.part + (int64_t)a.t.rows * a.heads_q * a.splits * D + (out_row * a.splits + split) * 2;
-            to[0] = top;
-            to[1] = total;
-        } else if (a.lse) {
-            a.lse[out_row] = (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
-        }
+        if (q == 0) put_sums(a, to, 0, D, st.top, total);
     }
 }
 

@@ -2,6 +2,7 @@
 #pragma once
 #include "attend_few.h"
 #include "attend_many.h"
+#include "attend_step.h"
 
 template <int D, int NS>
 void launch_join(const AttendArgs &a, hipStream_t stream) {
@@ -10,11 +11,17 @@ void launch_join(const AttendArgs &a, hipStream_t stream) {
 
 template <int NS>
 int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
-    VL_REQUIRE(tiles * a.splits <= 4 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)(tiles * a.splits));
+    VL_REQUIRE(tiles * (a.splits ? a.splits : 1) <= 4 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)tiles);
     for_dim(a.c.dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        attend_few_kernel<D, NS><<<dim3((unsigned)(tiles * a.splits), (unsigned)a.c.heads), 256, 0, stream>>>(a);
-        launch_join<D, NS>(a, stream);
+        if (a.splits) {
+            attend_few_kernel<D, NS, true><<<dim3((unsigned)(tiles * a.splits), (unsigned)a.c.heads), 256, 0, stream>>>(a, (int)tiles);
+            launch_join<D, NS>(a, stream);
+        } else {
+            AttendArgs one = a;
+            one.splits = 1;
+            attend_few_kernel<D, NS, false><<<dim3((unsigned)((tiles + 3) / 4), (unsigned)a.c.heads), 256, 0, stream>>>(one, (int)tiles);
+        }
     });
     VL_LAUNCH_CHECK("attend_few_kernel");
     return VL_OK;
@@ -35,5 +42,20 @@ int launch_attend_many(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
     });
     VL_HIP(e);
     VL_LAUNCH_CHECK("attend_many_kernel");
+    return VL_OK;
+}
+
+template <int NS>
+int launch_attend_step(const AttendArgs &a, const SelectArgs &s, hipStream_t stream) {
+    hipError_t e = hipSuccess;
+    const size_t keys = ((size_t)a.t.blocks * 4 + 15) / 16 * 16, join = sizeof(JoinLds<kStepWaves>);
+    const size_t lds = (keys > join ? keys : join) + (size_t)s.count * 4;
+    for_dim(a.c.dim, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        e = vl_allow_lds(attend_step_kernel<D, NS>, lds);
+        if (e == hipSuccess) attend_step_kernel<D, NS><<<(unsigned)(a.t.rows * (int64_t)a.c.heads), 512, lds, stream>>>(a, s);
+    });
+    VL_HIP(e);
+    VL_LAUNCH_CHECK("attend_step_kernel");
     return VL_OK;
 }

@@ -174,15 +174,16 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && D * NS <= 128 ? 2 : 1) vo
 
     bf16x8 q[NS][D / 16];
     {
-        const E *const p = (const E *)a.queries + (real ? row * a.q_row + head * a.q_head : 0) + hi * 8;
+        Eight<NS> x[D / 16];
+        const E *const at = (const E *)a.queries + (real ? row * a.q_row + head * a.q_head : 0) + hi * 8;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) x[k] = load8<NS>(at + k * 16, real);
 #pragma unroll
         for (int k = 0; k < D / 16; k++) {
-            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (real) load8<NS>(p + k * 16, a.aligned, x);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 __bf16 s[NS];
-                split_into<NS>(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[i]) ^ a.sign), s);
+                split_into<NS>(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)x[k][i]) ^ a.sign), s);
 #pragma unroll
                 for (int n = 0; n < NS; n++) q[n][k][i] = s[n];
             }

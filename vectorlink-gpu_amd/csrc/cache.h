@@ -109,20 +109,23 @@ template <> struct ElementOf<1> { typedef __bf16 type; };
 template <> struct ElementOf<2> { typedef _Float16 type; };
 template <> struct ElementOf<3> { typedef float type; };
 
-// 8 elements from p, which lies on a 16-byte boundary if `aligned`
+// 8 elements that lie on a boundary of their own type: gfx950 loads 16 bytes from any address, so there is no other path for rows
+// off 16-byte boundaries.
 template <int NS>
-__device__ inline void load8(const typename ElementOf<NS>::type *p, bool aligned, float (&x)[8]) {
+using Eight = typename ElementOf<NS>::type __attribute__((ext_vector_type(8)));
+template <int NS>
+__device__ inline Eight<NS> load8(const typename ElementOf<NS>::type *p) {
+    typedef Eight<NS> Anywhere __attribute__((aligned(sizeof(typename ElementOf<NS>::type))));
+    return *reinterpret_cast<const Anywhere *>(p);
+}
+// The same where `real`, else zeros; p is readable all the same.  A load behind a branch would be waited for before the next.
+template <int NS>
+__device__ inline Eight<NS> load8(const typename ElementOf<NS>::type *p, bool real) {
     typedef typename ElementOf<NS>::type E;
-    typedef E e8 __attribute__((ext_vector_type(8)));
-    e8 v;
-    if (aligned) {
-        v = *reinterpret_cast<const e8 *>(p);
-    } else {
+    Eight<NS> v = load8<NS>(p);
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = p[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (float)v[i];
+    for (int i = 0; i < 8; i++) v[i] = real ? v[i] : (E)0.0f;
+    return v;
 }
 template <int NS>
 __device__ inline void store8(typename ElementOf<NS>::type *p, const float (&x)[8]) {

@@ -37,11 +37,14 @@ namespace {
 struct Rows {  // [rows, heads, dim] of a call
     const void *at;
     int64_t row, head;
-    bool aligned;
 };
 
 // The codes of 8 elements of a token, four lanes of a group together: the scale's byte, and whether the elements are finite.
-__device__ inline uint32_t quantise8(const float (&x)[8], int *byte, bool *finite) {
+template <int NS>
+__device__ inline uint32_t quantise8(const Eight<NS> &v, int *byte, bool *finite) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = (float)v[i];
     uint32_t bits = 0;  // the largest magnitude's, NaN above infinity above all others
 #pragma unroll
     for (int i = 0; i < 8; i++) bits = max(bits, __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu);
@@ -72,16 +75,18 @@ __device__ inline void widen(float (&hi)[8], float (&lo)[8], uint32_t code, floa
 }
 
 // One workgroup makes one block of one head: T = 2^n >= D / 8 lanes take a token, 8 dimensions each, 256 / T tokens at a time.
-// New tokens are quantised and stored, older ones of the block are read back, and both go into the bounds.
+// New tokens are quantised and stored, older ones of the block are read back, and both go into the bounds.  What bounds it is the
+// bytes: rows are asked for kAhead at a time, and scales, a byte for each 32 elements, are collected in LDS.
 template <int D, int NS>
 __global__ __launch_bounds__(256) void cache_write_kernel(CacheView c, Tokens t, Rows keys, Rows values) {
     constexpr int kSegs = D / 8;
     constexpr int T = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32;
-    constexpr int kAtOnce = 256 / T;
+    constexpr int kAtOnce = 256 / T, kAhead = kPage / kAtOnce < 4 ? kPage / kAtOnce : 4;
     typedef typename ElementOf<NS>::type E;
     __shared__ float s_hi[kAtOnce][D], s_lo[kAtOnce][D];
     __shared__ float s_top[4];
     __shared__ int s_bad;
+    __shared__ __attribute__((aligned(4))) uint8_t s_scale[2][D / 32][kPage];
 
     const int h = blockIdx.y;
     const Piece w = find_piece(t.sequences, blockIdx.x, [&](int b) {
@@ -110,41 +115,55 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheView c, Tokens t,
         lo[i] = INFINITY;
     }
     if (threadIdx.x == 0) s_bad = 0;
+    for (int i = threadIdx.x; i < 2 * D / 32 * kPage / 4; i += 256) reinterpret_cast<uint32_t *>(s_scale)[i] = 0;
     __syncthreads();
     bool bad = false;
-    for (int j0 = 0; j0 < last; j0 += kAtOnce) {
-        const int j = j0 + at;
-        const bool fresh = j >= first && j < last, old = j < first;
-        const int64_t row = row0 + ((int64_t)block * kPage + j - start);
-        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0}, y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (fresh && seg < kSegs) {
-            load8<NS>((const E *)keys.at + row * keys.row + h * keys.head + seg * 8, keys.aligned, x);
-            load8<NS>((const E *)values.at + row * values.row + h * values.head + seg * 8, values.aligned, y);
+    for (int j0 = 0; j0 < last; j0 += kAtOnce * kAhead) {
+        Eight<NS> x[kAhead], y[kAhead];
+        uint32_t oldk[kAhead];
+        int oldkb[kAhead], oldvb[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const int j = j0 + k * kAtOnce + at;
+            const bool real = j >= first && j < last && seg < kSegs;
+            const int64_t row = row0 + ((int64_t)block * kPage + j - start);
+            x[k] = load8<NS>((const E *)keys.at + (real ? row * keys.row + h * keys.head + seg * 8 : 0), real);
+            y[k] = load8<NS>((const E *)values.at + (real ? row * values.row + h * values.head + seg * 8 : 0), real);
         }
-        int kb, vb;
-        bool kf, vf;
-        uint32_t kcode = quantise8(x, &kb, &kf), vcode = quantise8(y, &vb, &vf);
-        kf = !(__ballot(!kf) & mine);  // one element that is not finite spoils the token
-        vf = !(__ballot(!vf) & mine);
-        if (seg >= kSegs) continue;  // nothing after this needs other lanes
-        if (fresh) {
+        if (first > 0) {
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                const int j = min(j0 + k * kAtOnce + at, kPage - 1), g = min(seg, kSegs - 1);
+                oldk[k] = *reinterpret_cast<const uint32_t *>(kc + j * (D / 2) + g * 4);
+                oldkb[k] = ks[(g >> 2) * kPage + j];
+                oldvb[k] = vs[(g >> 2) * kPage + j];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const int j = j0 + k * kAtOnce + at;
+            const bool fresh = j >= first && j < last, old = j < first;
+            int kb, vb;
+            bool kf, vf;
+            uint32_t kcode = quantise8<NS>(x[k], &kb, &kf), vcode = quantise8<NS>(y[k], &vb, &vf);
+            kf = !(__ballot(!kf) & mine);  // one element that is not finite spoils the token
+            vf = !(__ballot(!vf) & mine);
             if (!kf) kcode = 0, kb = kNotFinite;
             if (!vf) vcode = 0, vb = kNotFinite;
-            *reinterpret_cast<uint32_t *>(kc + j * (D / 2) + seg * 4) = kcode;
-            *reinterpret_cast<uint32_t *>(vc + ((j >> 2) * kSegs + seg) * 16 + (j & 3) * 4) = vcode;
-            if ((seg & 3) == 0) {
-                ks[(seg >> 2) * kPage + j] = (uint8_t)kb;
-                vs[(seg >> 2) * kPage + j] = (uint8_t)vb;
+            if (old) kcode = oldk[k], kb = oldkb[k], vb = oldvb[k];
+            if (seg < kSegs && (fresh || old)) {
+                if (fresh) {
+                    *reinterpret_cast<uint32_t *>(kc + j * (D / 2) + seg * 4) = kcode;
+                    *reinterpret_cast<uint32_t *>(vc + ((j >> 2) * kSegs + seg) * 16 + (j & 3) * 4) = vcode;
+                }
+                if ((seg & 3) == 0) {
+                    s_scale[0][seg >> 2][j] = (uint8_t)kb;
+                    s_scale[1][seg >> 2][j] = (uint8_t)vb;
+                }
+                bad |= kb == kNotFinite || vb == kNotFinite;
+                if (kb != kNotFinite) widen(hi, lo, kcode, __builtin_bit_cast(float, (uint32_t)kb << 23));
             }
-        } else if (old) {
-            kcode = *reinterpret_cast<const uint32_t *>(kc + j * (D / 2) + seg * 4);
-            kb = ks[(seg >> 2) * kPage + j];
-            vb = vs[(seg >> 2) * kPage + j];
-        } else {
-            continue;
         }
-        bad |= kb == kNotFinite || vb == kNotFinite;
-        if (kb != kNotFinite) widen(hi, lo, kcode, __builtin_bit_cast(float, (uint32_t)kb << 23));
     }
     if (seg < kSegs) {
 #pragma unroll
@@ -155,6 +174,12 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheView c, Tokens t,
     }
     if (bad) s_bad = 1;
     __syncthreads();
+    // scales four tokens at a time; behind the last token a word is filled up with zeros
+    for (int i = threadIdx.x; i < 2 * D / 32 * kPage / 4; i += 256) {
+        const int word = i % (kPage / 4), g = i / (kPage / 4) % (D / 32), which = i / (kPage / 4) / (D / 32);
+        if (word >= first >> 2 && word * 4 < last)
+            reinterpret_cast<uint32_t *>(which ? vs : ks)[g * (kPage / 4) + word] = *reinterpret_cast<const uint32_t *>(&s_scale[which][g][word * 4]);
+    }
     // D <= 256: a thread for each dimension
     const int d = threadIdx.x;
     float top = 0, dh = 0, dl = 0;
@@ -257,10 +282,6 @@ int read_rows(const CacheView &c, const Tokens &t, void *keys, void *values, hip
     return VL_OK;
 }
 
-bool on16(const void *p, int64_t row, int64_t head, int size) {
-    return ((uintptr_t)p & 15) == 0 && (row * size) % 16 == 0 && (head * size) % 16 == 0;
-}
-
 }  // namespace
 
 VL_EXPORT int vl_cache_write(const vl_cache *cache, const vl_tokens *tokens, int type, const void *keys, int64_t key_row,
@@ -275,8 +296,7 @@ VL_EXPORT int vl_cache_write(const vl_cache *cache, const vl_tokens *tokens, int
     VL_REQUIRE(keys && values, "keys or values is null");
     const int size = type == VL_F32 ? 4 : 2;
     VL_REQUIRE(((uintptr_t)keys | (uintptr_t)values) % size == 0, "keys or values not aligned to their type");
-    const Rows k = {keys, key_row, key_head, on16(keys, key_row, key_head, size)};
-    const Rows v = {values, value_row, value_head, on16(values, value_row, value_head, size)};
+    const Rows k = {keys, key_row, key_head}, v = {values, value_row, value_head};
     const hipStream_t s = (hipStream_t)stream;
     return type == VL_BF16 ? write_rows<1>(c, t, k, v, s) : type == VL_F16 ? write_rows<2>(c, t, k, v, s) : write_rows<3>(c, t, k, v, s);
 }

@@ -7,7 +7,7 @@ struct SelectArgs {
     Tokens t;
     const void *queries;
     int64_t q_row, q_head;
-    int group, aligned;
+    int group;
     int count;
     int32_t *out;    // [rows, c.heads, count]
     uint32_t *keys;  // [rows, c.heads, t.blocks]: scores, in an order that unsigned numbers have
