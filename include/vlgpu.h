@@ -557,6 +557,7 @@ typedef struct vl_queries {
     double scale; /* scores are scale * <query, key> */
     int32_t type; /* VL_BF16, VL_F16, VL_F32 */
     int32_t causal; /* 0: every row sees all lengths[b] tokens; else those up to its own place */
+    int64_t form; /* of vl_attend: 0, or VL_ATTEND_FEW or VL_ATTEND_MANY whatever the sizes, for tests and measurements */
 } vl_queries;
 
 /* Softmax attention over everything the cache holds of the sequences.  Sums and
@@ -565,10 +566,12 @@ typedef struct vl_queries {
 int64_t vl_attend_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries);
 int vl_attend(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
               void *workspace, int64_t workspace_bytes, void *stream);
-/* The form that takes such a call: VL_ATTEND_FEW splits the tokens over
- * workgroups, VL_ATTEND_MANY shares them among the rows of a workgroup. */
-#define VL_ATTEND_FEW 0
-#define VL_ATTEND_MANY 1
+/* The form that takes such a call: VL_ATTEND_FEW has tiles of 16 rows and splits
+ * the tokens of each over workgroups, VL_ATTEND_MANY shares a page among 256 or
+ * 128 rows.  The latter is there for bfloat16, for half precision up to 128
+ * dimensions and for float32 up to 64; the former takes the other calls. */
+#define VL_ATTEND_FEW 1
+#define VL_ATTEND_MANY 2
 int vl_attend_form(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries);
 
 /* blocks [rows, cache.heads, count]: for every row and head of the cache the

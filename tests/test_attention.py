@@ -26,7 +26,7 @@ def tokens(**kw):
 
 
 def queries(**kw):
-    p = dict(heads=8, row_stride=1024, head_stride=128, queries=256, out=256, lse=None, scale=1.0, type=1, causal=1)
+    p = dict(heads=8, row_stride=1024, head_stride=128, queries=256, out=256, lse=None, scale=1.0, type=1, causal=1, form=0)
     p.update(kw)
     return C.byref(nv.Queries(**p))
 
@@ -36,7 +36,7 @@ BAD_CACHES = [dict(dim=80), dict(dim=0), dict(dim=512), dict(heads=0), dict(head
 BAD_TOKENS = [dict(rows=-1), dict(rows=4), dict(sequences=-1), dict(blocks=-1), dict(table_stride=3), dict(table=None), dict(lengths=None),
               dict(rows=3, sequences=0, offsets=256)]
 BAD_QUERIES = [dict(heads=3), dict(heads=0), dict(type=0), dict(type=4), dict(queries=None), dict(out=None), dict(queries=257),
-               dict(out=264), dict(scale=float("nan")), dict(scale=float("inf"))]
+               dict(out=264), dict(scale=float("nan")), dict(scale=float("inf")), dict(form=3), dict(form=-1)]
 
 
 def test_cache_and_tokens_are_checked_by_every_call(lib):
@@ -89,6 +89,22 @@ def test_workspaces_are_checked(lib):
     both = lib.vl_attend_selected_workspace_bytes(cache(), t, queries(), 40)
     assert both == sizes[1][0] + sizes[2][0]
     assert lib.vl_attend_selected(cache(), t, queries(), 40, 256, 256, sizes[1][0] - 1, None) == -3
+
+
+def test_form_by_sizes(lib):
+    """Single tokens and a few go to the one form, prompts to the other where it is there."""
+    def form(rows, length, type=1, dim=128, heads=8, group=4, batch=1, **kw):
+        blocks = -(-length // 64)
+        t = tokens(rows=rows * batch, sequences=batch, blocks=blocks, table_stride=blocks, offsets=None if rows == 1 else 256)
+        return lib.vl_attend_form(cache(dim=dim, heads=heads), t, queries(heads=heads * group, type=type, **kw))
+
+    (few, many) = (1, 2)
+    assert form(1, 131_072) == few and form(1, 8192, batch=64) == few and form(5, 2050, type=3, dim=256) == few
+    assert form(2048, 16_384) == many and form(2048, 16_384, dim=256) == many and form(2048, 8192, type=2) == many
+    assert form(2048, 8192, type=3, dim=64) == many
+    assert form(2048, 8192, type=3) == few and form(2048, 8192, type=2, dim=192) == few
+    assert form(1, 64, form=many) == many and form(2048, 16_384, form=few) == few
+    assert form(2048, 8192, type=3, form=many) == -1
 
 
 def test_calls_without_rows_succeed(lib):

@@ -64,24 +64,18 @@ def check(got, lse, want, dtype, dim):
     assert ((lse - want_lse).abs() <= 2 * score[..., 0] + 2.0 ** -20 + want_lse.abs() * 2.0 ** -22)[some].all()
 
 
-def form(q, cache, table, lengths, offsets):
-    """The form that the library takes for such a call."""
-    import ctypes as C
-
-    from vectorlink_gpu import attention
-
-    tokens = attention._tokens(q.shape[0], table, lengths, offsets)
-    return nv.lib().vl_attend_form(cache._ref, C.byref(tokens), C.byref(attention._queries(q, cache, None, True, q, None)))
+def form(dim, dtype):
+    """Asks for the form for many rows where it is there; the one for few takes the others."""
+    return "many" if dim * nv.TYPES[dtype] <= 256 else None
 
 
 def run(counts, lengths, heads, group, dim, dtype, seed, causal=True, scale=None):
     cache, table, lengths, gen = filled(lengths, heads, dim, seed, dtype)
     q = queries_for(sum(counts), heads * group, dim, gen, dtype)
     at = ends(counts)
-    assert form(q, cache, table, lengths, at) == nv.ATTEND_FORMS["many"]
-    (out, lse) = attend(q, cache, table, lengths, offsets=at, causal=causal, scale=scale, return_lse=True)
+    (out, lse) = attend(q, cache, table, lengths, offsets=at, causal=causal, scale=scale, return_lse=True, form=form(dim, dtype))
     check(out, lse, dense(q, cache, table, lengths, at, scale, causal), dtype, dim)
-    assert torch.equal(out, attend(q, cache, table, lengths, offsets=at, causal=causal, scale=scale))
+    assert torch.equal(out, attend(q, cache, table, lengths, offsets=at, causal=causal, scale=scale, form=form(dim, dtype)))
     return out
 
 
@@ -116,7 +110,7 @@ def test_scores_that_grow(dtype):
     k = torch.randn((700, 1, 64), generator=gen, device=DEV) * torch.logspace(-2, 1.3, 700, device=DEV)[:, None, None]
     cache.write(k.to(dtype), k.to(dtype), table, lengths - 700, ends([700]))
     q = queries_for(400, 2, 64, gen, dtype, 3.0)
-    (out, lse) = attend(q, cache, table, lengths, offsets=ends([400]), return_lse=True)
+    (out, lse) = attend(q, cache, table, lengths, offsets=ends([400]), return_lse=True, form=form(64, dtype))
     check(out, lse, dense(q, cache, table, lengths, ends([400])), dtype, 64)
 
 
@@ -130,7 +124,7 @@ def test_tokens_that_are_not_finite(dtype):
     v[390, 1, 60] = math.inf
     cache.write(k, v, table, lengths - torch.tensor([400, 0], dtype=torch.int32, device=DEV), ends([400, 0]))
     q = queries_for(600, 4, 64, gen, dtype)
-    (out, lse) = attend(q, cache, table, lengths, offsets=ends([400, 200]), return_lse=True)
+    (out, lse) = attend(q, cache, table, lengths, offsets=ends([400, 200]), return_lse=True, form=form(64, dtype))
     want = dense(q, cache, table, lengths, ends([400, 200]))
     assert want[0][:350].isfinite().all() and want[0][350:400, :2].isnan().all() and want[0][390:400].isnan().all() and want[0][400:].isfinite().all()
     check(out, lse, want, dtype, 64)
@@ -142,7 +136,7 @@ def test_pages_that_hold_nothing_take_no_part():
     table[0, 5] = 2147483647
     table[1] = cache.pages
     q = queries_for(900, 2, 128, gen, torch.bfloat16)
-    (out, lse) = attend(q, cache, table, lengths, offsets=ends([500, 400]), return_lse=True)
+    (out, lse) = attend(q, cache, table, lengths, offsets=ends([500, 400]), return_lse=True, form="many")
     check(out, lse, dense(q, cache, table, lengths, ends([500, 400])), torch.bfloat16, 128)
     assert not out[500:].any()
 
@@ -151,8 +145,29 @@ def test_strides_and_alignment():
     cache, table, lengths, gen = filled([500, 130], 2, 96, 15)
     flat = queries_for(430, 6, 96, gen, torch.bfloat16)
     at = ends([400, 30])
-    want = attend(flat, cache, table, lengths, offsets=at)
+    want = attend(flat, cache, table, lengths, offsets=at, form="many")
     for q in (torch.empty((430, 10, 99), dtype=torch.bfloat16, device=DEV)[:, 2:8, 1:97],
               torch.empty((6, 430, 96), dtype=torch.bfloat16, device=DEV).transpose(0, 1)):
         q.copy_(flat)
-        assert torch.equal(attend(q, cache, table, lengths, offsets=at), want)
+        assert torch.equal(attend(q, cache, table, lengths, offsets=at, form="many"), want)
+
+
+def test_single_tokens_in_the_form_for_many():
+    """Without offsets, one row a sequence."""
+    cache, table, lengths, gen = filled([300, 0, 77], 2, 128, 17)
+    q = queries_for(3, 8, 128, gen, torch.bfloat16)
+    (out, lse) = attend(q, cache, table, lengths, return_lse=True, form="many")
+    check(out, lse, dense(q, cache, table, lengths, ends([1, 1, 1])), torch.bfloat16, 128)
+
+
+def test_rows_behind_the_last_offset_are_left_alone():
+    """Offsets that name fewer rows than there are, or more: nothing outside is read or written."""
+    cache, table, lengths, gen = filled([300, 200], 1, 64, 19)
+    q = queries_for(300, 2, 64, gen, torch.bfloat16)
+    for f in ("few", "many"):
+        want = attend(q[:250], cache, table, lengths, offsets=ends([150, 100]), form=f)
+        got = attend(q, cache, table, lengths, offsets=ends([150, 100]), form=f)
+        assert torch.equal(got[:250], want)
+        over = ends([150, 100])
+        over[2] = 1_000_000  # cut to the rows that there are
+        attend(q[:250], cache, table, lengths, offsets=over, form=f)

@@ -25,7 +25,11 @@ constexpr int kMaxSplits = 64;
 template <int NS>
 int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream);
 // 32 rows a wavefront, all of a workgroup's on the same pages: 8 wavefronts, or 4 where a row's registers are many
-constexpr int many_waves(int dim, int parts) { return dim <= 128 && dim * parts <= 256 ? 8 : 4; }
+constexpr int many_waves(int dim) { return dim <= 128 ? 8 : 4; }
+constexpr bool many_built(int dim, int parts) { return dim * parts <= 256; }
+// pages a round: two where two sets of them fit LDS (2,048 rows over 16,384 tokens of 128: 503 us with one, 492 with two; of 64: 365
+// and 333)
+constexpr int many_pages(int dim) { return dim <= 128 ? 2 : 1; }
 template <int NS>
 int launch_attend_many(const AttendArgs &a, int64_t tiles, hipStream_t stream);
 // a choice of blocks and attention over it, a workgroup for a token and head

@@ -6,8 +6,6 @@
 
 namespace {
 
-// From so many rows a sequence on (queries that share a head counted each) the form that shares a page among them is the faster.
-constexpr int kManyRows = 256;
 // Tokens times heads up to which one launch for a choice and its attention is the faster: a workgroup for each compute unit (512
 // workgroups over 8,192 tokens each: 56 us, in several launches 45; 128 over 131,072: 46 and 57).  A compute unit alone reads about
 // 25 GB/s, so few workgroups take it for few bytes each (8 over 32,768 tokens, 0.4 MB each: 24 and 29 us; over 131,072, 0.8
@@ -23,6 +21,8 @@ int attend_args(const vl_cache *cache, const vl_tokens *tokens, const vl_queries
     VL_REQUIRE(q->type >= VL_BF16 && q->type <= VL_F32, "type: %d", q->type);
     VL_REQUIRE(q->heads >= 1 && q->heads <= (1 << 24) && q->heads % a->c.heads == 0, "%lld heads of queries for %d of the cache",
                (long long)q->heads, a->c.heads);
+    VL_REQUIRE(q->form == 0 || q->form == VL_ATTEND_FEW || (q->form == VL_ATTEND_MANY && many_built(a->c.dim, q->type)), "form: %lld",
+               (long long)q->form);
     const int size = q->type == VL_F32 ? 4 : 2;
     if (data && a->t.rows) {
         VL_REQUIRE(q->queries && q->out, "queries or out is null");
@@ -70,21 +70,39 @@ int64_t part_bytes(const AttendArgs &a, int splits) {
     return ((int64_t)a.t.rows * a.heads_q * splits * (a.c.dim + 2) * 4 + 255) / 256 * 256;
 }
 
-// Tiles of the rows of a workgroup of attend_many_kernel
-int many_rows(const AttendArgs &a, int type) { return 32 * many_waves(a.c.dim, type); }
-int64_t many_tiles(const AttendArgs &a, int type) { return (int64_t)a.t.rows * a.group / many_rows(a, type) + a.t.sequences; }
-
-bool takes_many(const AttendArgs &a, int type) {
-    return a.t.offsets && (int64_t)a.t.rows * a.group >= (int64_t)kManyRows * a.t.sequences;
+// Tiles of the rows of a workgroup of attend_many_kernel: at most, and about
+int64_t many_tiles(const AttendArgs &a) { return (int64_t)a.t.rows * a.group / (32 * many_waves(a.c.dim)) + a.t.sequences; }
+int64_t many_tiles_about(const AttendArgs &a) {
+    const int64_t rows = 32 * many_waves(a.c.dim), each = (int64_t)a.t.rows * a.group / a.t.sequences;
+    return a.t.sequences * (each / rows + (each % rows != 0));
 }
 
-// Workgroups that share a tile's tokens: enough for one on every compute unit, but eight pages for each.
-int many_splits(const AttendArgs &a, int64_t tiles) {
-    const int64_t items = tiles * a.c.heads;
-    if (items == 0) return 1;
-    int64_t s = kComputeUnits / items;
-    s = s < a.t.blocks / 8 ? s : a.t.blocks / 8;
-    return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+// Pages that the busiest compute unit takes one after the other, a workgroup's start and end counted as kEnds, if the tokens of a
+// tile are split over `splits` workgroups.
+constexpr int64_t kEnds = 3;
+int64_t many_pages_in_turn(const AttendArgs &a, int64_t splits) {
+    const int64_t groups = many_tiles_about(a) * a.c.heads * splits;
+    return (groups + kComputeUnits - 1) / kComputeUnits * ((a.t.blocks + splits - 1) / splits + kEnds);
+}
+int many_splits(const AttendArgs &a) {
+    int best = 1;
+    for (int s = 2; s <= 32 && a.t.blocks / s >= 4; s++)
+        if (many_pages_in_turn(a, s) < many_pages_in_turn(a, best)) best = s;
+    return best;
+}
+
+// The form whose compute units are done first.  A page of a workgroup of attend_many_kernel takes a compute unit about as long as 8
+// pages of 16 rows in attend_few_kernel take it (11 where queries are two or three parts): at 8,192 rows and 128 dimensions 2.0
+// us against 0.26, half precision 3.4 and 0.28, so of a tile's 256 rows more than half have to be there; 6 for the 128 rows of longer
+// ones (256 dimensions: 3.6 and 0.58).  Where a row's
+// registers leave one wavefront a SIMD (half precision of 192, float32 of 96 and more) the few-row form is never slower: 256
+// dimensions of float32 1026 us against 699.
+bool takes_many(const AttendArgs &a, const vl_queries *q) {
+    const int type = q->type;
+    if (q->form) return q->form == VL_ATTEND_MANY;
+    if (!a.t.offsets || !many_built(a.c.dim, type) || a.t.sequences == 0) return false;
+    const int64_t few = ((int64_t)a.t.rows * a.group + 15) / 16 * a.c.heads * a.t.blocks / kComputeUnits;
+    return many_pages_in_turn(a, many_splits(a)) * (type != VL_BF16 ? 11 : a.c.dim <= 128 ? 8 : 6) < few;
 }
 
 int check_workspace(int64_t need, const void *workspace, int64_t bytes) {
@@ -106,8 +124,8 @@ int attend_few(AttendArgs &a, int type, void *workspace, int64_t bytes, hipStrea
 }
 
 int attend_many(AttendArgs &a, int type, void *workspace, int64_t bytes, hipStream_t stream) {
-    const int64_t tiles = many_tiles(a, type);
-    a.splits = many_splits(a, tiles);
+    const int64_t tiles = many_tiles(a);
+    a.splits = many_splits(a);
     const int rc = check_workspace(part_bytes(a, a.splits), workspace, bytes);
     if (rc != VL_OK) return rc;
     a.part = (float *)workspace;
@@ -145,14 +163,14 @@ bool in_one_step(const AttendArgs &a, int64_t count) {
 VL_EXPORT int vl_attend_form(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries) {
     AttendArgs a;
     const int rc = attend_args(cache, tokens, queries, false, &a);
-    return rc != VL_OK ? rc : takes_many(a, queries->type) ? VL_ATTEND_MANY : VL_ATTEND_FEW;
+    return rc != VL_OK ? rc : takes_many(a, queries) ? VL_ATTEND_MANY : VL_ATTEND_FEW;
 }
 
 VL_EXPORT int64_t vl_attend_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries) {
     AttendArgs a;
     const int rc = attend_args(cache, tokens, queries, false, &a);
     if (rc != VL_OK) return rc;
-    if (takes_many(a, queries->type)) return part_bytes(a, many_splits(a, many_tiles(a, queries->type)));
+    if (takes_many(a, queries)) return part_bytes(a, many_splits(a));
     return part_bytes(a, splits_for(a, few_tiles(a)));
 }
 
@@ -161,7 +179,7 @@ VL_EXPORT int vl_attend(const vl_cache *cache, const vl_tokens *tokens, const vl
     AttendArgs a;
     const int rc = attend_args(cache, tokens, queries, true, &a);
     if (rc != VL_OK || a.t.rows == 0) return rc;
-    return takes_many(a, queries->type) ? attend_many(a, queries->type, workspace, workspace_bytes, (hipStream_t)stream)
+    return takes_many(a, queries) ? attend_many(a, queries->type, workspace, workspace_bytes, (hipStream_t)stream)
                                         : attend_few(a, queries->type, workspace, workspace_bytes, (hipStream_t)stream);
 }
 

@@ -33,12 +33,14 @@ int launch_attend_many(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
     VL_REQUIRE(groups <= 2 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)groups);
     hipError_t e = hipSuccess;
     for_dim(a.c.dim, [&](auto d) {
-        constexpr int D = decltype(d)::value, W = many_waves(D, NS);
-        constexpr size_t lds = 2 * (Images<D>::kBytes + kPage);
-        e = vl_allow_lds(attend_many_kernel<D, NS, W>, lds);
-        if (e != hipSuccess) return;
-        attend_many_kernel<D, NS, W><<<(unsigned)groups, W * 64, lds, stream>>>(a, (int)tiles);
-        launch_join<D, NS>(a, stream);
+        constexpr int D = decltype(d)::value, W = many_waves(D), P = many_pages(D);
+        if constexpr (many_built(D, NS)) {
+            constexpr size_t lds = 2 * P * (Images<D>::kBytes + kPage);
+            e = vl_allow_lds(attend_many_kernel<D, NS, W, P>, lds);
+            if (e != hipSuccess) return;
+            attend_many_kernel<D, NS, W, P><<<(unsigned)groups, W * 64, lds, stream>>>(a, (int)tiles);
+            launch_join<D, NS>(a, stream);
+        }
     });
     VL_HIP(e);
     VL_LAUNCH_CHECK("attend_many_kernel");

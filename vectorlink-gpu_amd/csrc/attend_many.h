@@ -3,8 +3,8 @@
 // What bounds it is the two matrix products, 4 D operations a row and token, and beside them the vector units' work on every
 // score (maximum, exponential, sum, rounding).  A workgroup has kRows = 32 WAVES rows of one head - tokens and the queries that
 // share the head, one after the other - and takes a page of 64 tokens at a time: all wavefronts turn its bytes into bfloat16
-// in LDS once, then each reads all of it for 32 rows of its own.  Two buffers, one barrier a page: the next page's bytes are
-// on their way while this one is worked on, and are turned into the other buffer after it.
+// in LDS once, then each reads all of it for 32 rows of its own.  PAGES pages a round, two sets of buffers, one barrier a round:
+// the next pages' bytes are on their way while these are worked on, and are turned into the other buffers after them.
 //
 // S^T = K Q^T in tiles of 32 tokens x 32 rows: lane l holds row l % 32, and of a tile the tokens 8 (i / 4) + 4 (l / 32) + i % 4.
 // out^T = V^T P^T takes P^T as it lies, 16 tokens a step: of half l / 32 the tokens 16 s + 4 (l / 32) + j and those 8 further, so
@@ -145,8 +145,8 @@ __device__ inline float sum_of_halves(float x) {
     return __builtin_bit_cast(float, a0) + __builtin_bit_cast(float, a1);
 }
 
-template <int D, int NS, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, WAVES == 4 && D * NS <= 128 ? 2 : 1) void attend_many_kernel(AttendArgs a, int tiles) {
+template <int D, int NS, int WAVES, int PAGES>
+__global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, int tiles) {
     typedef Images<D> I;
     typedef typename ElementOf<NS>::type E;
     constexpr int kRows = 32 * WAVES, kBuffer = I::kBytes + kPage;
@@ -196,53 +196,73 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && D * NS <= 128 ? 2 : 1) vo
         for (int i = 0; i < 16; i++) acc[d][i] = 0;
     float top = -INFINITY, sum = 0;
 
-    KeyPart<D> kp;
-    ValuePart<D> vp;
+    KeyPart<D> kp[PAGES];
+    ValuePart<D> vp[PAGES];
     const int id = threadIdx.x & 255;
     const bool brings_keys = WAVES == 4 || wave < 4, brings_values = WAVES == 4 || wave >= 4;
-    auto fetch = [&](int64_t page) {
-        if (brings_keys) fetch_keys<D>(kp, a.c, page * a.c.heads + h, id);
-        if (brings_values) fetch_values<D>(vp, a.c, page * a.c.heads + h, id);
+    auto fetch = [&](int k, int page) {
+        if (brings_keys) fetch_keys<D>(kp[k], a.c, (int64_t)page * a.c.heads + h, id);
+        if (brings_values) fetch_values<D>(vp[k], a.c, (int64_t)page * a.c.heads + h, id);
     };
-    auto is_edge = [&](int64_t page, int block) {
-        return page >= 0 && ((block + 1) * kPage > least || a.c.bound_scales[page * a.c.heads + h] == kBoundless);
-    };
-    auto store = [&](int buffer, int block, bool edge) {
+    auto store = [&](int k, int buffer, int block, bool edge) {
         char *const to = lds + buffer * kBuffer;
-        if (brings_keys) store_keys<D>(kp, to, id);
-        if (brings_values) store_values<D>(vp, to, (uint8_t *)to + I::kBytes, id, edge, length - block * kPage);
+        if (brings_keys) store_keys<D>(kp[k], to, id);
+        if (brings_values) store_values<D>(vp[k], to, (uint8_t *)to + I::kBytes, id, edge, length - block * kPage);
     };
 
     const int blocks = (most + kPage - 1) / kPage;
     const int from = (int)((int64_t)blocks * split / a.splits), to = (int)((int64_t)blocks * (split + 1) / a.splits);
-    int64_t page = from < to ? page_of(a.t, a.c, b, from) : -1;
-    bool edge = is_edge(page, from);
-    if (page >= 0) {
-        fetch(page);
-        store(0, from, edge);
+    // 64 blocks' pages are looked up at once, a lane each, and handed out as scalars: a lookup of the next page would be waited for
+    // at the head of every round
+    int pages = -1;
+    uint64_t edges = 0;
+    auto look_up = [&](int block) {
+        block += lane;
+        pages = block < to ? (int)page_of(a.t, a.c, b, block) : -1;
+        edges = __ballot(pages >= 0 && ((block + 1) * kPage > least || a.c.bound_scales[(int64_t)pages * a.c.heads + h] == kBoundless));
+    };
+    look_up(from);
+    int page[PAGES], next[PAGES];
+    uint32_t edge = 0, next_edge = 0;
+#pragma unroll
+    for (int k = 0; k < PAGES; k++) {
+        page[k] = __builtin_amdgcn_readlane(pages, k);
+        if (page[k] >= 0) fetch(k, page[k]);
     }
+    edge = (uint32_t)edges & ((1u << PAGES) - 1);
+#pragma unroll
+    for (int k = 0; k < PAGES; k++)
+        if (page[k] >= 0) store(k, k, from + k, edge >> k & 1);
     __syncthreads();
-    for (int block = from; block < to; block++) {
-        const int64_t next = block + 1 < to ? page_of(a.t, a.c, b, block + 1) : -1;
-        const bool next_edge = is_edge(next, block + 1);
-        if (next >= 0) fetch(next);
-        if (page >= 0) {
-            const char *const in = lds + (block - from & 1) * kBuffer;
+    for (int round = from, turn = 0; round < to; round += PAGES, turn ^= 1) {
+        const int at = round + PAGES - from & 63;
+        if (at == 0) look_up(round + PAGES);
+        next_edge = (uint32_t)(edges >> at) & ((1u << PAGES) - 1);
+#pragma unroll
+        for (int k = 0; k < PAGES; k++) {
+            next[k] = __builtin_amdgcn_readlane(pages, at + k);  // -1 behind the last
+            if (next[k] >= 0) fetch(k, next[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < PAGES; k++) {
+            if (page[k] < 0) continue;
+            const int block = round + k;
+            const char *const in = lds + (turn * PAGES + k) * kBuffer;
             f32x16 s[2];
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) s[t][i] = 0;
 #pragma unroll
-            for (int k = 0; k < D / 16; k++) {
+            for (int c = 0; c < D / 16; c++) {
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    const bf16x8 x = *reinterpret_cast<const bf16x8 *>(in + I::key(t * 32 + col, k * 2 + hi));
+                    const bf16x8 x = *reinterpret_cast<const bf16x8 *>(in + I::key(t * 32 + col, c * 2 + hi));
 #pragma unroll
-                    for (int n = 0; n < NS; n++) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, q[n][k], s[t], 0, 0, 0);
+                    for (int n = 0; n < NS; n++) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, q[n][c], s[t], 0, 0, 0);
                 }
             }
-            if (edge) {
+            if (edge >> k & 1) {
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -297,10 +317,13 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && D * NS <= 128 ? 2 : 1) vo
                 }
             }
         }
-        if (next >= 0) store(block + 1 - from & 1, block + 1, next_edge);
-        __syncthreads();
-        page = next;
+#pragma unroll
+        for (int k = 0; k < PAGES; k++) {
+            if (next[k] >= 0) store(k, (turn ^ 1) * PAGES + k, round + PAGES + k, next_edge >> k & 1);
+            page[k] = next[k];
+        }
         edge = next_edge;
+        __syncthreads();
     }
     sum = sum_of_halves(sum);
     if (!real) return;

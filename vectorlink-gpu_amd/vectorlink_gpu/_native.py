@@ -35,11 +35,12 @@ class Tokens(C.Structure):
 
 class Queries(C.Structure):
     _fields_ = [("heads", C.c_int64), ("row_stride", C.c_int64), ("head_stride", C.c_int64), ("queries", C.c_void_p),
-                ("out", C.c_void_p), ("lse", C.c_void_p), ("scale", C.c_double), ("type", C.c_int32), ("causal", C.c_int32)]
+                ("out", C.c_void_p), ("lse", C.c_void_p), ("scale", C.c_double), ("type", C.c_int32), ("causal", C.c_int32),
+                ("form", C.c_int64)]
 
 
 TYPES = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}  # VL_BF16, VL_F16, VL_F32
-ATTEND_FORMS = {"few": 0, "many": 1}  # VL_ATTEND_FEW, VL_ATTEND_MANY
+ATTEND_FORMS = {"few": 1, "many": 2}  # VL_ATTEND_FEW, VL_ATTEND_MANY
 METRICS = {"cosine": 0, "l2": 1}  # include/vlgpu.h: VL_METRIC_COSINE, VL_METRIC_L2
 KNN_FORMS = {"tiles": 0, "few": 1, "filter": 2}  # VL_KNN_TILES, VL_KNN_FEW, VL_KNN_FILTER
 KNN_ANY_SIZE = 256  # VL_KNN_ANY_SIZE

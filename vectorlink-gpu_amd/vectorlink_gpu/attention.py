@@ -116,11 +116,12 @@ class KVCache:
 
 
 def _queries(queries: Tensor, cache: KVCache, scale: Optional[float], causal: bool, out: Optional[Tensor],
-             lse: Optional[Tensor]) -> nv.Queries:
+             lse: Optional[Tensor], form: Optional[str] = None) -> nv.Queries:
     (row, head, _) = queries.stride()
     return nv.Queries(queries.shape[1], row, head, queries.data_ptr(), None if out is None else out.data_ptr(),
                       None if lse is None else lse.data_ptr(), cache.dim ** -0.5 if scale is None else scale,
-                      nv.TYPES[queries.dtype], causal)
+                      nv.TYPES[queries.dtype], causal,
+                      0 if form is None else nv.ATTEND_FORMS[form])
 
 
 def _check_queries(queries: Tensor, cache: KVCache):
@@ -134,17 +135,19 @@ def _workspace(need: int, beside: Tensor) -> Optional[Tensor]:
 
 
 def attend(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, offsets: Optional[Tensor] = None,
-           scale: Optional[float] = None, causal: bool = True, return_lse: bool = False):
+           scale: Optional[float] = None, causal: bool = True, return_lse: bool = False, form: Optional[str] = None):
     """softmax(scale * queries keys^T) values over the `lengths` [sequences] tokens that the cache holds.  queries [rows, heads,
     dim], heads a multiple of the cache's; scale defaults to dim ** -0.5.  The rows of a sequence are its last tokens and see
     what stands before them and themselves, or with causal=False everything.  A row that sees nothing gives zeros.  With
-    return_lse also the logarithms of the sums of exponentials [rows, heads], by which parts of an attention are joined."""
+    return_lse also the logarithms of the sums of exponentials [rows, heads], by which parts of an attention are joined.
+    form: the library chooses one by the sizes; "few" or "many" ask for it, for tests and measurements."""
+    assert form is None or form in nv.ATTEND_FORMS, f"unknown form {form!r}: expected one of {sorted(nv.ATTEND_FORMS)}"
     tokens = C.byref(_tokens(queries.shape[0], table, lengths, offsets))
     _check_queries(queries, cache)
     nv.require_gpu(queries, table, lengths, offsets)
     out = queries.new_empty(queries.shape)
     lse = queries.new_empty(queries.shape[:2], dtype=torch.float32) if return_lse else None
-    q = C.byref(_queries(queries, cache, scale, causal, out, lse))
+    q = C.byref(_queries(queries, cache, scale, causal, out, lse, form))
     lib = nv.lib()
     need = lib.vl_attend_workspace_bytes(cache._ref, tokens, q)
     ws = _workspace(need, queries)
