@@ -104,24 +104,31 @@ struct QueryRegs {
 };
 
 template <int D, int NS>
-__device__ inline void load_queries(QueryRegs<D, NS> &f, const AttendArgs &a, bool real, int64_t row, int head) {
+struct QueryLoads {
+    Eight<NS> x[D / 32];
+};
+template <int D, int NS>
+__device__ inline void load_queries(QueryLoads<D, NS> &l, const AttendArgs &a, bool real, int64_t row, int head) {
     typedef Parts<D> PT;
     typedef typename ElementOf<NS>::type E;
     const int q = (threadIdx.x & 63) >> 4;
     const E *const at = (const E *)a.queries + (real ? row * a.q_row + head * a.q_head : 0);
-    Eight<NS> x[D / 32];
 #pragma unroll
     for (int p = 0; p < PT::kCount; p++) {
         const int W = PT::width(p), base = PT::base(p);
 #pragma unroll
-        for (int j = 0; j < W / 32; j++) x[base / 32 + j] = load8<NS>(at + base + q * (W / 4) + j * 8, real);
+        for (int j = 0; j < W / 32; j++) l.x[base / 32 + j] = load8<NS>(at + base + q * (W / 4) + j * 8);
     }
+}
+template <int D, int NS>
+__device__ inline void take_queries(QueryRegs<D, NS> &f, const QueryLoads<D, NS> &l, bool real, uint32_t sign) {
+    typedef typename ElementOf<NS>::type E;
 #pragma unroll
     for (int k = 0; k < D / 32; k++) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             __bf16 s[NS];
-            split_into<NS>(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)x[k][i]) ^ a.sign), s);
+            split_into<NS>(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)(real ? l.x[k][i] : (E)0.0f)) ^ sign), s);
 #pragma unroll
             for (int n = 0; n < NS; n++) f.x[n][k][i] = s[n];
         }
@@ -249,24 +256,25 @@ struct Blocks {
 // loop would wait, in order, for the page's bytes that were asked for before it.  Where two pages fit the registers of two
 // wavefronts a SIMD, the next page's bytes are loaded before a page is worked on (64 dimensions: 61 us with one, 54 with two, 64
 // tokens over 4,096 to 8,192 and 8 heads; 128: 94 and 92; 96 spills); behind the last one the same page is loaded once more instead
-// of a branch, over which the compiler would have to wait for all loads.
+// of a branch, over which the compiler would have to wait for all loads.  The queries' loads are waited for with the first
+// page's.
 template <int D, int NS>
-__device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const QueryRegs<D, NS> &f, Blocks l, int b, int h, int sees,
-                                   int least, int most, int length) {
+__device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const QueryLoads<D, NS> &queries, bool real, Blocks l, int b,
+                                   int h, int sees, int least, int most, int length) {
     const int lane = threadIdx.x & 63;
+    QueryRegs<D, NS> f;
+    bool first = true;
     for (int i0 = l.from; i0 < l.to; i0 += 64 * l.step) {
         const int i = i0 + lane * l.step;
         int block = 0, page = -1;
-        bool edge = false;
         if (i < l.to) {
             block = l.list ? l.list[i] : i;
             page = (int)page_of(a.t, a.c, b, block);
             if (page >= 0 && block * kPage >= most) page = -1;
-            if (page >= 0) edge = (block + 1) * kPage > least || a.c.bound_scales[(int64_t)page * a.c.heads + h] == kBoundless;
         }
-        uint64_t left = __ballot(page >= 0);
-        const uint64_t edges = __ballot(edge);
+        uint64_t left = __ballot(page >= 0), edges = 0;
         if (!left) continue;
+        const int bound = a.c.bound_scales[(int64_t)max(page, 0) * a.c.heads + h];  // there is a page
         int at = 0;
         auto next = [&](PageRegs<D> &g) {  // the next page's loads
             if (left) {
@@ -279,10 +287,16 @@ __device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const Q
             const int first = __builtin_amdgcn_readlane(block, at) * kPage;
             take_page<D, NS>(st, g, f, a.scale, edges >> at & 1, sees - first, length - first);
         };
+        auto look = [&] {  // after the first page's loads
+            edges = __ballot(page >= 0 && ((block + 1) * kPage > least || bound == kBoundless));
+            if (first) take_queries<D, NS>(f, queries, real, a.sign);
+            first = false;
+        };
         PageRegs<D> x;
+        next(x);
+        look();
         if constexpr (D == 64 || D == 128) {
             PageRegs<D> y;
-            next(x);
             for (;;) {
                 int here = at;
                 bool last = !left;
@@ -296,9 +310,10 @@ __device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const Q
                 if (last) break;
             }
         } else {
-            while (left) {
-                next(x);
+            for (;;) {
                 take(x, at);
+                if (!left) break;
+                next(x);
             }
         }
     }
@@ -374,7 +389,8 @@ __device__ inline void join_waves(const RowState<D> &st, JoinLds<WAVES> &s, cons
 #pragma unroll
         for (int e = 0; e < 4; e++)
 #pragma unroll
-            for (int k = 0; k < W / 16; k++) s.sum[wave][r * kJoinPad + q * (W / 4) + e * (W / 16) + k] = st.acc[t0 + k][e];
+            for (int k = 0; k < W / 16; k += 2)
+                *reinterpret_cast<f32x2 *>(&s.sum[wave][r * kJoinPad + q * (W / 4) + e * (W / 16) + k]) = f32x2{st.acc[t0 + k][e], st.acc[t0 + k + 1][e]};
         __syncthreads();
         if (js * 8 < W && to >= 0) {
             float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -389,10 +405,11 @@ __device__ inline void join_waves(const RowState<D> &st, JoinLds<WAVES> &s, cons
 }
 
 // A tile is 16 rows of one head: of the queries of one token where there is a list, of all tokens of a sequence otherwise.
-// JOIN: the four wavefronts of a workgroup share a tile's blocks and are joined; else each has a tile of its own.
-template <int D, int NS, bool JOIN>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_few_kernel(AttendArgs a, int tiles) {
+// The WAVES wavefronts of a workgroup share a tile's blocks and are joined; 1: each of four has a tile of its own.
+template <int D, int NS, int WAVES>
+__global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 : 1) void attend_few_kernel(AttendArgs a, int tiles) {
     typedef Parts<D> PT;
+    constexpr bool JOIN = WAVES > 1;
     const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.y, split = JOIN ? blockIdx.x % a.splits : 0, tile = JOIN ? blockIdx.x / a.splits : blockIdx.x * 4 + wave;
@@ -428,22 +445,22 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attend_few_kernel(Atten
     most = __builtin_amdgcn_readfirstlane(most);
     least = __builtin_amdgcn_readfirstlane(least);
 
-    QueryRegs<D, NS> f;
+    QueryLoads<D, NS> f;
     load_queries<D, NS>(f, a, real, row0 + (int64_t)token, head);
     RowState<D> st;
     start_rows<D>(st);
     const int entries = a.list ? a.count : (most + kPage - 1) / kPage;
     const int from = (int)((int64_t)entries * split / a.splits), to = (int)((int64_t)entries * (split + 1) / a.splits);
     const int32_t *const list = a.list ? a.list + ((row0 + (int64_t)token0) * a.c.heads + h) * a.count : nullptr;
-    take_blocks<D, NS>(st, a, f, {list, JOIN ? from + wave : from, JOIN ? 4 : 1, to}, b, h, sees, least, most, length);
+    take_blocks<D, NS>(st, a, f, real, {list, JOIN ? from + wave : from, WAVES, to}, b, h, sees, least, most, length);
 
     auto out_row = [&](int r) {
         const int i = w.piece * 16 + r;
         return i < tokens * a.group ? (row0 + (int64_t)(token0 + i / a.group)) * a.heads_q + h * a.group + i % a.group : -1;
     };
     if constexpr (JOIN) {
-        __shared__ JoinLds<4> s_join;
-        join_waves<D, NS, 4>(st, s_join, a, split, out_row);
+        extern __shared__ char lds[];  // a JoinLds<WAVES>
+        join_waves<D, NS, WAVES>(st, *reinterpret_cast<JoinLds<WAVES> *>(lds), a, split, out_row);
     } else {
         const float total = sum_over_quads(st.sum);
         const int64_t to = out_row(r);

@@ -11,18 +11,28 @@ void launch_join(const AttendArgs &a, hipStream_t stream) {
 
 template <int NS>
 int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
-    VL_REQUIRE(tiles * (a.splits ? a.splits : 1) <= 4 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)tiles);
+    VL_REQUIRE(tiles * (a.splits > 0 ? a.splits : 1) <= 4 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)tiles);
+    hipError_t e = hipSuccess;
     for_dim(a.c.dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (a.splits) {
-            attend_few_kernel<D, NS, true><<<dim3((unsigned)(tiles * a.splits), (unsigned)a.c.heads), 256, 0, stream>>>(a, (int)tiles);
-            launch_join<D, NS>(a, stream);
-        } else {
+        const unsigned groups = (unsigned)(tiles * (a.splits > 0 ? a.splits : 1)), heads = (unsigned)a.c.heads;
+        if (a.splits == kWaveTiles) {
             AttendArgs one = a;
             one.splits = 1;
-            attend_few_kernel<D, NS, false><<<dim3((unsigned)((tiles + 3) / 4), (unsigned)a.c.heads), 256, 0, stream>>>(one, (int)tiles);
+            attend_few_kernel<D, NS, 1><<<dim3((unsigned)((tiles + 3) / 4), heads), 256, 0, stream>>>(one, (int)tiles);
+        } else if (a.splits == kWideTiles) {
+            AttendArgs one = a;
+            one.splits = 1;
+            if constexpr (D <= 128) {
+                e = vl_allow_lds(attend_few_kernel<D, NS, 8>, sizeof(JoinLds<8>));
+                if (e == hipSuccess) attend_few_kernel<D, NS, 8><<<dim3(groups, heads), 512, sizeof(JoinLds<8>), stream>>>(one, (int)tiles);
+            }
+        } else {
+            attend_few_kernel<D, NS, 4><<<dim3(groups, heads), 256, sizeof(JoinLds<4>), stream>>>(a, (int)tiles);
+            launch_join<D, NS>(a, stream);
         }
     });
+    VL_HIP(e);
     VL_LAUNCH_CHECK("attend_few_kernel");
     return VL_OK;
 }

@@ -24,6 +24,7 @@ __global__ __launch_bounds__(512) void attend_step_kernel(AttendArgs a, SelectAr
     const Standing at = standing_of(a.t, row);
     const int b = __builtin_amdgcn_readfirstlane(at.b), blocks = __builtin_amdgcn_readfirstlane(at.blocks);
     const Scored what = {b, h, at.token, 1, at.place0, at.length, row - at.token};
+    const bool real = r < a.group;
     score_blocks<D, NS, kStepWaves, false>(s, what, 0, blocks, keys, 0, s_score);
     __syncthreads();
     int32_t *const out = s.out + ((int64_t)row * a.c.heads + h) * s.count;
@@ -34,14 +35,13 @@ __global__ __launch_bounds__(512) void attend_step_kernel(AttendArgs a, SelectAr
     for (int i = found + threadIdx.x; i < s.count; i += 512) out[i] = VL_MAXINT;
     __syncthreads();
 
-    const bool real = r < a.group;
     const int sees = max(min(at.place0 + at.token + 1, at.length), 0);
-    QueryRegs<D, NS> f;
+    QueryLoads<D, NS> f;
     load_queries<D, NS>(f, a, real, row, h * a.group + r);
     RowState<D> st;
     start_rows<D>(st);
     const int most = __builtin_amdgcn_readfirstlane(sees), length = __builtin_amdgcn_readfirstlane(at.length);
-    take_blocks<D, NS>(st, a, f, {list, wave, kStepWaves, found}, b, h, real ? sees : 0, most, most, length);
+    take_blocks<D, NS>(st, a, f, real, {list, wave, kStepWaves, found}, b, h, real ? sees : 0, most, most, length);
     __syncthreads();
     join_waves<D, NS, kStepWaves>(st, *(Join *)lds, a, 0, [&](int r) { return r < a.group ? (int64_t)row * a.heads_q + h * a.group + r : -1; });
 }
