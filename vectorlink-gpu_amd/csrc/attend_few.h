@@ -135,13 +135,67 @@ __device__ inline void take_queries(QueryRegs<D, NS> &f, const QueryLoads<D, NS>
     }
 }
 
-// Tokens of a page: see(token) says whether this lane's row sees the token's place in the page; edge: some row does not see
-// some token, or some token may not be finite.  spoilt tokens (scale 255) turn the rows that see them into NaN, and no others.
-template <int D, int NS>
+// Where a tile has at most C = 4 or 8 rows, three quarters or half of the lanes of S^T hold nothing, and the softmax of it would
+// cost as much as that of 16.  Scores then move to where they fill the lanes: of lane (q, r) row r % C, and of its 16 tokens the
+// tiles m = (C / 4) (r / C) + k.  Exponentials and all that is around them are C / 16 of the work, for 12 (C = 4) or 8 moves of a
+// register there and 12 or 8 back: of 560 vector instructions a page 470 are left with C = 4.
+template <int C>
+__device__ inline void spread_scores(const f32x4 (&s)[4], float (&t)[C / 4][4]) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        auto moved = [](float to, float from, auto control, auto banks) {
+            return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, to), __builtin_bit_cast(int, from),
+                                                                         decltype(control)::value, 0xF, decltype(banks)::value, false));
+        };
+        const float x0 = s[0][e], x1 = s[1][e], x2 = s[2][e], x3 = s[3][e];
+        if constexpr (C == 4) {  // row_shr: 4, 8, 12 into the second, third and fourth 4 lanes of a row
+            t[0][e] = moved(x0, x1, std::integral_constant<int, 0x114>(), std::integral_constant<int, 2>());
+            t[0][e] = moved(t[0][e], x2, std::integral_constant<int, 0x118>(), std::integral_constant<int, 4>());
+            t[0][e] = moved(t[0][e], x3, std::integral_constant<int, 0x11C>(), std::integral_constant<int, 8>());
+        } else if constexpr (C == 8) {
+            t[0][e] = moved(x0, x2, std::integral_constant<int, 0x118>(), std::integral_constant<int, 12>());
+            t[1][e] = moved(x1, x3, std::integral_constant<int, 0x118>(), std::integral_constant<int, 12>());
+        } else {
+            t[0][e] = x0, t[1][e] = x1, t[2][e] = x2, t[3][e] = x3;
+        }
+    }
+}
+// The way back, for the word that tile m = (C / 4) (r / C) + k has of a row: lane (q, r < C) gets those of all four tiles.
+template <int C>
+__device__ inline void gather_words(const uint32_t (&u)[C / 4], uint32_t (&w)[4]) {
+    if constexpr (C == 4) {  // row_shl: 4, 8, 12
+        w[0] = u[0];
+        w[1] = __builtin_amdgcn_update_dpp(0, (int)u[0], 0x104, 0xF, 0xF, false);
+        w[2] = __builtin_amdgcn_update_dpp(0, (int)u[0], 0x108, 0xF, 0xF, false);
+        w[3] = __builtin_amdgcn_update_dpp(0, (int)u[0], 0x10C, 0xF, 0xF, false);
+    } else if constexpr (C == 8) {
+        w[0] = u[0], w[1] = u[1];
+        w[2] = __builtin_amdgcn_update_dpp(0, (int)u[0], 0x108, 0xF, 0xF, false);
+        w[3] = __builtin_amdgcn_update_dpp(0, (int)u[1], 0x108, 0xF, 0xF, false);
+    } else {
+        w[0] = u[0], w[1] = u[1], w[2] = u[2], w[3] = u[3];
+    }
+}
+// f over the lanes of a row of 16 that hold the same row of the tile
+template <int C, class F>
+__device__ inline float over_copies(float x, F f) {
+    auto turned = [](float x, auto control) {  // row_ror
+        const int u = __builtin_bit_cast(int, x);
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(u, u, decltype(control)::value, 0xF, 0xF, false));
+    };
+    if constexpr (C <= 8) x = f(x, turned(x, std::integral_constant<int, 0x128>()));
+    if constexpr (C == 4) x = f(x, turned(x, std::integral_constant<int, 0x124>()));
+    return x;
+}
+
+// A page's 64 tokens: this lane's row (r % C) sees the first `sees` of them, `written` hold something; edge: some row does not see
+// some token, or some token may not be finite.  Spoilt tokens (scale 255) turn the rows that see them into NaN, and no others.
+template <int D, int NS, int C>
 __device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryRegs<D, NS> &f, float scale, bool edge, int sees,
                                  int written) {
     typedef Parts<D> PT;
     constexpr int NW = NS < 2 ? 2 : NS;  // parts of a weight
+    constexpr int M = C / 4;             // tiles of 4 tokens of this lane
     const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
     f32x4 s[4];
     const int turn = (8 * (r & 3) + 9) & 31;
@@ -159,28 +213,40 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryReg
                     s[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, f.x[n][PT::base(p) / 32 + j], s[m], 0, 0, 0);
             }
         }
-        s[m] *= scale;
     }
-    if (edge) {
+    float t[M][4];
+    spread_scores<C>(s, t);
 #pragma unroll
-        for (int m = 0; m < 4; m++) {
+    for (int k = 0; k < M; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) t[k][e] *= scale;
+    if (edge) {
+        const int m0 = M * (r / C);
+#pragma unroll
+        for (int k = 0; k < M; k++) {
+            uint32_t word = g.vs[0][k];
+            if constexpr (C == 4) word = r < 4 ? g.vs[0][0] : r < 8 ? g.vs[0][1] : r < 12 ? g.vs[0][2] : g.vs[0][3];
+            if constexpr (C == 8) word = r < 8 ? g.vs[0][k] : g.vs[0][2 + k];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const int token = q * 16 + m * 4 + e;
-                const uint32_t byte = g.vs[0][m] >> (8 * e) & 255;
-                if (byte == kNotFinite) s[m][e] = NAN;
-                if (token >= sees) s[m][e] = -INFINITY;
-                if (byte == kNotFinite || token >= written) {
-                    // its weight is 0 or NaN whatever it holds: any finite value will do
-#pragma unroll
-                    for (int p = 0; p < PT::kCount; p++) g.vs[p][m] = g.vs[p][m] & ~(255u << (8 * e)) | (127u << (8 * e));
-                }
+                if ((word >> (8 * e) & 255) == kNotFinite) t[k][e] = NAN;
+                if (q * 16 + (m0 + k) * 4 + e >= sees) t[k][e] = -INFINITY;
             }
         }
-    }
-    float top = s[0][0];
+        // values of a token that is spoilt or not there: its weight is 0 or NaN whatever it holds, so any finite value will do
 #pragma unroll
-    for (int i = 1; i < 16; i++) top = fmaxf(top, s[i >> 2][i & 3]);
+        for (int m = 0; m < 4; m++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if ((g.vs[0][m] >> (8 * e) & 255) == kNotFinite || q * 16 + m * 4 + e >= written) {
+#pragma unroll
+                    for (int p = 0; p < PT::kCount; p++) g.vs[p][m] = (g.vs[p][m] & ~(255u << (8 * e))) | (127u << (8 * e));
+                }
+    }
+    float top = t[0][0];
+#pragma unroll
+    for (int i = 1; i < 4 * M; i++) top = fmaxf(top, t[i >> 2][i & 3]);
+    top = over_copies<C>(top, [](float a, float b) { return fmaxf(a, b); });
     top = fmaxf(max_over_quads(top), st.top);
     if (__ballot(top > st.top)) {
         const float less = top > -INFINITY ? __builtin_amdgcn_exp2f(st.top - top) : 1.0f;
@@ -190,22 +256,34 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryReg
         for (int k = 0; k < D / 16; k++) st.acc[k] *= less;
     }
     const float from = st.top > -INFINITY ? st.top : 0.0f;  // a row that has seen nothing yet: all weights 0
+    uint32_t weight[NW][2][4];  // [part][two tokens][tile]
+    {
+        uint32_t pair[NW][2][M];
 #pragma unroll
-    for (int m = 0; m < 4; m++) {
+        for (int k = 0; k < M; k++) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[m][e] = __builtin_amdgcn_exp2f(s[m][e] - from);
-        st.sum += (s[m][0] + s[m][1]) + (s[m][2] + s[m][3]);
+            for (int e = 0; e < 4; e++) t[k][e] = __builtin_amdgcn_exp2f(t[k][e] - from);
+            st.sum += (t[k][0] + t[k][1]) + (t[k][2] + t[k][3]);
+#pragma unroll
+            for (int two = 0; two < 2; two++) {
+                __bf16 a[NW], b[NW];
+                split_into<NW>(t[k][2 * two], a);
+                split_into<NW>(t[k][2 * two + 1], b);
+#pragma unroll
+                for (int n = 0; n < NW; n++) pair[n][two][k] = __builtin_bit_cast(uint32_t, bf16x2{a[n], b[n]});
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NW; n++)
+#pragma unroll
+            for (int two = 0; two < 2; two++) gather_words<C>(pair[n][two], weight[n][two]);
     }
 #pragma unroll
     for (int h = 0; h < 2; h++) {  // 32 tokens a step: of every quad 8
         bf16x8 w[NW];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            __bf16 x[NW];
-            split_into<NW>(s[2 * h + (i >> 2)][i & 3], x);
-#pragma unroll
-            for (int n = 0; n < NW; n++) w[n][i] = x[n];
-        }
+        for (int n = 0; n < NW; n++)
+            w[n] = __builtin_bit_cast(bf16x8, u32x4{weight[n][0][2 * h], weight[n][1][2 * h], weight[n][0][2 * h + 1], weight[n][1][2 * h + 1]});
         auto product = [&](int tile, u32x4 a) {
 #pragma unroll
             for (int n = 0; n < NW; n++)
@@ -258,7 +336,7 @@ struct Blocks {
 // tokens over 4,096 to 8,192 and 8 heads; 128: 94 and 92; 96 spills); behind the last one the same page is loaded once more instead
 // of a branch, over which the compiler would have to wait for all loads.  The queries' loads are waited for with the first
 // page's.
-template <int D, int NS>
+template <int D, int NS, int C>
 __device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const QueryLoads<D, NS> &queries, bool real, Blocks l, int b,
                                    int h, int sees, int least, int most, int length) {
     const int lane = threadIdx.x & 63;
@@ -285,7 +363,7 @@ __device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const Q
         };
         auto take = [&](PageRegs<D> &g, int at) {
             const int first = __builtin_amdgcn_readlane(block, at) * kPage;
-            take_page<D, NS>(st, g, f, a.scale, edges >> at & 1, sees - first, length - first);
+            take_page<D, NS, C>(st, g, f, a.scale, edges >> at & 1, sees - first, length - first);
         };
         auto look = [&] {  // after the first page's loads
             edges = __ballot(page >= 0 && ((block + 1) * kPage > least || bound == kBoundless));
@@ -317,6 +395,11 @@ __device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const Q
             }
         }
     }
+}
+
+template <int C>
+__device__ inline float sum_of_row(float x) {
+    return sum_over_quads(over_copies<C>(x, [](float a, float b) { return a + b; }));
 }
 
 template <int D>
@@ -360,11 +443,11 @@ struct JoinLds {
     float sum[WAVES][16 * kJoinPad];
     float top[WAVES][16], all[WAVES][16];
 };
-template <int D, int NS, int WAVES, class F>
+template <int D, int NS, int WAVES, int C, class F>
 __device__ inline void join_waves(const RowState<D> &st, JoinLds<WAVES> &s, const AttendArgs &a, int split, F out_row) {
     typedef Parts<D> PT;
     const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15, wave = threadIdx.x >> 6;
-    const float sum = sum_over_quads(st.sum);
+    const float sum = sum_of_row<C>(st.sum);
     if (q == 0) {
         s.top[wave][r] = st.top;
         s.all[wave][r] = sum;
@@ -405,8 +488,9 @@ __device__ inline void join_waves(const RowState<D> &st, JoinLds<WAVES> &s, cons
 }
 
 // A tile is 16 rows of one head: of the queries of one token where there is a list, of all tokens of a sequence otherwise.
-// The WAVES wavefronts of a workgroup share a tile's blocks and are joined; 1: each of four has a tile of its own.
-template <int D, int NS, int WAVES>
+// The WAVES wavefronts of a workgroup share a tile's blocks and are joined; 1: each of four has a tile of its own.  C: the most
+// rows that a tile has, 16 unless its rows are one token's, which see the same.
+template <int D, int NS, int WAVES, int C>
 __global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 : 1) void attend_few_kernel(AttendArgs a, int tiles) {
     typedef Parts<D> PT;
     constexpr bool JOIN = WAVES > 1;
@@ -452,7 +536,7 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 
     const int entries = a.list ? a.count : (most + kPage - 1) / kPage;
     const int from = (int)((int64_t)entries * split / a.splits), to = (int)((int64_t)entries * (split + 1) / a.splits);
     const int32_t *const list = a.list ? a.list + ((row0 + (int64_t)token0) * a.c.heads + h) * a.count : nullptr;
-    take_blocks<D, NS>(st, a, f, real, {list, JOIN ? from + wave : from, WAVES, to}, b, h, sees, least, most, length);
+    take_blocks<D, NS, C>(st, a, f, real, {list, JOIN ? from + wave : from, WAVES, to}, b, h, C < 16 ? most : sees, least, most, length);
 
     auto out_row = [&](int r) {
         const int i = w.piece * 16 + r;
@@ -460,9 +544,9 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 
     };
     if constexpr (JOIN) {
         extern __shared__ char lds[];  // a JoinLds<WAVES>
-        join_waves<D, NS, WAVES>(st, *reinterpret_cast<JoinLds<WAVES> *>(lds), a, split, out_row);
+        join_waves<D, NS, WAVES, C>(st, *reinterpret_cast<JoinLds<WAVES> *>(lds), a, split, out_row);
     } else {
-        const float total = sum_over_quads(st.sum);
+        const float total = sum_of_row<C>(st.sum);
         const int64_t to = out_row(r);
         if (to < 0) return;
 #pragma unroll

@@ -4,6 +4,14 @@
 #include "attend_many.h"
 #include "attend_step.h"
 
+// f(std::integral_constant<int, C>) for tiles of at most `rows` rows
+template <class F>
+void for_rows(int rows, F f) {
+    if (rows <= 4) f(std::integral_constant<int, 4>());
+    else if (rows <= 8) f(std::integral_constant<int, 8>());
+    else f(std::integral_constant<int, 16>());
+}
+
 template <int D, int NS>
 void launch_join(const AttendArgs &a, hipStream_t stream) {
     if (a.splits > 1) attend_join_kernel<D, NS><<<(unsigned)(((int64_t)a.t.rows * a.heads_q + 3) / 4), 256, 0, stream>>>(a);
@@ -16,21 +24,22 @@ int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
     for_dim(a.c.dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
         const unsigned groups = (unsigned)(tiles * (a.splits > 0 ? a.splits : 1)), heads = (unsigned)a.c.heads;
-        if (a.splits == kWaveTiles) {
-            AttendArgs one = a;
-            one.splits = 1;
-            attend_few_kernel<D, NS, 1><<<dim3((unsigned)((tiles + 3) / 4), heads), 256, 0, stream>>>(one, (int)tiles);
-        } else if (a.splits == kWideTiles) {
-            AttendArgs one = a;
-            one.splits = 1;
-            if constexpr (D <= 128) {
-                e = vl_allow_lds(attend_few_kernel<D, NS, 8>, sizeof(JoinLds<8>));
-                if (e == hipSuccess) attend_few_kernel<D, NS, 8><<<dim3(groups, heads), 512, sizeof(JoinLds<8>), stream>>>(one, (int)tiles);
+        AttendArgs one = a;
+        one.splits = a.splits > 0 ? a.splits : 1;
+        for_rows(a.list || !a.t.offsets ? a.group : 16, [&](auto c) {
+            constexpr int C = decltype(c)::value;
+            if (a.splits == kWaveTiles) {
+                attend_few_kernel<D, NS, 1, C><<<dim3((unsigned)((tiles + 3) / 4), heads), 256, 0, stream>>>(one, (int)tiles);
+            } else if (a.splits == kWideTiles) {
+                if constexpr (D <= 128) {
+                    e = vl_allow_lds(attend_few_kernel<D, NS, 8, C>, sizeof(JoinLds<8>));
+                    if (e == hipSuccess) attend_few_kernel<D, NS, 8, C><<<dim3(groups, heads), 512, sizeof(JoinLds<8>), stream>>>(one, (int)tiles);
+                }
+            } else {
+                attend_few_kernel<D, NS, 4, C><<<dim3(groups, heads), 256, sizeof(JoinLds<4>), stream>>>(one, (int)tiles);
             }
-        } else {
-            attend_few_kernel<D, NS, 4><<<dim3(groups, heads), 256, sizeof(JoinLds<4>), stream>>>(a, (int)tiles);
-            launch_join<D, NS>(a, stream);
-        }
+        });
+        launch_join<D, NS>(a, stream);
     });
     VL_HIP(e);
     VL_LAUNCH_CHECK("attend_few_kernel");
@@ -64,8 +73,11 @@ int launch_attend_step(const AttendArgs &a, const SelectArgs &s, hipStream_t str
     const size_t lds = (keys > join ? keys : join) + (size_t)s.count * 4;
     for_dim(a.c.dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        e = vl_allow_lds(attend_step_kernel<D, NS>, lds);
-        if (e == hipSuccess) attend_step_kernel<D, NS><<<(unsigned)(a.t.rows * (int64_t)a.c.heads), 512, lds, stream>>>(a, s);
+        for_rows(a.group, [&](auto c) {
+            constexpr int C = decltype(c)::value;
+            e = vl_allow_lds(attend_step_kernel<D, NS, C>, lds);
+            if (e == hipSuccess) attend_step_kernel<D, NS, C><<<(unsigned)(a.t.rows * (int64_t)a.c.heads), 512, lds, stream>>>(a, s);
+        });
     });
     VL_HIP(e);
     VL_LAUNCH_CHECK("attend_step_kernel");

@@ -8,7 +8,7 @@
 
 constexpr int kStepWaves = 8;
 
-template <int D, int NS>
+template <int D, int NS, int C>
 __global__ __launch_bounds__(512) void attend_step_kernel(AttendArgs a, SelectArgs s) {
     typedef JoinLds<kStepWaves> Join;
     extern __shared__ char lds[];  // scores [blocks] and then the join's sums; behind them the list [count]
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(512) void attend_step_kernel(AttendArgs a, SelectAr
     RowState<D> st;
     start_rows<D>(st);
     const int most = __builtin_amdgcn_readfirstlane(sees), length = __builtin_amdgcn_readfirstlane(at.length);
-    take_blocks<D, NS>(st, a, f, real, {list, wave, kStepWaves, found}, b, h, real ? sees : 0, most, most, length);
+    take_blocks<D, NS, C>(st, a, f, real, {list, wave, kStepWaves, found}, b, h, C < 16 || real ? sees : 0, most, most, length);
     __syncthreads();
-    join_waves<D, NS, kStepWaves>(st, *(Join *)lds, a, 0, [&](int r) { return r < a.group ? (int64_t)row * a.heads_q + h * a.group + r : -1; });
+    join_waves<D, NS, kStepWaves, C>(st, *(Join *)lds, a, 0, [&](int r) { return r < a.group ? (int64_t)row * a.heads_q + h * a.group + r : -1; });
 }
