@@ -34,7 +34,8 @@ constexpr bool many_built(int dim, int parts) { return dim * parts <= 256; }
 constexpr int many_pages(int dim) { return dim <= 128 ? 2 : 1; }
 template <int NS>
 int launch_attend_many(const AttendArgs &a, int64_t tiles, hipStream_t stream);
-// a choice of blocks and attention over it, a workgroup for a token and head
+// a choice of blocks and attention over it, a workgroup for a token and head; longer rows of other types do not fit the registers
+constexpr bool step_built(int dim, int parts) { return dim <= 128 || parts == 1; }
 template <int NS>
 int launch_attend_step(const AttendArgs &a, const SelectArgs &s, hipStream_t stream);
 extern template int launch_attend_few<1>(const AttendArgs &, int64_t, hipStream_t);

@@ -154,9 +154,9 @@ int choose(const AttendArgs &a, int type, int64_t count, int32_t *blocks, void *
 }
 
 // Whether attend_step_kernel takes a choice and the attention over it: few tokens, and for one workgroup not too many bytes.
-bool in_one_step(const AttendArgs &a, int64_t count) {
+bool in_one_step(const AttendArgs &a, int type, int64_t count) {
     const int64_t items = (int64_t)a.t.rows * a.c.heads, bytes = (int64_t)a.t.blocks * 2 * a.c.dim + count * kPage * (a.c.dim + a.c.dim / 16);
-    return a.group <= 16 && a.t.blocks <= 16384 && count <= 2048 && items <= kStepItems &&
+    return step_built(a.c.dim, type) && a.group <= 16 && a.t.blocks <= 16384 && count <= 2048 && items <= kStepItems &&
            (bytes <= kStepBytes || items >= kStepFull);
 }
 
@@ -230,7 +230,7 @@ VL_EXPORT int64_t vl_attend_selected_workspace_bytes(const vl_cache *cache, cons
     int rc = attend_args(cache, tokens, queries, false, &a);
     if (rc == VL_OK) rc = check_count(count);
     if (rc != VL_OK) return rc;
-    if (in_one_step(a, count)) return 0;
+    if (in_one_step(a, queries->type, count)) return 0;
     a.count = (int)count;
     return select_workspace_bytes(select_args(a, count)) + part_bytes(a, splits_for(a, few_tiles(a)));
 }
@@ -241,7 +241,7 @@ VL_EXPORT int vl_attend_selected(const vl_cache *cache, const vl_tokens *tokens,
     int rc = attend_args(cache, tokens, queries, true, &a);
     if (rc == VL_OK) rc = check_count(count);
     if (rc != VL_OK || a.t.rows == 0) return rc;
-    if (in_one_step(a, count)) {
+    if (in_one_step(a, queries->type, count)) {
         VL_REQUIRE(blocks, "blocks is null");
         SelectArgs s = select_args(a, count);
         s.out = blocks;

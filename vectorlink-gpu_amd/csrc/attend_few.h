@@ -199,19 +199,24 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryReg
     const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
     f32x4 s[4];
     const int turn = (8 * (r & 3) + 9) & 31;
+    // products that add to the same sums lie four apart: one waits for the other's result
 #pragma unroll
-    for (int m = 0; m < 4; m++) {
-        s[m] = f32x4{0, 0, 0, 0};
+    for (int m = 0; m < 4; m++) s[m] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int p = 0; p < PT::kCount; p++) {
-            const float ks = __builtin_bit_cast(float, __builtin_amdgcn_alignbit(g.ks[p][m], g.ks[p][m], turn));
+    for (int p = 0; p < PT::kCount; p++) {
+        float ks[4];
 #pragma unroll
-            for (int j = 0; j < PT::width(p) / 32; j++) {
-                const bf16x8 k = eight_values(g.k[p][m][j], ks);
+        for (int m = 0; m < 4; m++) ks[m] = __builtin_bit_cast(float, __builtin_amdgcn_alignbit(g.ks[p][m], g.ks[p][m], turn));
 #pragma unroll
-                for (int n = 0; n < NS; n++)
-                    s[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, f.x[n][PT::base(p) / 32 + j], s[m], 0, 0, 0);
-            }
+        for (int j = 0; j < PT::width(p) / 32; j++) {
+            bf16x8 k[4];
+#pragma unroll
+            for (int m = 0; m < 4; m++) k[m] = eight_values(g.k[p][m][j], ks[m]);
+#pragma unroll
+            for (int n = 0; n < NS; n++)
+#pragma unroll
+                for (int m = 0; m < 4; m++)
+                    s[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[m], f.x[n][PT::base(p) / 32 + j], s[m], 0, 0, 0);
         }
     }
     float t[M][4];
@@ -284,11 +289,6 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryReg
 #pragma unroll
         for (int n = 0; n < NW; n++)
             w[n] = __builtin_bit_cast(bf16x8, u32x4{weight[n][0][2 * h], weight[n][1][2 * h], weight[n][0][2 * h + 1], weight[n][1][2 * h + 1]});
-        auto product = [&](int tile, u32x4 a) {
-#pragma unroll
-            for (int n = 0; n < NW; n++)
-                st.acc[tile] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), w[n], st.acc[tile], 0, 0, 0);
-        };
 #pragma unroll
         for (int p = 0; p < PT::kCount; p++) {
             const int W = PT::width(p), t0 = PT::base(p) / 16;
@@ -302,23 +302,32 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryReg
                 if (W == 32) word[u] >>= 8 * (r & 3);
                 vs[u] = scale_at(g.vs[p][m], u & 3);
             }
-#define VL_TWO_TILES(B)                                                                     \
-    if (B < W / 32) {                                                                       \
-        u32x4 even, odd;                                                                    \
-        _Pragma("unroll") for (int i = 0; i < 4; i++) {                                     \
-            const uint32_t x = two_values<B>(word[2 * i], vs[2 * i]);                       \
-            const uint32_t y = two_values<B>(word[2 * i + 1], vs[2 * i + 1]);               \
-            even[i] = __builtin_amdgcn_perm(y, x, 0x05040100);                              \
-            odd[i] = __builtin_amdgcn_perm(y, x, 0x07060302);                               \
-        }                                                                                   \
-        product(t0 + 2 * B, even);                                                          \
-        product(t0 + 2 * B + 1, odd);                                                       \
-    }
-            VL_TWO_TILES(0)
-            VL_TWO_TILES(1)
-            VL_TWO_TILES(2)
-            VL_TWO_TILES(3)
-#undef VL_TWO_TILES
+            // byte B of the words: dimensions of tiles 2 B and 2 B + 1
+            auto two_tiles = [&](auto byte, u32x4(&a)[2]) {
+                constexpr int B = decltype(byte)::value;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t x = two_values<B>(word[2 * i], vs[2 * i]), y = two_values<B>(word[2 * i + 1], vs[2 * i + 1]);
+                    a[0][i] = __builtin_amdgcn_perm(y, x, 0x05040100);
+                    a[1][i] = __builtin_amdgcn_perm(y, x, 0x07060302);
+                }
+            };
+            auto products = [&](int tile, const u32x4(&a)[2][2], int tiles) {
+#pragma unroll
+                for (int n = 0; n < NW; n++)
+#pragma unroll
+                    for (int k = 0; k < tiles; k++)
+                        st.acc[tile + k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[k >> 1][k & 1]), w[n], st.acc[tile + k], 0, 0, 0);
+            };
+            u32x4 a[2][2];
+            two_tiles(std::integral_constant<int, 0>(), a[0]);
+            if (W >= 64) two_tiles(std::integral_constant<int, 1>(), a[1]);
+            products(t0, a, W >= 64 ? 4 : 2);
+            if (W >= 128) {
+                two_tiles(std::integral_constant<int, 2>(), a[0]);
+                two_tiles(std::integral_constant<int, 3>(), a[1]);
+                products(t0 + 4, a, 4);
+            }
         }
     }
 }
@@ -333,7 +342,7 @@ struct Blocks {
 // All of a wavefront's blocks.  64 blocks' pages are looked up at once, a lane each, and handed out as scalars: a lookup in the
 // loop would wait, in order, for the page's bytes that were asked for before it.  Where two pages fit the registers of two
 // wavefronts a SIMD, the next page's bytes are loaded before a page is worked on (64 dimensions: 61 us with one, 54 with two, 64
-// tokens over 4,096 to 8,192 and 8 heads; 128: 94 and 92; 96 spills); behind the last one the same page is loaded once more instead
+// tokens over 4,096 to 8,192 and 8 heads; 128: 94 and 92; 96, and 128 of float32, spill); behind the last one the same page is loaded once more instead
 // of a branch, over which the compiler would have to wait for all loads.  The queries' loads are waited for with the first
 // page's.
 template <int D, int NS, int C>
@@ -373,7 +382,7 @@ __device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const Q
         PageRegs<D> x;
         next(x);
         look();
-        if constexpr (D == 64 || D == 128) {
+        if constexpr (D == 64 || (D == 128 && NS < 3)) {
             PageRegs<D> y;
             for (;;) {
                 int here = at;

@@ -73,11 +73,13 @@ int launch_attend_step(const AttendArgs &a, const SelectArgs &s, hipStream_t str
     const size_t lds = (keys > join ? keys : join) + (size_t)s.count * 4;
     for_dim(a.c.dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        for_rows(a.group, [&](auto c) {
-            constexpr int C = decltype(c)::value;
-            e = vl_allow_lds(attend_step_kernel<D, NS, C>, lds);
-            if (e == hipSuccess) attend_step_kernel<D, NS, C><<<(unsigned)(a.t.rows * (int64_t)a.c.heads), 512, lds, stream>>>(a, s);
-        });
+        if constexpr (step_built(D, NS)) {
+            for_rows(a.group, [&](auto c) {
+                constexpr int C = decltype(c)::value;
+                e = vl_allow_lds(attend_step_kernel<D, NS, C>, lds);
+                if (e == hipSuccess) attend_step_kernel<D, NS, C><<<(unsigned)(a.t.rows * (int64_t)a.c.heads), 512, lds, stream>>>(a, s);
+            });
+        }
     });
     VL_HIP(e);
     VL_LAUNCH_CHECK("attend_step_kernel");

@@ -255,12 +255,14 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
                 for (int i = 0; i < 16; i++) s[t][i] = 0;
 #pragma unroll
             for (int c = 0; c < D / 16; c++) {
+                // products that add to the same sums do not follow each other: one waits for the other's result
+                bf16x8 x[2];
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const bf16x8 x = *reinterpret_cast<const bf16x8 *>(in + I::key(t * 32 + col, c * 2 + hi));
+                for (int t = 0; t < 2; t++) x[t] = *reinterpret_cast<const bf16x8 *>(in + I::key(t * 32 + col, c * 2 + hi));
 #pragma unroll
-                    for (int n = 0; n < NS; n++) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, q[n][c], s[t], 0, 0, 0);
-                }
+                for (int n = 0; n < NS; n++)
+#pragma unroll
+                    for (int t = 0; t < 2; t++) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[t], q[n][c], s[t], 0, 0, 0);
             }
             if (edge >> k & 1) {
 #pragma unroll
@@ -309,12 +311,13 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
 #pragma unroll
                     for (int n = 0; n < NW; n++) p[n][i] = x[n];
                 }
+                bf16x8 v[D / 32];
 #pragma unroll
-                for (int d = 0; d < D / 32; d++) {
-                    const bf16x8 v = *reinterpret_cast<const bf16x8 *>(in + I::value(d * 32 + col, step * 2 + hi));
+                for (int d = 0; d < D / 32; d++) v[d] = *reinterpret_cast<const bf16x8 *>(in + I::value(d * 32 + col, step * 2 + hi));
 #pragma unroll
-                    for (int n = 0; n < NW; n++) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p[n], acc[d], 0, 0, 0);
-                }
+                for (int n = 0; n < NW; n++)
+#pragma unroll
+                    for (int d = 0; d < D / 32; d++) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[d], p[n], acc[d], 0, 0, 0);
             }
         }
 #pragma unroll
