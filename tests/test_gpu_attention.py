@@ -450,3 +450,21 @@ def test_captured_steps():
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(cache.keys, image)
         assert torch.equal(state, before + 1)
+
+
+def test_the_example_runs():
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "vectorlink-gpu_amd", "attend.py")
+    spec = importlib.util.spec_from_file_location("attend_example", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    options = example.parse(["-c", "1500", "-b", "2", "-n", "2", "-d", "64", "-k", "8", "-p", "600", "-s", "4"])
+    report = example.main(options)
+    # codes of three magnitude bits: a quarter of a step of a sixth at most, and the token's subject dominates what is chosen
+    assert report["blocks"] == 24 and 0.0 < report["keys_off"] < 0.2 and 0.0 < report["values_off"] < 0.2
+    assert 0.0 < report["chosen_off"] < 1.0
+    # all blocks chosen: the same tokens, joined in another order
+    everything = example.main(dict(options, count=24))
+    assert everything["chosen_off"] < 2.0 ** -7

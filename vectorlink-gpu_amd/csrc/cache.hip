@@ -39,40 +39,75 @@ struct Rows {  // [rows, heads, dim] of a call
     int64_t row, head;
 };
 
+__device__ inline uint32_t max_of_four_lanes(uint32_t x) {  // lanes 4 n ... 4 n + 3
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, false));  // quad_perm: [1, 0, 3, 2]
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, false));  // [2, 3, 0, 1]
+}
+
+// The largest magnitude of a group, 8 elements of each of four lanes, as the bits of a float32: a NaN above an infinity above all
+// others.  Magnitudes of 16 bits are compared two at a time as whole numbers, which have the same order.
+template <int NS>
+__device__ inline uint32_t top_of_group(const Eight<NS> &v) {
+    if constexpr (NS == 3) {
+        const u32x4 a = {__builtin_bit_cast(uint32_t, (float)v[0]), __builtin_bit_cast(uint32_t, (float)v[1]),
+                         __builtin_bit_cast(uint32_t, (float)v[2]), __builtin_bit_cast(uint32_t, (float)v[3])};
+        const u32x4 b = {__builtin_bit_cast(uint32_t, (float)v[4]), __builtin_bit_cast(uint32_t, (float)v[5]),
+                         __builtin_bit_cast(uint32_t, (float)v[6]), __builtin_bit_cast(uint32_t, (float)v[7])};
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) top = max(top, max(a[i] & 0x7FFFFFFFu, b[i] & 0x7FFFFFFFu));
+        return max_of_four_lanes(top);
+    } else {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        const u32x4 w = __builtin_bit_cast(u32x4, v) & 0x7FFF7FFFu;
+        const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3];
+        const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(__builtin_bit_cast(u16x2, w0), __builtin_bit_cast(u16x2, w1)),
+                                                  __builtin_elementwise_max(__builtin_bit_cast(u16x2, w2), __builtin_bit_cast(u16x2, w3)));
+        const uint32_t top = max_of_four_lanes(max((uint32_t)m[0], (uint32_t)m[1]));
+        if constexpr (NS == 1) return top << 16;
+        if (top >= 0x7C00u) return 0x7F800000u;
+        return __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(_Float16, (uint16_t)top));
+    }
+}
+
 // The codes of 8 elements of a token, four lanes of a group together: the scale's byte, and whether the elements are finite.
 template <int NS>
 __device__ inline uint32_t quantise8(const Eight<NS> &v, int *byte, bool *finite) {
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (float)v[i];
-    uint32_t bits = 0;  // the largest magnitude's, NaN above infinity above all others
-#pragma unroll
-    for (int i = 0; i < 8; i++) bits = max(bits, __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu);
-    bits = max(bits, (uint32_t)__shfl_xor((int)bits, 1));
-    bits = max(bits, (uint32_t)__shfl_xor((int)bits, 2));
+    const uint32_t bits = top_of_group<NS>(v);
     *finite = bits < 0x7F800000u;
     // the exponent of a number below 2^-126 reads as -127, and both are far below the least
     const int e = max((int)(bits >> 23) - 127 - 2, kLeastExponent);
     *byte = e + 127;
     const float scale = __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
     uint32_t code = 0;  // rounds to nearest, ties to the even code, magnitudes over 6 to 6
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[0], x[1], scale, 0);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[2], x[3], scale, 1);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[4], x[5], scale, 2);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[6], x[7], scale, 3);
+    if constexpr (NS == 1) {
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, v.s01, scale, 0);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, v.s23, scale, 1);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, v.s45, scale, 2);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, v.s67, scale, 3);
+    } else {
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, (float)v[0], (float)v[1], scale, 0);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, (float)v[2], (float)v[3], scale, 1);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, (float)v[4], (float)v[5], scale, 2);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, (float)v[6], (float)v[7], scale, 3);
+    }
     return code;
 }
 
+// The upper value of a word stays in it with the lower one's bits behind its own: they change no comparison of two values that
+// differ, and are cut off at the end.
 __device__ inline void widen(float (&hi)[8], float (&lo)[8], uint32_t code, float scale) {
     const uint32_t w[4] = {two_values<0>(code, scale), two_values<1>(code, scale), two_values<2>(code, scale),
                            two_values<3>(code, scale)};
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const float v = __builtin_bit_cast(float, i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+        const uint32_t u = i & 1 ? w[i >> 1] : w[i >> 1] << 16;
+        const float v = __builtin_bit_cast(float, u);
         hi[i] = fmaxf(hi[i], v);
         lo[i] = fminf(lo[i], v);
     }
 }
+__device__ inline float cut_off(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xFFFF0000u); }
 
 // One workgroup makes one block of one head: T = 2^n >= D / 8 lanes take a token, 8 dimensions each, 256 / T tokens at a time.
 // New tokens are quantised and stored, older ones of the block are read back, and both go into the bounds.  What bounds it is the
@@ -88,8 +123,10 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheView c, Tokens t,
     __shared__ int s_bad;
     __shared__ __attribute__((aligned(4))) uint8_t s_scale[2][D / 32][kPage];
 
-    const int h = blockIdx.y;
-    const Piece w = find_piece(t.sequences, blockIdx.x, [&](int b) {
+    // the heads of a block come one after the other: a token's rows lie side by side (written and read back, 32,768 tokens of 8 heads:
+    // 90 us, and 97 with each head's blocks together)
+    const int h = blockIdx.x % c.heads;
+    const Piece w = find_piece(t.sequences, blockIdx.x / c.heads, [&](int b) {
         const int n = row_count(t, b), start = length_of(t, b);
         return n ? (int)((start + (int64_t)n - 1) / kPage) - start / kPage + 1 : 0;
     });
@@ -168,8 +205,8 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheView c, Tokens t,
     if (seg < kSegs) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            s_hi[at][seg * 8 + i] = hi[i];
-            s_lo[at][seg * 8 + i] = lo[i];
+            s_hi[at][seg * 8 + i] = cut_off(hi[i]);
+            s_lo[at][seg * 8 + i] = cut_off(lo[i]);
         }
     }
     if (bad) s_bad = 1;
@@ -262,10 +299,10 @@ template <int NS>
 int write_rows(const CacheView &c, const Tokens &t, Rows k, Rows v, hipStream_t stream) {
     // a sequence's n rows lie in at most n / 64 + 2 blocks, one row in one
     const int64_t tiles = t.offsets ? (int64_t)t.rows / kPage + 2 * (int64_t)t.sequences : t.rows;
-    VL_REQUIRE(tiles <= kMaxBlocks, "more sequences and rows than one call takes: %lld blocks", (long long)tiles);
+    VL_REQUIRE(tiles * c.heads <= 4 * kMaxBlocks, "more sequences and rows than one call takes: %lld blocks", (long long)tiles);
     for_dim(c.dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        cache_write_kernel<D, NS><<<dim3((unsigned)tiles, (unsigned)c.heads), 256, 0, stream>>>(c, t, k, v);
+        cache_write_kernel<D, NS><<<(unsigned)(tiles * c.heads), 256, 0, stream>>>(c, t, k, v);
     });
     VL_LAUNCH_CHECK("cache_write_kernel");
     return VL_OK;
