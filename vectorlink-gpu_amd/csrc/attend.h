@@ -16,12 +16,11 @@ struct AttendArgs {
     int causal;
     float scale;            // |scale| log2(e): exponentials are powers of two here
     uint32_t sign;          // 0x80000000 where the scale is negative: turns the queries' sign
-    int splits;             // workgroups that share a tile; of attend_few_kernel also kWaveTiles or kWideTiles
+    int splits;             // workgroups that share a tile
+    int waves;              // of attend_few_kernel: wavefronts of a workgroup that share a tile, 4 or 8; 1: four have one each
     float *part;            // splits > 1: [rows * heads_q, splits, D] sums, then [rows * heads_q, splits, 2] maxima and sums of weights
 };
 constexpr int kMaxSplits = 64;
-constexpr int kWaveTiles = 0;   // a tile for every wavefront
-constexpr int kWideTiles = -1;  // a tile for every workgroup of 8 wavefronts
 
 // 16 rows at a time, the tokens split over wavefronts and workgroups
 template <int NS>

@@ -52,19 +52,25 @@ int64_t few_tiles(const AttendArgs &a) {
     return (int64_t)a.t.rows * a.group / 16 + a.t.sequences;
 }
 
-// Workgroups that the tokens of a tile are split over: enough for the two that a compute unit holds at once, but a page for every
-// wavefront.  More cost their starts and ends (64 tokens over 4,096 to 8,192: 92 us with 512 workgroups, 98 with 1,024, 123 with
-// 4,096).  A tile for every wavefront where that alone gives every SIMD two; a workgroup of 8 wavefronts for a tile where that leaves
-// each at most four pages, which takes no second launch to join (1,000 tokens, 32 heads: 14.5 us in two launches, 10.3 in one).
-int splits_for(const AttendArgs &a, int64_t tiles) {
+// How the pages of a tile are shared out.  A tile for every wavefront where that alone gives every SIMD two.  A workgroup of 8
+// wavefronts for a tile where that leaves each at most four pages, which takes no second launch to join (1,000 tokens, 32 heads:
+// 14.5 us in two launches, 10.3 in one).  Else workgroups of 4, as many a tile as give every compute unit one (two for float32,
+// which is three times the products), but two pages (one) for every wavefront: parts cost their starts and ends, and joining them.
+// One workgroup a compute unit and two: one sequence of 65,536 tokens 27 us and 36, 32 of 4,096 to 8,192 with 8 heads of 8 47 and 53,
+// in float32 68 and 59.  Two pages a wavefront and one: 2 sequences of 16,384 19 us and 27.
+struct Shares {
+    int waves, splits;
+};
+Shares shares_for(const AttendArgs &a, int type, int64_t tiles) {
     const int64_t entries = a.count ? a.count : a.t.blocks;
     const int64_t items = tiles * a.c.heads;
-    if (items == 0) return 1;
-    if (items >= 8 * kComputeUnits) return kWaveTiles;
-    if (a.c.dim <= 128 && items <= kComputeUnits && entries <= 32) return kWideTiles;
-    int64_t s = (2 * kComputeUnits + items - 1) / items;
-    s = s < (entries + 3) / 4 ? s : (entries + 3) / 4;
-    return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+    if (items == 0) return {4, 1};
+    if (items >= 8 * kComputeUnits) return {1, 1};
+    if (a.c.dim <= 128 && items <= kComputeUnits && entries <= 32) return {8, 1};
+    const int64_t groups = (type == VL_F32 ? 2 : 1) * kComputeUnits, pages = type == VL_F32 ? 4 : 8;
+    int64_t s = (groups + items - 1) / items;
+    s = s < (entries + pages - 1) / pages ? s : (entries + pages - 1) / pages;
+    return {4, (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s)};
 }
 
 int64_t part_bytes(const AttendArgs &a, int splits) {
@@ -118,7 +124,9 @@ int check_workspace(int64_t need, const void *workspace, int64_t bytes) {
 
 int attend_few(AttendArgs &a, int type, void *workspace, int64_t bytes, hipStream_t stream) {
     const int64_t tiles = few_tiles(a);
-    a.splits = splits_for(a, tiles);
+    const Shares shares = shares_for(a, type, tiles);
+    a.waves = shares.waves;
+    a.splits = shares.splits;
     const int rc = check_workspace(part_bytes(a, a.splits), workspace, bytes);
     if (rc != VL_OK) return rc;
     a.part = (float *)workspace;
@@ -173,7 +181,7 @@ VL_EXPORT int64_t vl_attend_workspace_bytes(const vl_cache *cache, const vl_toke
     const int rc = attend_args(cache, tokens, queries, false, &a);
     if (rc != VL_OK) return rc;
     if (takes_many(a, queries)) return part_bytes(a, many_splits(a));
-    return part_bytes(a, splits_for(a, few_tiles(a)));
+    return part_bytes(a, shares_for(a, queries->type, few_tiles(a)).splits);
 }
 
 VL_EXPORT int vl_attend(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries, void *workspace,
@@ -209,7 +217,7 @@ VL_EXPORT int64_t vl_attend_blocks_workspace_bytes(const vl_cache *cache, const 
     int rc = attend_args(cache, tokens, queries, false, &a);
     if (rc == VL_OK) rc = check_count(count);
     a.count = (int)count;
-    return rc != VL_OK ? rc : part_bytes(a, splits_for(a, few_tiles(a)));
+    return rc != VL_OK ? rc : part_bytes(a, shares_for(a, queries->type, few_tiles(a)).splits);
 }
 
 VL_EXPORT int vl_attend_blocks(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries, const int32_t *blocks,
@@ -232,7 +240,7 @@ VL_EXPORT int64_t vl_attend_selected_workspace_bytes(const vl_cache *cache, cons
     if (rc != VL_OK) return rc;
     if (in_one_step(a, queries->type, count)) return 0;
     a.count = (int)count;
-    return select_workspace_bytes(select_args(a, count)) + part_bytes(a, splits_for(a, few_tiles(a)));
+    return select_workspace_bytes(select_args(a, count)) + part_bytes(a, shares_for(a, queries->type, few_tiles(a)).splits);
 }
 
 VL_EXPORT int vl_attend_selected(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries, int64_t count,

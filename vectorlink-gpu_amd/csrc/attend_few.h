@@ -595,11 +595,18 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
     float x[kEach];
 #pragma unroll
     for (int k = 0; k < kEach; k++) x[k] = 0;
-    for (int s = 0; s < a.splits; s++) {
-        const float by = __shfl(weight, s);
-        if (at < D) {
+    for (int s0 = 0; s0 < a.splits; s0 += 8) {  // 8 parts on their way at once
+        float part[8][kEach];
 #pragma unroll
-            for (int k = 0; k < kEach; k++) x[k] += by * a.part[(row * a.splits + s) * D + at + k];
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int k = 0; k < kEach; k++) part[i][k] = a.part[(row * a.splits + min(s0 + i, a.splits - 1)) * D + min(at, D - kEach) + k];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int w = __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), min(s0 + i, kMaxSplits - 1));
+            const float by = s0 + i < a.splits ? __builtin_bit_cast(float, w) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < kEach; k++) x[k] += by * part[i][k];
         }
     }
     const float by = total == 0 ? 0.0f : 1.0f / total;

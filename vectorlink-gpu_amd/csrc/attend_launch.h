@@ -19,24 +19,22 @@ void launch_join(const AttendArgs &a, hipStream_t stream) {
 
 template <int NS>
 int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
-    VL_REQUIRE(tiles * (a.splits > 0 ? a.splits : 1) <= 4 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)tiles);
+    VL_REQUIRE(tiles * a.splits <= 4 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)tiles);
     hipError_t e = hipSuccess;
     for_dim(a.c.dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        const unsigned groups = (unsigned)(tiles * (a.splits > 0 ? a.splits : 1)), heads = (unsigned)a.c.heads;
-        AttendArgs one = a;
-        one.splits = a.splits > 0 ? a.splits : 1;
+        const unsigned groups = (unsigned)(tiles * a.splits), heads = (unsigned)a.c.heads;
         for_rows(a.list || !a.t.offsets ? a.group : 16, [&](auto c) {
             constexpr int C = decltype(c)::value;
-            if (a.splits == kWaveTiles) {
-                attend_few_kernel<D, NS, 1, C><<<dim3((unsigned)((tiles + 3) / 4), heads), 256, 0, stream>>>(one, (int)tiles);
-            } else if (a.splits == kWideTiles) {
+            if (a.waves == 1) {
+                attend_few_kernel<D, NS, 1, C><<<dim3((unsigned)((tiles + 3) / 4), heads), 256, 0, stream>>>(a, (int)tiles);
+            } else if (a.waves == 8) {
                 if constexpr (D <= 128) {
                     e = vl_allow_lds(attend_few_kernel<D, NS, 8, C>, sizeof(JoinLds<8>));
-                    if (e == hipSuccess) attend_few_kernel<D, NS, 8, C><<<dim3(groups, heads), 512, sizeof(JoinLds<8>), stream>>>(one, (int)tiles);
+                    if (e == hipSuccess) attend_few_kernel<D, NS, 8, C><<<dim3(groups, heads), 512, sizeof(JoinLds<8>), stream>>>(a, (int)tiles);
                 }
             } else {
-                attend_few_kernel<D, NS, 4, C><<<dim3(groups, heads), 256, sizeof(JoinLds<4>), stream>>>(one, (int)tiles);
+                attend_few_kernel<D, NS, 4, C><<<dim3(groups, heads), 256, sizeof(JoinLds<4>), stream>>>(a, (int)tiles);
             }
         });
         launch_join<D, NS>(a, stream);
