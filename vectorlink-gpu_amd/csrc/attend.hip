@@ -53,7 +53,8 @@ int64_t few_tiles(const AttendArgs &a) {
 }
 
 // How the pages of a tile are shared out.  A tile for every wavefront where that alone gives every SIMD two.  A workgroup of 8
-// wavefronts for a tile where that leaves each at most four pages, which takes no second launch to join (1,000 tokens, 32 heads:
+// wavefronts for a tile where that leaves each at most four pages (two of a list, whose call has more launches anyway: 8 tiles of
+// 32 blocks 13.2 us, and 6.9 and 4.4 split and joined), which takes no second launch to join (1,000 tokens, 32 heads:
 // 14.5 us in two launches, 10.3 in one).  Else workgroups of 4, as many a tile as give every compute unit one (two for float32,
 // which is three times the products), but two pages (one) for every wavefront: parts cost their starts and ends, and joining them.
 // One workgroup a compute unit and two: one sequence of 65,536 tokens 27 us and 36, 32 of 4,096 to 8,192 with 8 heads of 8 47 and 53,
@@ -66,7 +67,7 @@ Shares shares_for(const AttendArgs &a, int type, int64_t tiles) {
     const int64_t items = tiles * a.c.heads;
     if (items == 0) return {4, 1};
     if (items >= 8 * kComputeUnits) return {1, 1};
-    if (a.c.dim <= 128 && items <= kComputeUnits && entries <= 32) return {8, 1};
+    if (a.c.dim <= 128 && items <= kComputeUnits && entries <= (a.count ? 16 : 32)) return {8, 1};
     const int64_t groups = (type == VL_F32 ? 2 : 1) * kComputeUnits, pages = type == VL_F32 ? 4 : 8;
     int64_t s = (groups + items - 1) / items;
     s = s < (entries + pages - 1) / pages ? s : (entries + pages - 1) / pages;
