@@ -287,6 +287,30 @@ def test_a_long_context():
     ref.check_attention(attend(q, cache, table, lengths), ref.attention(q, cache, table, lengths), torch.bfloat16)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_few_tokens_over_a_long_context(dtype):
+    """Rows of one sequence that see differently many, tiles split over workgroups; 48 rows of a head are three tiles."""
+    cache, table, lengths, gen = filled([5000, 3001], 2, 64, 14, dtype)
+    q = queries_for(19, 6, 64, gen, dtype)
+    out = attend(q, cache, table, lengths, offsets=ends([16, 3]))
+    ref.check_attention(out, ref.attention(q, cache, table, lengths, ends([16, 3])), dtype)
+
+
+@pytest.mark.parametrize("dim,group", [(64, 2), (128, 5), (96, 17)])
+def test_so_many_tiles_that_every_wavefront_has_one(dim, group):
+    lengths = [i * 37 % 150 for i in range(300)]
+    cache, table, lengths, gen = filled(lengths, 8, dim, 16, blocks=3)
+    q = queries_for(300, 8 * group, dim, gen, torch.bfloat16)
+    (out, lse) = attend(q, cache, table, lengths, return_lse=True)
+    some = torch.arange(0, 300, 7, device=DEV)  # the rest has the same code and the reference is slow
+    want = ref.attention(q[some], cache, table[some], lengths[some])
+    ref.check_attention(out[some], want, torch.bfloat16)
+    assert torch.equal(lse[some].cpu().isneginf(), want[1].isneginf())
+    (out, blocks) = attend_selected(q, cache, table, lengths, 2)
+    assert torch.equal(blocks[some].cpu(), ref.selection(q[some], cache, table[some], lengths[some], 2))
+    ref.check_attention(out[some], ref.attention(q[some], cache, table[some], lengths[some], blocks=blocks[some]), torch.bfloat16)
+
+
 # ---- the choice of blocks ------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", TYPES)
