@@ -11,6 +11,7 @@ queries are tokens; offsets [sequences + 1] int32 says which rows are whose (Non
 enqueued on torch's current stream; nothing is synchronised, and no length is read on the host.
 """
 import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -20,9 +21,13 @@ from . import _native as nv
 
 PAGE = 64  # tokens
 DIMS = (32, 64, 96, 128, 192, 256)
+# A call's vl_tokens and vl_queries as bytes: a third of the time of a ctypes structure, which a single token's call notices
+_TOKENS = struct.Struct("@qqqqPPP")
+_QUERIES = struct.Struct("@qqqPPPdiiq")
+assert _TOKENS.size == C.sizeof(nv.Tokens) and _QUERIES.size == C.sizeof(nv.Queries)
 
 
-def _tokens(rows: int, table: Tensor, lengths: Tensor, offsets: Optional[Tensor]) -> nv.Tokens:
+def _tokens(rows: int, table: Tensor, lengths: Tensor, offsets: Optional[Tensor]) -> bytes:
     assert table.dtype == torch.int32 and table.dim() == 2, "table must be int32 [sequences, blocks]"
     (sequences, blocks) = table.shape
     (stride, one) = table.stride()
@@ -31,12 +36,12 @@ def _tokens(rows: int, table: Tensor, lengths: Tensor, offsets: Optional[Tensor]
         f"lengths must be a contiguous int32 tensor of {sequences}"
     if offsets is None:
         assert rows == sequences, f"without offsets every sequence has one row: {rows} rows, {sequences} sequences"
-        at = None
+        at = 0
     else:
         assert offsets.dtype == torch.int32 and offsets.shape == (sequences + 1,) and offsets.is_contiguous(), \
             f"offsets must be a contiguous int32 tensor of {sequences + 1}"
         at = offsets.data_ptr()
-    return nv.Tokens(rows, sequences, blocks, stride if sequences > 1 else blocks, table.data_ptr(), lengths.data_ptr(), at)
+    return _TOKENS.pack(rows, sequences, blocks, stride if sequences > 1 else blocks, table.data_ptr(), lengths.data_ptr(), at)
 
 
 def _check_rows(t: Tensor, name: str, dim: int) -> int:
@@ -90,7 +95,7 @@ class KVCache:
         assert keys.shape[1] == self.heads, f"keys have {keys.shape[1]} heads, the cache {self.heads}"
         tokens = _tokens(keys.shape[0], table, starts, offsets)
         nv.require_gpu(keys, values, table, starts, offsets)
-        nv.check(nv.lib().vl_cache_write(self._ref, C.byref(tokens), kind, keys.data_ptr(), keys.stride(0), keys.stride(1),
+        nv.check(nv.lib().vl_cache_write(self._ref, tokens, kind, keys.data_ptr(), keys.stride(0), keys.stride(1),
                                          values.data_ptr(), values.stride(0), values.stride(1), nv.stream()))
 
     def read(self, table: Tensor, starts: Tensor, rows: int, offsets: Optional[Tensor] = None,
@@ -102,7 +107,7 @@ class KVCache:
         nv.require_gpu(table, starts, offsets)
         keys = torch.empty((rows, self.heads, self.dim), dtype=dtype, device=self.keys.device)
         values = torch.empty_like(keys)
-        nv.check(nv.lib().vl_cache_read(self._ref, C.byref(tokens), nv.TYPES[dtype], keys.data_ptr(), values.data_ptr(), nv.stream()))
+        nv.check(nv.lib().vl_cache_read(self._ref, tokens, nv.TYPES[dtype], keys.data_ptr(), values.data_ptr(), nv.stream()))
         return (keys, values)
 
     def read_bounds(self, pages: Tensor) -> Tensor:
@@ -116,12 +121,11 @@ class KVCache:
 
 
 def _queries(queries: Tensor, cache: KVCache, scale: Optional[float], causal: bool, out: Optional[Tensor],
-             lse: Optional[Tensor], form: Optional[str] = None) -> nv.Queries:
+             lse: Optional[Tensor], form: Optional[str] = None) -> bytes:
     (row, head, _) = queries.stride()
-    return nv.Queries(queries.shape[1], row, head, queries.data_ptr(), None if out is None else out.data_ptr(),
-                      None if lse is None else lse.data_ptr(), cache.dim ** -0.5 if scale is None else scale,
-                      nv.TYPES[queries.dtype], causal,
-                      0 if form is None else nv.ATTEND_FORMS[form])
+    return _QUERIES.pack(queries.shape[1], row, head, queries.data_ptr(), 0 if out is None else out.data_ptr(),
+                         0 if lse is None else lse.data_ptr(), cache.dim ** -0.5 if scale is None else scale,
+                         nv.TYPES[queries.dtype], causal, 0 if form is None else nv.ATTEND_FORMS[form])
 
 
 def _check_queries(queries: Tensor, cache: KVCache):
@@ -142,12 +146,12 @@ def attend(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, offs
     return_lse also the logarithms of the sums of exponentials [rows, heads], by which parts of an attention are joined.
     form: the library chooses one by the sizes; "few" or "many" ask for it, for tests and measurements."""
     assert form is None or form in nv.ATTEND_FORMS, f"unknown form {form!r}: expected one of {sorted(nv.ATTEND_FORMS)}"
-    tokens = C.byref(_tokens(queries.shape[0], table, lengths, offsets))
+    tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
     nv.require_gpu(queries, table, lengths, offsets)
     out = queries.new_empty(queries.shape)
     lse = queries.new_empty(queries.shape[:2], dtype=torch.float32) if return_lse else None
-    q = C.byref(_queries(queries, cache, scale, causal, out, lse, form))
+    q = _queries(queries, cache, scale, causal, out, lse, form)
     lib = nv.lib()
     need = lib.vl_attend_workspace_bytes(cache._ref, tokens, q)
     ws = _workspace(need, queries)
@@ -160,11 +164,11 @@ def select_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tenso
     """For every row and head of the cache `count` blocks of its sequence, ascending: the row's own and those with the highest
     upper bound on a score in them, by queries and bounds of 8 bits; MAXINT where there are no more.  [rows, cache.heads, count]"""
     assert count >= 1, f"count: {count}"
-    tokens = C.byref(_tokens(queries.shape[0], table, lengths, offsets))
+    tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
     nv.require_gpu(queries, table, lengths, offsets)
     blocks = table.new_empty((queries.shape[0], cache.heads, count))
-    q = C.byref(_queries(queries, cache, None, True, None, None))
+    q = _queries(queries, cache, None, True, None, None)
     lib = nv.lib()
     need = lib.vl_select_blocks_workspace_bytes(cache._ref, tokens, q, count)
     ws = _workspace(need, queries)
@@ -175,7 +179,7 @@ def select_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tenso
 def attend_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, blocks: Tensor,
                   offsets: Optional[Tensor] = None, scale: Optional[float] = None, return_lse: bool = False):
     """attend over the tokens of blocks [rows, cache.heads, count] alone, up to the row's own place."""
-    tokens = C.byref(_tokens(queries.shape[0], table, lengths, offsets))
+    tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
     nv.require_gpu(queries, table, lengths, offsets)
     assert blocks.dtype == torch.int32 and blocks.is_contiguous(), "blocks must be contiguous int32"
@@ -185,7 +189,7 @@ def attend_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tenso
     count = blocks.shape[2]
     out = queries.new_empty(queries.shape)
     lse = queries.new_empty(queries.shape[:2], dtype=torch.float32) if return_lse else None
-    q = C.byref(_queries(queries, cache, scale, True, out, lse))
+    q = _queries(queries, cache, scale, True, out, lse)
     lib = nv.lib()
     need = lib.vl_attend_blocks_workspace_bytes(cache._ref, tokens, q, count)
     ws = _workspace(need, queries)
@@ -197,12 +201,12 @@ def attend_selected(queries: Tensor, cache: KVCache, table: Tensor, lengths: Ten
                     offsets: Optional[Tensor] = None, scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
     """(attend_blocks(...), blocks) with the blocks of select_blocks, in one call."""
     assert count >= 1, f"count: {count}"
-    tokens = C.byref(_tokens(queries.shape[0], table, lengths, offsets))
+    tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
     nv.require_gpu(queries, table, lengths, offsets)
     blocks = table.new_empty((queries.shape[0], cache.heads, count))
     out = queries.new_empty(queries.shape)
-    q = C.byref(_queries(queries, cache, scale, True, out, None))
+    q = _queries(queries, cache, scale, True, out, None)
     lib = nv.lib()
     need = lib.vl_attend_selected_workspace_bytes(cache._ref, tokens, q, count)
     ws = _workspace(need, queries)
