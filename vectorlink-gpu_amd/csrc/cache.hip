@@ -126,10 +126,12 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheView c, Tokens t,
     // the heads of a block come one after the other: a token's rows lie side by side (written and read back, 32,768 tokens of 8 heads:
     // 90 us, and 97 with each head's blocks together)
     const int h = blockIdx.x % c.heads;
-    const Piece w = find_piece(t.sequences, blockIdx.x / c.heads, [&](int b) {
-        const int n = row_count(t, b), start = length_of(t, b);
-        return n ? (int)((start + (int64_t)n - 1) / kPage) - start / kPage + 1 : 0;
-    });
+    Piece w = {(int)blockIdx.x / c.heads, 0};  // without offsets every sequence has one row, in one block
+    if (t.offsets)
+        w = find_piece(t.sequences, blockIdx.x / c.heads, [&](int b) {
+            const int n = row_count(t, b), start = length_of(t, b);
+            return n ? (int)((start + (int64_t)n - 1) / kPage) - start / kPage + 1 : 0;
+        });
     if (w.sequence < 0) return;
     const int b = w.sequence, start = length_of(t, b);
     const int block = start / kPage + w.piece;
