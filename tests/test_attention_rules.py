@@ -1,0 +1,41 @@
+"""Attention over the cache without a GPU: sizes at the ends of what the rules divide by and choose between."""
+import ctypes as C
+import os
+import subprocess
+import sys
+
+from vectorlink_gpu import _native as nv
+
+PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "vectorlink-gpu_amd")
+
+# every call that says how much workspace a call takes, and the calls, of no rows: in a process of its own, which a division by zero ends
+NO_ROWS = """
+import ctypes as C
+import sys
+sys.path.insert(0, sys.argv[1])
+from vectorlink_gpu import _native as nv
+lib = nv.lib()
+parts = dict(keys=256, key_scales=256, values=256, value_scales=256, bounds=256, bound_scales=256)
+for dim in (32, 64, 96, 128, 192, 256):
+    for (heads, group) in ((1, 1), (8, 4), (2, 20)):
+        cache = C.byref(nv.Cache(pages=10, heads=heads, dim=dim, **parts))
+        for blocks in (0, 1, 7, 8, 64, 40_000):
+            for sequences in (0, 1, 5):
+                tokens = C.byref(nv.Tokens(rows=0, sequences=sequences, blocks=blocks, table_stride=blocks, table=256, lengths=256, offsets=256))
+                for type in (1, 2, 3):
+                    for form in (0, 1, 2) if dim * type <= 256 else (0, 1):
+                        q = C.byref(nv.Queries(heads=heads * group, row_stride=0, head_stride=0, scale=1.0, type=type, causal=1, form=form))
+                        assert lib.vl_attend_form(cache, tokens, q) in ((1, 2) if form == 0 else (form,))
+                        assert lib.vl_attend_workspace_bytes(cache, tokens, q) == 0
+                        assert lib.vl_select_blocks_workspace_bytes(cache, tokens, q, 4) == 0
+                        assert lib.vl_attend_blocks_workspace_bytes(cache, tokens, q, 4) == 0
+                        assert lib.vl_attend_selected_workspace_bytes(cache, tokens, q, 4) == 0
+                        assert lib.vl_attend(cache, tokens, q, None, 0, None) == 0
+                        assert lib.vl_attend_selected(cache, tokens, q, 4, None, None, 0, None) == 0
+print("all answered")
+"""
+
+
+def test_no_rows_in_every_form():
+    r = subprocess.run([sys.executable, "-c", NO_ROWS, PKG], capture_output=True, text=True)
+    assert r.returncode == 0 and "all answered" in r.stdout, (r.returncode, r.stderr[-500:])

@@ -82,6 +82,7 @@ int64_t part_bytes(const AttendArgs &a, int splits) {
 // Tiles of the rows of a workgroup of attend_many_kernel: at most, and about
 int64_t many_tiles(const AttendArgs &a) { return (int64_t)a.t.rows * a.group / (32 * many_waves(a.c.dim)) + a.t.sequences; }
 int64_t many_tiles_about(const AttendArgs &a) {
+    if (a.t.rows == 0) return 0;  // and perhaps no sequences either
     const int64_t rows = 32 * many_waves(a.c.dim), each = (int64_t)a.t.rows * a.group / a.t.sequences;
     return a.t.sequences * (each / rows + (each % rows != 0));
 }
