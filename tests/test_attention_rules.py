@@ -39,3 +39,24 @@ print("all answered")
 def test_no_rows_in_every_form():
     r = subprocess.run([sys.executable, "-c", NO_ROWS, PKG], capture_output=True, text=True)
     assert r.returncode == 0 and "all answered" in r.stdout, (r.returncode, r.stderr[-500:])
+
+
+def native(rows, sequences, blocks, heads=8, group=4, dim=128, type=1):
+    parts = dict(keys=256, key_scales=256, values=256, value_scales=256, bounds=256, bound_scales=256)
+    return (C.byref(nv.Cache(pages=10, heads=heads, dim=dim, **parts)),
+            C.byref(nv.Tokens(rows=rows, sequences=sequences, blocks=blocks, table_stride=blocks, table=256, lengths=256, offsets=256)),
+            C.byref(nv.Queries(heads=heads * group, row_stride=0, head_stride=0, scale=1.0, type=type, causal=1, form=0)))
+
+
+def test_sequences_without_rows_count_for_nothing():
+    """A batch with a place for each of many sequences, of which few have new tokens, is answered as those few are."""
+    lib = nv.lib()
+    for rows in (1, 3, 10, 63):
+        for blocks in (16, 128, 2048):
+            for kw in (dict(), dict(heads=1, group=1, dim=64), dict(type=2), dict(dim=256)):
+                alone = native(rows, rows, blocks, **kw)
+                want = (lib.vl_attend_form(*alone), lib.vl_attend_workspace_bytes(*alone))
+                assert want[0] == 1
+                for sequences in (rows + 1, 64, 256, 4096):
+                    among = native(rows, sequences, blocks, **kw)
+                    assert (lib.vl_attend_form(*among), lib.vl_attend_workspace_bytes(*among)) == want, (rows, sequences, blocks, kw)

@@ -49,7 +49,7 @@ int attend_args(const vl_cache *cache, const vl_tokens *tokens, const vl_queries
 int64_t few_tiles(const AttendArgs &a) {
     const int64_t per = (a.group + 15) / 16;
     if (a.count || !a.t.offsets) return a.t.rows * per;
-    return (int64_t)a.t.rows * a.group / 16 + a.t.sequences;
+    return (int64_t)a.t.rows * a.group / 16 + sequences_with_rows(a.t);
 }
 
 // How the pages of a tile are shared out.  A tile for every wavefront where that alone gives every SIMD two.  A workgroup of 8
@@ -80,11 +80,12 @@ int64_t part_bytes(const AttendArgs &a, int splits) {
 }
 
 // Tiles of the rows of a workgroup of attend_many_kernel: at most, and about
-int64_t many_tiles(const AttendArgs &a) { return (int64_t)a.t.rows * a.group / (32 * many_waves(a.c.dim)) + a.t.sequences; }
+int64_t many_tiles(const AttendArgs &a) { return (int64_t)a.t.rows * a.group / (32 * many_waves(a.c.dim)) + sequences_with_rows(a.t); }
 int64_t many_tiles_about(const AttendArgs &a) {
     if (a.t.rows == 0) return 0;  // and perhaps no sequences either
-    const int64_t rows = 32 * many_waves(a.c.dim), each = (int64_t)a.t.rows * a.group / a.t.sequences;
-    return a.t.sequences * (each / rows + (each % rows != 0));
+    const int64_t sequences = sequences_with_rows(a.t);
+    const int64_t rows = 32 * many_waves(a.c.dim), each = (int64_t)a.t.rows * a.group / sequences;
+    return sequences * (each / rows + (each % rows != 0));
 }
 
 // Pages that the busiest compute unit takes one after the other, a workgroup's start and end counted as kEnds, if the tokens of a

@@ -173,6 +173,9 @@ __device__ inline float sum_over_quads(float x) {
 int vl_cache_of(const vl_cache *cache, CacheView *out);
 int vl_tokens_of(const vl_tokens *tokens, Tokens *out);
 
+// Sequences that have a row, at most: each may end inside a tile of its own
+static inline int64_t sequences_with_rows(const Tokens &t) { return t.rows < t.sequences ? t.rows : t.sequences; }
+
 // f(std::integral_constant<int, dim>) for a cache's row length
 template <class F>
 static inline void for_dim(int dim, F f) {

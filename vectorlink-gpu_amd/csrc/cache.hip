@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256) void cache_bounds_kernel(CacheView c, const in
 template <int NS>
 int write_rows(const CacheView &c, const Tokens &t, Rows k, Rows v, hipStream_t stream) {
     // a sequence's n rows lie in at most n / 64 + 2 blocks, one row in one
-    const int64_t tiles = t.offsets ? (int64_t)t.rows / kPage + 2 * (int64_t)t.sequences : t.rows;
+    const int64_t tiles = t.offsets ? (int64_t)t.rows / kPage + 2 * sequences_with_rows(t) : t.rows;
     VL_REQUIRE(tiles * c.heads <= 4 * kMaxBlocks, "more sequences and rows than one call takes: %lld blocks", (long long)tiles);
     for_dim(c.dim, [&](auto d) {
         constexpr int D = decltype(d)::value;

@@ -63,7 +63,7 @@ int launch(const SelectArgs &a, hipStream_t stream) {
     hipError_t e = hipSuccess;
     if (in_one(a)) {
         const int T = tokens_together(a);
-        const int64_t tiles = a.t.offsets ? a.t.rows / T + (int64_t)a.t.sequences : a.t.rows;
+        const int64_t tiles = a.t.offsets ? a.t.rows / T + sequences_with_rows(a.t) : a.t.rows;
         VL_REQUIRE(tiles <= 4 * kMaxBlocks, "more rows than one call takes: %lld", (long long)tiles);
         const size_t lds = (size_t)T * a.t.blocks * 4;
         for_dim(a.c.dim, [&](auto d) {
