@@ -509,7 +509,9 @@ typedef struct vl_cache {
 } vl_cache;
 
 /* The tokens of a call.  Rows [offsets[b], offsets[b + 1]) belong to sequence b;
- * offsets NULL: rows == sequences and row b belongs to sequence b.  table[b, :]
+ * offsets NULL: rows == sequences and row b belongs to sequence b.  Rows before
+ * offsets[0] and from offsets[sequences] on belong to none: what a call would
+ * write for them is left as it is (vl_cache_read: zeros).  table[b, :]
  * names the page of each block of 64 tokens of the sequence; a page outside
  * [0, pages) holds nothing: what is written there is dropped, and it takes no
  * part in attention.  lengths[b]: tokens in the sequence, see each call. */

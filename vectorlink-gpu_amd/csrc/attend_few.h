@@ -519,6 +519,7 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 
     if (a.list) {
         w = {__builtin_amdgcn_readfirstlane(sequence_of(a.t, tile / per)), tile % per};
         token0 = tile / per - first_row(a.t, w.sequence);
+        if (!__builtin_amdgcn_readfirstlane(is_row_of(a.t, w.sequence, tile / per))) return;
     } else if (!a.t.offsets) {
         w = {tile / per, tile % per};
     } else {
@@ -586,6 +587,9 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= (int64_t)a.t.rows * a.heads_q) return;
+    // rows that are no sequence's have no parts and are not written
+    const int token = (int)(row / a.heads_q);
+    const bool real = !a.t.offsets || (token >= a.t.offsets[0] && token < a.t.offsets[a.t.sequences]);
     const float *const ends = a.part + (int64_t)a.t.rows * a.heads_q * a.splits * D + row * a.splits * 2;
     float top = lane < a.splits ? ends[lane * 2] : -INFINITY;
     float sum = lane < a.splits ? ends[lane * 2 + 1] : 0;
@@ -616,6 +620,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
         }
     }
     const float by = total == 0 ? 0.0f : 1.0f / total;
+    if (!real) return;
     if (at < D) {
 #pragma unroll
         for (int k = 0; k < kEach; k++) ((E *)a.out)[row * D + at + k] = (E)(x[k] * by);

@@ -22,6 +22,7 @@ __global__ __launch_bounds__(512) void attend_step_kernel(AttendArgs a, SelectAr
     const int lane = threadIdx.x & 63, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Standing at = standing_of(a.t, row);
+    if (!at.real) return;
     const int b = __builtin_amdgcn_readfirstlane(at.b), blocks = __builtin_amdgcn_readfirstlane(at.blocks);
     const Scored what = {b, h, at.token, 1, at.place0, at.length, row - at.token};
     const bool real = r < a.group;

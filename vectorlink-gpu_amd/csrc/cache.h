@@ -64,6 +64,10 @@ __device__ inline int sequence_of(const Tokens &t, int row) {
     }
     return lo;
 }
+// Whether a row is one of that sequence's: rows before the first offset and behind the last are nobody's.
+__device__ inline bool is_row_of(const Tokens &t, int b, int row) {
+    return row >= first_row(t, b) && row - first_row(t, b) < row_count(t, b);
+}
 // Length of a sequence, cut to what its table can name.
 __device__ inline int length_of(const Tokens &t, int b) {
     return (int)min((int64_t)max(t.lengths[b], 0), (int64_t)t.blocks * kPage);

@@ -255,9 +255,9 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheView c, Tokens t, 
     const int64_t n = (int64_t)t.rows * c.heads * kSegs;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int seg = (int)(i % kSegs), h = (int)(i / kSegs % c.heads), row = (int)(i / kSegs / c.heads);
-        const int b = sequence_of(t, row);
-        const int64_t place = (int64_t)length_of(t, b) + row - first_row(t, b);
-        const int64_t page = place >= 0 && row < first_row(t, b) + row_count(t, b) ? page_of(t, c, b, (int)min(place / kPage, (int64_t)t.blocks)) : -1;
+        const int b = sequence_of(t, row), first = first_row(t, b);
+        const int64_t place = (int64_t)length_of(t, b) + row - first;
+        const int64_t page = row >= first && row < first + row_count(t, b) ? page_of(t, c, b, (int)min(place / kPage, (int64_t)t.blocks)) : -1;
         float k[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (page >= 0) {
             const int j = (int)(place % kPage);

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256) void score_kernel(SelectArgs a, int chunks) {
     __shared__ ScoreLds<4> s_score;
     const int row = blockIdx.x / chunks, from = blockIdx.x % chunks * kChunk, h = blockIdx.y;
     const Standing at = standing_of(a.t, row);
-    if (from >= at.blocks) return;
+    if (!at.real || from >= at.blocks) return;
     const Scored s = {at.b, h, at.token, 1, at.place0, at.length, row - at.token};
     score_blocks<D, NS, 4, WHOLE>(a, s, from, min(from + kChunk, at.blocks), a.keys + ((int64_t)row * a.c.heads + h) * a.t.blocks, 0, s_score);
 }
@@ -53,6 +53,7 @@ __global__ __launch_bounds__(512) void select_kernel(SelectArgs a) {
     __shared__ ChooseLds<8> s_choose;
     const int row = blockIdx.x, h = blockIdx.y;
     const Standing at = standing_of(a.t, row);
+    if (!at.real) return;
     int32_t *const out = a.out + ((int64_t)row * a.c.heads + h) * a.count;
     const int found = choose<8>(a.keys + ((int64_t)row * a.c.heads + h) * a.t.blocks, at.blocks, a.count, s_choose, [&](int k, int i) { out[k] = i; });
     for (int i = found + threadIdx.x; i < a.count; i += 512) out[i] = VL_MAXINT;

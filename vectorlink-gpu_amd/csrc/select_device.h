@@ -331,9 +331,10 @@ __device__ inline int choose(const uint32_t *keys, int n, int count, ChooseLds<W
     return more + min(equal, ties);
 }
 
-// Where a row stands in its sequence, and of how many blocks it chooses
+// Where a row stands in its sequence, and of how many blocks it chooses; not real: the row is no sequence's
 struct Standing {
     int b, token, place0, length, blocks;
+    bool real;
 };
 __device__ inline Standing standing_of(const Tokens &t, int row) {
     Standing s;
@@ -343,5 +344,6 @@ __device__ inline Standing standing_of(const Tokens &t, int row) {
     s.place0 = (int)min((int64_t)t.lengths[s.b], (int64_t)1 << 30) - row_count(t, s.b);
     const int place = min(s.place0 + s.token, s.length - 1);
     s.blocks = place < 0 ? 0 : place / kPage + 1;
+    s.real = __builtin_amdgcn_readfirstlane(is_row_of(t, s.b, row));
     return s;
 }
