@@ -559,7 +559,7 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 
         return i < tokens * a.group ? (row0 + (int64_t)(token0 + i / a.group)) * a.heads_q + h * a.group + i % a.group : -1;
     };
     if constexpr (JOIN) {
-        extern __shared__ char lds[];  // a JoinLds<WAVES>
+        extern __shared__ __attribute__((aligned(16))) char lds[];  // a JoinLds<WAVES>
         join_waves<D, NS, WAVES, C>(st, *reinterpret_cast<JoinLds<WAVES> *>(lds), a, split, out_row);
     } else {
         const float total = sum_of_row<C>(st.sum);

@@ -155,7 +155,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
     // Parts of a weight, as many as of a query: a bfloat16 result's error is then sqrt(2) times that of its own rounding at most, and
     // a second part would make half as many products again (half precision and float32 keep 16 and 24 bits).
     constexpr int NW = NS;
-    extern __shared__ char lds[];
+    extern __shared__ __attribute__((aligned(16))) char lds[];
 
     // all tiles of a head go to the same XCD where there are 8 heads; the last tiles, which see most, come first
     const int h = blockIdx.x % a.c.heads, at = blockIdx.x / a.c.heads, split = at % a.splits, tile = tiles - 1 - at / a.splits;

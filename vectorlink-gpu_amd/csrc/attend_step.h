@@ -11,7 +11,7 @@ constexpr int kStepWaves = 8;
 template <int D, int NS, int C>
 __global__ __launch_bounds__(512) void attend_step_kernel(AttendArgs a, SelectArgs s) {
     typedef JoinLds<kStepWaves> Join;
-    extern __shared__ char lds[];  // scores [blocks] and then the join's sums; behind them the list [count]
+    extern __shared__ __attribute__((aligned(16))) char lds[];  // scores [blocks] and then the join's sums; behind them the list [count]
     __shared__ ScoreLds<kStepWaves> s_score;
     __shared__ ChooseLds<kStepWaves> s_choose;
     uint32_t *const keys = (uint32_t *)lds;

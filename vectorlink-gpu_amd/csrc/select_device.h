@@ -190,7 +190,7 @@ __device__ inline void score_blocks(const SelectArgs &a, const Scored &s, int fr
 
 template <int WAVES>
 struct ChooseLds {
-    int count[4][256];
+    alignas(16) int count[4][256];  // read four at a time
     uint32_t differ;
     int more[WAVES], equal[WAVES];
 };
