@@ -14,32 +14,37 @@ int tokens_together(const SelectArgs &a) {
 // One workgroup a token scores and chooses where that fills the GPU or the blocks are few; else they are scored by many.
 bool in_one(const SelectArgs &a) { return tokens_together(a) > 0 && (a.t.blocks <= 1024 || (int64_t)a.t.rows * a.c.heads >= kComputeUnits); }
 
+// What a workgroup of choose_kernel has of LDS beside the scores
+struct ChooseKernelLds {
+    ScoreLds<4> score;
+    ChooseLds<1> choose[4];
+};
+
 // A workgroup scores all blocks of T tokens for one head into LDS, then every wavefront chooses for a token at a time.
 template <int D, int NS, bool WHOLE>
 __global__ __launch_bounds__(256) void choose_kernel(SelectArgs a, int T) {
     extern __shared__ uint32_t s_keys[];  // [T][a.t.blocks]
-    __shared__ ScoreLds<4> s_score;
-    __shared__ ChooseLds<1> s_choose[4];
+    __shared__ ChooseKernelLds s;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     Piece w = {(int)blockIdx.x, 0};
     if (a.t.offsets) w = find_piece(a.t.sequences, blockIdx.x, [&](int b) { return (row_count(a.t, b) + T - 1) / T; });
     if (w.sequence < 0) return;
     const int b = w.sequence, all = row_count(a.t, b), length = length_of(a.t, b);
     const int place0 = (int)min((int64_t)a.t.lengths[b], (int64_t)1 << 30) - all;
-    const Scored s = {b, (int)blockIdx.y, w.piece * T, min(T, all - w.piece * T), place0, length, first_row(a.t, b)};
-    const int last = min(place0 + s.token0 + s.tokens, length) - 1;
+    const Scored what = {b, (int)blockIdx.y, w.piece * T, min(T, all - w.piece * T), place0, length, first_row(a.t, b)};
+    const int last = min(place0 + what.token0 + what.tokens, length) - 1;
     const int blocks = last < 0 ? 0 : last / kPage + 1;
-    score_blocks<D, NS, 4, WHOLE>(a, s, 0, blocks, s_keys, a.t.blocks, s_score);
+    score_blocks<D, NS, 4, WHOLE>(a, what, 0, blocks, s_keys, a.t.blocks, s.score);
     __syncthreads();
-    for (int token = wave; token < s.tokens; token += 4) {
-        const int place = min(place0 + s.token0 + token, length - 1), n = place < 0 ? 0 : place / kPage + 1;
-        int32_t *const out = a.out + ((s.row0 + s.token0 + token) * a.c.heads + s.h) * a.count;
-        const int found = choose<1>(s_keys + token * a.t.blocks, n, a.count, s_choose[wave], [&](int at, int i) { out[at] = i; });
+    for (int token = wave; token < what.tokens; token += 4) {
+        const int place = min(place0 + what.token0 + token, length - 1), n = place < 0 ? 0 : place / kPage + 1;
+        int32_t *const out = a.out + ((what.row0 + what.token0 + token) * a.c.heads + what.h) * a.count;
+        const int found = choose<1>(s_keys + token * a.t.blocks, n, a.count, s.choose[wave], [&](int at, int i) { out[at] = i; });
         for (int i = found + lane; i < a.count; i += 64) out[i] = VL_MAXINT;
     }
 }
 
-// A workgroup scores 256 blocks of one token and head.
+// A workgroup scores kChunk blocks of one token and head.
 template <int D, int NS, bool WHOLE>
 __global__ __launch_bounds__(256) void score_kernel(SelectArgs a, int chunks) {
     __shared__ ScoreLds<4> s_score;
@@ -69,7 +74,7 @@ int launch(const SelectArgs &a, hipStream_t stream) {
         const size_t lds = (size_t)T * a.t.blocks * 4;
         for_dim(a.c.dim, [&](auto d) {
             constexpr int D = decltype(d)::value;
-            e = vl_allow_lds(choose_kernel<D, NS, WHOLE>, lds + 12 * 1024);  // and its static LDS
+            e = vl_allow_lds(choose_kernel<D, NS, WHOLE>, lds + sizeof(ChooseKernelLds));  // both count towards a launch's 64 KiB
             if (e == hipSuccess) choose_kernel<D, NS, WHOLE><<<dim3((unsigned)tiles, (unsigned)a.c.heads), 256, lds, stream>>>(a, T);
         });
     } else {
