@@ -599,7 +599,9 @@ int64_t vl_attend_blocks_workspace_bytes(const vl_cache *cache, const vl_tokens 
 int vl_attend_blocks(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
                      const int32_t *blocks, int64_t count,
                      void *workspace, int64_t workspace_bytes, void *stream);
-/* vl_select_blocks, then vl_attend_blocks on its choice, which it leaves in blocks. */
+/* vl_select_blocks, then vl_attend_blocks on its choice, which it leaves in
+ * blocks.  Where scale is negative the choice is made for the negated queries:
+ * the blocks where scale * <query, key> may be largest. */
 int64_t vl_attend_selected_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
                                            int64_t count);
 int vl_attend_selected(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries, int64_t count,

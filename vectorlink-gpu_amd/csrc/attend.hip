@@ -151,11 +151,12 @@ int check_count(int64_t count) {
 }
 
 SelectArgs select_args(const AttendArgs &a, int64_t count) {
-    return {a.c, a.t, a.queries, a.q_row, a.q_head, a.group, (int)count, nullptr, nullptr};
+    return {a.c, a.t, a.queries, a.q_row, a.q_head, a.group, (int)count, 0, nullptr, nullptr};
 }
 
-int choose(const AttendArgs &a, int type, int64_t count, int32_t *blocks, void *workspace, int64_t bytes, hipStream_t stream) {
+int choose(const AttendArgs &a, int type, int64_t count, bool turned, int32_t *blocks, void *workspace, int64_t bytes, hipStream_t stream) {
     SelectArgs s = select_args(a, count);
+    s.turned = turned;
     const int rc = check_workspace(select_workspace_bytes(s), workspace, bytes);
     if (rc != VL_OK) return rc;
     VL_REQUIRE(blocks, "blocks is null");
@@ -211,7 +212,7 @@ VL_EXPORT int vl_select_blocks(const vl_cache *cache, const vl_tokens *tokens, c
     if (rc == VL_OK) rc = check_count(count);
     if (rc != VL_OK || a.t.rows == 0) return rc;
     VL_REQUIRE(a.queries && (uintptr_t)a.queries % (queries->type == VL_F32 ? 4 : 2) == 0, "queries is null or not aligned to its type");
-    return choose(a, queries->type, count, blocks, workspace, workspace_bytes, (hipStream_t)stream);
+    return choose(a, queries->type, count, false, blocks, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 VL_EXPORT int64_t vl_attend_blocks_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
@@ -256,10 +257,11 @@ VL_EXPORT int vl_attend_selected(const vl_cache *cache, const vl_tokens *tokens,
         VL_REQUIRE(blocks, "blocks is null");
         SelectArgs s = select_args(a, count);
         s.out = blocks;
+        s.turned = queries->scale < 0;
         const hipStream_t at = (hipStream_t)stream;
         return queries->type == VL_BF16 ? launch_attend_step<1>(a, s, at) : queries->type == VL_F16 ? launch_attend_step<2>(a, s, at) : launch_attend_step<3>(a, s, at);
     }
-    rc = choose(a, queries->type, count, blocks, workspace, workspace_bytes, (hipStream_t)stream);
+    rc = choose(a, queries->type, count, queries->scale < 0, blocks, workspace, workspace_bytes, (hipStream_t)stream);
     if (rc != VL_OK) return rc;
     const int64_t used = select_workspace_bytes(select_args(a, count));
     a.list = blocks;

@@ -9,6 +9,7 @@ struct SelectArgs {
     int64_t q_row, q_head;
     int group;
     int count;
+    int turned;      // 1: the queries' signs are turned, for scores that a negative scale will be multiplied with
     int32_t *out;    // [rows, c.heads, count]
     uint32_t *keys;  // [rows, c.heads, t.blocks]: scores, in an order that unsigned numbers have
 };

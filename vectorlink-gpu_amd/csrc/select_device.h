@@ -85,7 +85,7 @@ __device__ inline void score_blocks(const SelectArgs &a, const Scored &s, int fr
     const int first_column = WHOLE ? 0 : token * a.group, columns = WHOLE ? 16 : a.group;
     for (int i = first_column; i < min(first_column + columns, 16); i++) top = fmaxf(top, lds.top[wave][i]);
     const int e = max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127 - 6, -100);
-    const float unit = top < INFINITY ? __builtin_bit_cast(float, (uint32_t)(127 - e) << 23) : 0.0f;
+    const float unit = top < INFINITY ? __builtin_bit_cast(float, (uint32_t)(127 - e) << 23 | (uint32_t)a.turned << 31) : 0.0f;
     i32x4 u[kSteps];
     auto ask = [&] {  // the queries in x as the products' operand
 #pragma unroll

@@ -199,7 +199,7 @@ def attend_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tenso
 
 def attend_selected(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, count: int,
                     offsets: Optional[Tensor] = None, scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
-    """(attend_blocks(...), blocks) with the blocks of select_blocks, in one call."""
+    """(attend_blocks(...), blocks) with the blocks of select_blocks (of the negated queries where scale is negative), in one call."""
     assert count >= 1, f"count: {count}"
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
