@@ -3,7 +3,15 @@
 #include "select.h"
 
 constexpr uint32_t kOwnKey = 0xFFFFFFFFu;        // the row's own block
-constexpr uint32_t kBoundlessKey = 0xFFFFFFFEu;  // a block without bounds; every other score is finite and lower
+constexpr uint32_t kBoundlessKey = 0xFFFFFFFEu;  // a block without bounds; every other score is lower
+
+// score 2^power in an order that unsigned numbers have.  As a float32 it would pass the largest one (scores lie below 2^22, powers go
+// up to 121), so the powers of two are added: the bits of |score| without two of mantissa, which are 0, on 2^21 for a binade.
+__device__ inline uint32_t score_key(int score, int power) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, (float)abs(score)) >> 2;
+    const uint32_t size = score ? bits + ((uint32_t)(power + 127) << 21) : 0;  // below 2^30
+    return score < 0 ? (1u << 30) - size : (1u << 30) + size;
+}
 
 // Tokens of a sequence that can share a tile of 16 queries
 __device__ __host__ inline int tokens_a_tile(int group) { return group >= 16 ? 1 : 16 / group; }
@@ -35,8 +43,8 @@ struct Scored {
 // 0 for a block that is none.
 //
 // score = max over the queries of sum_j max(u_j, 0) hi_j + min(u_j, 0) lo_j: one sum over 2 D channels of 8-bit products, which
-// the matrix cores make of 16 blocks x 16 (token, query) pairs at once; it is a whole number below 2^22, exact in float32, and
-// so is its product with the block's power of two.  What bounds it is the bounds' bytes, 2 D a block, and how many of them are on
+// the matrix cores make of 16 blocks x 16 (token, query) pairs at once; it is a whole number below 2^22 and is compared with others
+// exactly, whatever the blocks' powers of two.  What bounds it is the bounds' bytes, 2 D a block, and how many of them are on
 // their way: a wavefront asks for those of several tiles of 16 blocks before it works on the first.  WHOLE: more than 16 queries,
 // which fill several tiles.
 template <int D, int NS, int WAVES, bool WHOLE>
@@ -158,7 +166,7 @@ __device__ inline void score_blocks(const SelectArgs &a, const Scored &s, int fr
                 const int own = min(s.place0 + s.token0 + token, s.length - 1) / kPage;
                 if (block >= to || block > own) return;
                 uint32_t key = 0;
-                if (page >= 0) key = power == kBoundless ? kBoundlessKey : vl_float_key((float)score * __builtin_bit_cast(float, (uint32_t)(power + 127) << 23));
+                if (page >= 0) key = power == kBoundless ? kBoundlessKey : score_key(score, power);
                 if (block == own) key = kOwnKey;
                 keys[token * stride + block] = key;
             };
