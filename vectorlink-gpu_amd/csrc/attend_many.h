@@ -297,9 +297,10 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
             for (int i = 1; i < 32; i++) most_here = fmaxf(most_here, s[i >> 4][i & 15]);
             most_here = max_of_halves(most_here) * a.scale;
             // The maximum that weights are measured from may lie up to 8 below the true one: weights up to 256 cost nothing, and
-            // the sums are rescaled a few times a row instead of at every new maximum.
+            // the sums are rescaled a few times a row instead of at every new maximum.  Each row's moves when that row passes it, so
+            // that no result depends on the rows beside it.
             if (__ballot(most_here > top + 8.0f)) {
-                const float now = fmaxf(top, most_here);
+                const float now = most_here > top + 8.0f ? most_here : top;
                 const float less = now > -INFINITY ? __builtin_amdgcn_exp2f(top - now) : 1.0f;
                 top = now;
                 sum *= less;
