@@ -60,3 +60,15 @@ def test_sequences_without_rows_count_for_nothing():
                 for sequences in (rows + 1, 64, 256, 4096):
                     among = native(rows, sequences, blocks, **kw)
                     assert (lib.vl_attend_form(*among), lib.vl_attend_workspace_bytes(*among)) == want, (rows, sequences, blocks, kw)
+
+
+def test_scales_beyond_float32_are_refused():
+    lib = nv.lib()
+    parts = dict(keys=256, key_scales=256, values=256, value_scales=256, bounds=256, bound_scales=256)
+    cache = C.byref(nv.Cache(pages=10, heads=2, dim=128, **parts))
+    tokens = C.byref(nv.Tokens(rows=3, sequences=3, blocks=4, table_stride=4, table=256, lengths=256))
+    for scale in (1e39, -2.4e38, 1e300, float("inf"), float("nan")):
+        q = C.byref(nv.Queries(heads=8, row_stride=1024, head_stride=128, queries=256, out=256, scale=scale, type=1, causal=1))
+        assert lib.vl_attend(cache, tokens, q, 256, 1 << 40, None) == -1 and b"scale" in lib.vl_last_error()
+        assert lib.vl_attend_blocks(cache, tokens, q, 256, 4, 256, 1 << 40, None) == -1
+        assert lib.vl_attend_selected(cache, tokens, q, 4, 256, 256, 1 << 40, None) == -1

@@ -15,7 +15,7 @@ struct AttendArgs {
     int group, heads_q;     // queries that share a head of the cache; c.heads * group
     int causal;
     float scale;            // |scale| log2(e): exponentials are powers of two here
-    uint32_t sign;          // 0x80000000 where the scale is negative: turns the queries' sign
+    float turn;             // the scale's sign, 0 for no scale at all: what the queries are multiplied with
     int splits;             // workgroups that share a tile
     int waves;              // of attend_few_kernel: wavefronts of a workgroup that share a tile, 4 or 8; 1: four have one each
     float *part;            // splits > 1: [rows * heads_q, splits, D] sums, then [rows * heads_q, splits, 2] maxima and sums of weights

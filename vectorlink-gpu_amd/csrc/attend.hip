@@ -12,6 +12,8 @@ namespace {
 // MB: 39 and 28).
 constexpr int64_t kStepItems = 256, kStepBytes = 1 << 19, kStepFull = 64;
 
+float in_powers_of_two(double scale) { return (float)(fabs(scale) * 1.4426950408889634); }
+
 int attend_args(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *q, bool data, AttendArgs *a) {
     *a = {};
     int rc = vl_cache_of(cache, &a->c);
@@ -28,7 +30,7 @@ int attend_args(const vl_cache *cache, const vl_tokens *tokens, const vl_queries
         VL_REQUIRE(q->queries && q->out, "queries or out is null");
         VL_REQUIRE((uintptr_t)q->queries % size == 0, "queries not aligned to their type");
         VL_REQUIRE(((uintptr_t)q->out & 15) == 0, "out not on a 16-byte boundary");
-        VL_REQUIRE(isfinite(q->scale), "scale is not finite");
+        VL_REQUIRE(isfinite(in_powers_of_two(q->scale)), "scale: %g is not finite, or too large for float32", q->scale);
     }
     a->queries = q->queries;
     a->q_row = q->row_stride;
@@ -38,9 +40,12 @@ int attend_args(const vl_cache *cache, const vl_tokens *tokens, const vl_queries
     a->heads_q = (int)q->heads;
     a->group = (int)(q->heads / a->c.heads);
     a->causal = q->causal != 0;
-    // 0 becomes a scale that leaves all scores 0 after rounding but for those that a mask sets to -inf
-    a->scale = (float)fmax(fabs(q->scale) * 1.4426950408889634, 1e-37);
-    a->sign = q->scale < 0 ? 0x80000000u : 0;
+    a->scale = in_powers_of_two(q->scale);
+    a->turn = q->scale < 0 ? -1.0f : 1.0f;
+    if (a->scale == 0) {  // 0 times the -inf that masks a score would be none: the queries take the 0
+        a->scale = 1;
+        a->turn = 0;
+    }
     a->splits = 1;
     return VL_OK;
 }

@@ -122,14 +122,14 @@ __device__ inline void load_queries(QueryLoads<D, NS> &l, const AttendArgs &a, b
     }
 }
 template <int D, int NS>
-__device__ inline void take_queries(QueryRegs<D, NS> &f, const QueryLoads<D, NS> &l, bool real, uint32_t sign) {
+__device__ inline void take_queries(QueryRegs<D, NS> &f, const QueryLoads<D, NS> &l, bool real, float turn) {
     typedef typename ElementOf<NS>::type E;
 #pragma unroll
     for (int k = 0; k < D / 32; k++) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             __bf16 s[NS];
-            split_into<NS>(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)(real ? l.x[k][i] : (E)0.0f)) ^ sign), s);
+            split_into<NS>((float)(real ? l.x[k][i] : (E)0.0f) * turn, s);
 #pragma unroll
             for (int n = 0; n < NS; n++) f.x[n][k][i] = s[n];
         }
@@ -382,7 +382,7 @@ __device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const Q
         };
         auto look = [&] {  // after the first page's loads
             edges = __ballot(page >= 0 && ((block + 1) * kPage > least || bound == kBoundless));
-            if (first) take_queries<D, NS>(f, queries, real, a.sign);
+            if (first) take_queries<D, NS>(f, queries, real, a.turn);
             first = false;
         };
         PageRegs<D> x;

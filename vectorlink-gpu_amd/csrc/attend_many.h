@@ -187,7 +187,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 __bf16 s[NS];
-                split_into<NS>(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)x[k][i]) ^ a.sign), s);
+                split_into<NS>((float)x[k][i] * a.turn, s);
 #pragma unroll
                 for (int n = 0; n < NS; n++) q[n][k][i] = s[n];
             }
