@@ -1,10 +1,14 @@
-"""Attention over the cache without a GPU: sizes at the ends of what the rules divide by and choose between."""
+"""Attention over the cache without a GPU: sizes at the ends of what the rules divide by and choose between, and what is refused."""
 import ctypes as C
 import os
 import subprocess
 import sys
 
+import pytest
+import torch
+
 from vectorlink_gpu import _native as nv
+from vectorlink_gpu import attention
 
 PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "vectorlink-gpu_amd")
 
@@ -72,3 +76,25 @@ def test_scales_beyond_float32_are_refused():
         assert lib.vl_attend(cache, tokens, q, 256, 1 << 40, None) == -1 and b"scale" in lib.vl_last_error()
         assert lib.vl_attend_blocks(cache, tokens, q, 256, 4, 256, 1 << 40, None) == -1
         assert lib.vl_attend_selected(cache, tokens, q, 4, 256, 256, 1 << 40, None) == -1
+
+
+class Sizes:
+    """Stands for a cache where only its sizes are looked at."""
+    (pages, heads, dim) = (4, 2, 64)
+    _ref = None
+
+
+def test_what_asks_for_a_gradient_is_refused():
+    """There is none: it would be lost without a word."""
+    q = torch.zeros((3, 4, 64), requires_grad=True)
+    (table, lengths) = (torch.zeros((3, 4), dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
+    blocks = torch.zeros((3, 2, 1), dtype=torch.int32)
+    calls = [lambda: attention.attend(q, Sizes, table, lengths), lambda: attention.select_blocks(q, Sizes, table, lengths, 2),
+             lambda: attention.attend_blocks(q, Sizes, table, lengths, blocks), lambda: attention.attend_selected(q, Sizes, table, lengths, 2),
+             lambda: attention.KVCache.write(Sizes, q[:, :2], q[:, 2:].detach(), table, lengths),
+             lambda: attention.KVCache.write(Sizes, q[:, :2].detach(), q[:, 2:], table, lengths)]
+    for call in calls:
+        with pytest.raises(AssertionError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):  # as far as it goes without one
+            call()

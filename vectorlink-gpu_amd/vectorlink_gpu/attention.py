@@ -8,7 +8,8 @@ formats and formulas).
 
 table [sequences, blocks] int32 names the page of each block of 64 tokens of a sequence.  Rows of keys, values and
 queries are tokens; offsets [sequences + 1] int32 says which rows are whose (None: one row a sequence).  Everything is
-enqueued on torch's current stream; nothing is synchronised, and no length is read on the host.
+enqueued on torch's current stream; nothing is synchronised, and no length is read on the host.  There are no gradients: what
+asks for one is refused.
 """
 import ctypes as C
 import struct
@@ -48,6 +49,7 @@ def _check_rows(t: Tensor, name: str, dim: int) -> int:
     assert t.dim() == 3 and t.shape[2] == dim, f"{name} must be [rows, heads, {dim}]"
     assert t.stride(2) == 1, f"the last dimension of {name} must be contiguous"
     assert t.dtype in nv.TYPES, f"{name} must be bfloat16, float16 or float32"
+    assert not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient, and there is none through a cache in 4 bits: call under no_grad"
     return nv.TYPES[t.dtype]
 
 
