@@ -81,6 +81,7 @@ def test_scales_beyond_float32_are_refused():
 class Sizes:
     """Stands for a cache where only its sizes are looked at."""
     (pages, heads, dim) = (4, 2, 64)
+    keys = torch.zeros(1)
     _ref = None
 
 
@@ -98,3 +99,59 @@ def test_what_asks_for_a_gradient_is_refused():
             call()
         with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):  # as far as it goes without one
             call()
+
+
+class On:
+    """Stands for a tensor on a GPU of that number."""
+    is_cuda = True
+
+    def __init__(self, gpu):
+        self.gpu = gpu
+
+    def get_device(self):
+        return self.gpu
+
+
+def test_tensors_of_another_gpu_are_refused(monkeypatch):
+    """Kernels run on the current GPU, on its stream: what lies on another would be read across GPUs, if it can be."""
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda gpu: 100 + gpu, raising=False)
+    assert nv.require_one_gpu(On(1), None, On(1)) == 1 and nv.require_one_gpu(On(0)) == 0
+    assert nv.stream_on(1, 1).value == 101
+    for bad in ((On(1), On(0)), (On(0), None, On(1)), (On(1), torch.zeros(3)), (torch.zeros(3), On(1)), (torch.zeros(3),)):
+        with pytest.raises(RuntimeError, match="GPU"):
+            nv.require_one_gpu(*bad)
+    for bad in ((0,), (1, 0), (0, 0)):
+        with pytest.raises(RuntimeError, match="GPU"):
+            nv.stream_on(*bad)
+
+
+def test_every_call_asks_where_its_tensors_are(monkeypatch):
+    """The cache, what is written or asked, tables, lengths, offsets and lists; and for the stream of that GPU."""
+    (seen, gpus) = ([], [])
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: 0
+
+    class Cache(Sizes):
+        gpu = 5
+
+    monkeypatch.setattr(nv, "lib", Library)
+    monkeypatch.setattr(nv, "require_one_gpu", lambda *tensors: seen.extend(id(t) for t in tensors) or 7)
+    monkeypatch.setattr(nv, "stream_on", lambda *of: gpus.extend(of))
+    (q, kv) = (torch.zeros((3, 4, 64)), torch.zeros((3, 2, 64)))
+    (table, lengths, offsets) = (torch.zeros((3, 4), dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32))
+    blocks = torch.zeros((3, 2, 1), dtype=torch.int32)
+    calls = [(lambda: attention.attend(q, Cache, table, lengths, offsets), [q, table, lengths, offsets]),
+             (lambda: attention.select_blocks(q, Cache, table, lengths, 2, offsets), [q, table, lengths, offsets]),
+             (lambda: attention.attend_blocks(q, Cache, table, lengths, blocks, offsets), [q, table, lengths, offsets, blocks]),
+             (lambda: attention.attend_selected(q, Cache, table, lengths, 2, offsets), [q, table, lengths, offsets]),
+             (lambda: attention.KVCache.write(Cache, kv, kv, table, lengths, offsets), [kv, table, lengths, offsets]),
+             (lambda: attention.KVCache.read(Cache, table, lengths, 3, offsets), [table, lengths, offsets]),
+             (lambda: attention.KVCache.read_bounds(Cache, lengths), [lengths])]
+    for call, tensors in calls:
+        seen.clear()
+        gpus.clear()
+        call()
+        assert {id(t) for t in tensors} <= set(seen) and set(gpus) == {7, 5}

@@ -151,3 +151,22 @@ def require_gpu(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("vectorlink_gpu kernels need tensors on the GPU (there is no CPU path)")
+
+
+def require_one_gpu(*tensors) -> int:
+    """The number of the GPU that all of them lie on."""
+    gpu = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != gpu or gpu < 0):
+            require_gpu(*tensors)
+            raise RuntimeError(f"tensors on several GPUs: {[x.get_device() for x in tensors if x is not None]}")
+    return gpu
+
+
+def stream_on(*gpus) -> C.c_void_p:
+    """stream(), for tensors of these GPUs: kernels run on the current one."""
+    here = torch._C._cuda_getDevice()
+    for gpu in gpus:
+        if gpu != here:
+            raise RuntimeError(f"tensors on GPU {gpu}, and the current one is {here}")
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(here))

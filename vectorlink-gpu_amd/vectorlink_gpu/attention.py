@@ -71,7 +71,7 @@ class KVCache:
                                         (bound_scales, "bound_scales", torch.int8, (pages, heads))):
             assert t.dtype == dtype and tuple(t.shape) == shape, f"{name} must be {dtype} {shape}"
             assert t.is_contiguous(), f"{name} must be contiguous"
-        nv.require_gpu(keys, key_scales, values, value_scales, bounds, bound_scales)
+        self.gpu = nv.require_one_gpu(keys, key_scales, values, value_scales, bounds, bound_scales)
         (self.keys, self.key_scales, self.values, self.value_scales) = (keys, key_scales, values, value_scales)
         (self.bounds, self.bound_scales) = (bounds, bound_scales)
         (self.pages, self.heads, self.dim) = (pages, heads, dim)
@@ -96,9 +96,9 @@ class KVCache:
         assert _check_rows(values, "values", self.dim) == kind and values.shape == keys.shape, "keys and values differ in type or size"
         assert keys.shape[1] == self.heads, f"keys have {keys.shape[1]} heads, the cache {self.heads}"
         tokens = _tokens(keys.shape[0], table, starts, offsets)
-        nv.require_gpu(keys, values, table, starts, offsets)
+        gpu = nv.require_one_gpu(keys, values, table, starts, offsets)
         nv.check(nv.lib().vl_cache_write(self._ref, tokens, kind, keys.data_ptr(), keys.stride(0), keys.stride(1),
-                                         values.data_ptr(), values.stride(0), values.stride(1), nv.stream()))
+                                         values.data_ptr(), values.stride(0), values.stride(1), nv.stream_on(gpu, self.gpu)))
 
     def read(self, table: Tensor, starts: Tensor, rows: int, offsets: Optional[Tensor] = None,
              dtype: torch.dtype = torch.bfloat16) -> Tuple[Tensor, Tensor]:
@@ -106,19 +106,19 @@ class KVCache:
         there, rounded.  rows is the last of offsets, or the number of sequences."""
         assert dtype in nv.TYPES, "dtype must be bfloat16, float16 or float32"
         tokens = _tokens(rows, table, starts, offsets)
-        nv.require_gpu(table, starts, offsets)
+        gpu = nv.require_one_gpu(table, starts, offsets)
         keys = torch.empty((rows, self.heads, self.dim), dtype=dtype, device=self.keys.device)
         values = torch.empty_like(keys)
-        nv.check(nv.lib().vl_cache_read(self._ref, tokens, nv.TYPES[dtype], keys.data_ptr(), values.data_ptr(), nv.stream()))
+        nv.check(nv.lib().vl_cache_read(self._ref, tokens, nv.TYPES[dtype], keys.data_ptr(), values.data_ptr(), nv.stream_on(gpu, self.gpu)))
         return (keys, values)
 
     def read_bounds(self, pages: Tensor) -> Tensor:
         """The largest and the smallest key of these pages in each dimension, rounded outwards: [*pages.shape, heads, 2, dim]."""
         assert pages.dtype == torch.int32, "pages must be int32"
-        nv.require_gpu(pages)
+        gpu = nv.require_one_gpu(pages)
         pages = pages.contiguous()
         out = torch.empty((*pages.shape, self.heads, 2, self.dim), dtype=torch.float32, device=pages.device)
-        nv.check(nv.lib().vl_cache_read_bounds(self._ref, pages.data_ptr(), pages.numel(), out.data_ptr(), nv.stream()))
+        nv.check(nv.lib().vl_cache_read_bounds(self._ref, pages.data_ptr(), pages.numel(), out.data_ptr(), nv.stream_on(gpu, self.gpu)))
         return out
 
 
@@ -150,14 +150,14 @@ def attend(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, offs
     assert form is None or form in nv.ATTEND_FORMS, f"unknown form {form!r}: expected one of {sorted(nv.ATTEND_FORMS)}"
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
-    nv.require_gpu(queries, table, lengths, offsets)
+    gpu = nv.require_one_gpu(queries, table, lengths, offsets)
     out = queries.new_empty(queries.shape)
     lse = queries.new_empty(queries.shape[:2], dtype=torch.float32) if return_lse else None
     q = _queries(queries, cache, scale, causal, out, lse, form)
     lib = nv.lib()
     need = lib.vl_attend_workspace_bytes(cache._ref, tokens, q)
     ws = _workspace(need, queries)
-    nv.check(lib.vl_attend(cache._ref, tokens, q, nv.ptr(ws), need, nv.stream()))
+    nv.check(lib.vl_attend(cache._ref, tokens, q, nv.ptr(ws), need, nv.stream_on(gpu, cache.gpu)))
     return (out, lse) if return_lse else out
 
 
@@ -168,13 +168,13 @@ def select_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tenso
     assert count >= 1, f"count: {count}"
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
-    nv.require_gpu(queries, table, lengths, offsets)
+    gpu = nv.require_one_gpu(queries, table, lengths, offsets)
     blocks = table.new_empty((queries.shape[0], cache.heads, count))
     q = _queries(queries, cache, None, True, None, None)
     lib = nv.lib()
     need = lib.vl_select_blocks_workspace_bytes(cache._ref, tokens, q, count)
     ws = _workspace(need, queries)
-    nv.check(lib.vl_select_blocks(cache._ref, tokens, q, count, blocks.data_ptr(), nv.ptr(ws), need, nv.stream()))
+    nv.check(lib.vl_select_blocks(cache._ref, tokens, q, count, blocks.data_ptr(), nv.ptr(ws), need, nv.stream_on(gpu, cache.gpu)))
     return blocks
 
 
@@ -183,11 +183,10 @@ def attend_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tenso
     """attend over the tokens of blocks [rows, cache.heads, count] alone, up to the row's own place."""
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
-    nv.require_gpu(queries, table, lengths, offsets)
     assert blocks.dtype == torch.int32 and blocks.is_contiguous(), "blocks must be contiguous int32"
     assert blocks.dim() == 3 and blocks.shape[:2] == (queries.shape[0], cache.heads) and blocks.shape[2] > 0, \
         "blocks must be [rows, cache.heads, count]"
-    nv.require_gpu(blocks)
+    gpu = nv.require_one_gpu(queries, table, lengths, blocks, offsets)
     count = blocks.shape[2]
     out = queries.new_empty(queries.shape)
     lse = queries.new_empty(queries.shape[:2], dtype=torch.float32) if return_lse else None
@@ -195,7 +194,7 @@ def attend_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tenso
     lib = nv.lib()
     need = lib.vl_attend_blocks_workspace_bytes(cache._ref, tokens, q, count)
     ws = _workspace(need, queries)
-    nv.check(lib.vl_attend_blocks(cache._ref, tokens, q, blocks.data_ptr(), count, nv.ptr(ws), need, nv.stream()))
+    nv.check(lib.vl_attend_blocks(cache._ref, tokens, q, blocks.data_ptr(), count, nv.ptr(ws), need, nv.stream_on(gpu, cache.gpu)))
     return (out, lse) if return_lse else out
 
 
@@ -205,12 +204,12 @@ def attend_selected(queries: Tensor, cache: KVCache, table: Tensor, lengths: Ten
     assert count >= 1, f"count: {count}"
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
-    nv.require_gpu(queries, table, lengths, offsets)
+    gpu = nv.require_one_gpu(queries, table, lengths, offsets)
     blocks = table.new_empty((queries.shape[0], cache.heads, count))
     out = queries.new_empty(queries.shape)
     q = _queries(queries, cache, scale, True, out, None)
     lib = nv.lib()
     need = lib.vl_attend_selected_workspace_bytes(cache._ref, tokens, q, count)
     ws = _workspace(need, queries)
-    nv.check(lib.vl_attend_selected(cache._ref, tokens, q, count, blocks.data_ptr(), nv.ptr(ws), need, nv.stream()))
+    nv.check(lib.vl_attend_selected(cache._ref, tokens, q, count, blocks.data_ptr(), nv.ptr(ws), need, nv.stream_on(gpu, cache.gpu)))
     return (out, blocks)
