@@ -28,10 +28,17 @@ INT_OPTIONS = [
 ]
 
 
+def at_least_one(text: str) -> int:
+    n = int(text)
+    if n < 1:
+        raise argparse.ArgumentTypeError(f"at least 1, got {n}")
+    return n
+
+
 def parse(argv=None) -> dict:
     parser = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     for short, long_, default, text in INT_OPTIONS:
-        parser.add_argument(short, long_, type=int, default=default, help=text)
+        parser.add_argument(short, long_, type=at_least_one, default=default, help=text)
     return vars(parser.parse_args(argv))
 
 
