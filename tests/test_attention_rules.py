@@ -155,3 +155,19 @@ def test_every_call_asks_where_its_tensors_are(monkeypatch):
         gpus.clear()
         call()
         assert {id(t) for t in tensors} <= set(seen) and set(gpus) == {7, 5}
+
+
+def test_launches_of_a_choice_and_its_attention():
+    """One launch or several, by what was measured: (tokens, heads, dim, type, blocks, count) on either side.  One launch has no workspace."""
+    lib = nv.lib()
+
+    def one(rows, heads, dim, type, blocks, count):
+        (cache, tokens, q) = native(rows, rows, blocks, heads=heads, dim=dim, type=type)
+        return lib.vl_attend_selected_workspace_bytes(cache, tokens, q, count) == 0
+
+    for sizes in ((1, 8, 128, 1, 256, 16), (1, 8, 128, 1, 1024, 32), (1, 8, 128, 1, 1024, 64), (1, 4, 256, 1, 1024, 16), (8, 8, 128, 1, 1000, 64),
+                  (8, 8, 128, 2, 1000, 16), (1, 8, 128, 3, 1000, 16), (32, 8, 128, 1, 512, 32), (32, 8, 128, 1, 8000, 256), (16, 8, 128, 1, 1000, 256)):
+        assert one(*sizes), sizes
+    for sizes in ((1, 8, 128, 1, 2048, 32), (1, 8, 128, 1, 1040, 16), (1, 4, 64, 1, 2048, 32), (1, 8, 128, 1, 256, 64), (8, 8, 128, 1, 300, 256),
+                  (8, 8, 64, 1, 300, 256), (8, 8, 256, 1, 1000, 256), (1, 8, 128, 3, 256, 32), (4, 8, 128, 2, 300, 64), (16, 8, 128, 1, 300, 256)):
+        assert not one(*sizes), sizes

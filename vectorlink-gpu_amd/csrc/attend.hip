@@ -6,11 +6,9 @@
 
 namespace {
 
-// Tokens times heads up to which one launch for a choice and its attention is the faster: a workgroup for each compute unit (512
-// workgroups over 8,192 tokens each: 56 us, in several launches 45; 128 over 131,072: 46 and 57).  A compute unit alone reads about
-// 25 GB/s, so few workgroups take it for few bytes each (8 over 32,768 tokens, 0.4 MB each: 24 and 29 us; over 131,072, 0.8
-// MB: 39 and 28).
-constexpr int64_t kStepItems = 256, kStepBytes = 1 << 19, kStepFull = 64;
+// Tokens times heads up to which one launch may take a choice and its attention: a workgroup for each compute unit (512 workgroups over
+// 8,192 tokens each: 56 us, in several launches 45).
+constexpr int64_t kStepItems = 256;
 
 float in_powers_of_two(double scale) { return (float)(fabs(scale) * 1.4426950408889634); }
 
@@ -58,9 +56,9 @@ int64_t few_tiles(const AttendArgs &a) {
 }
 
 // How the pages of a tile are shared out.  A tile for every wavefront where that alone gives every SIMD two.  A workgroup of 8
-// wavefronts for a tile where that leaves each at most four pages (two of a list, whose call has more launches anyway: 8 tiles of
-// 32 blocks 13.2 us, and 6.9 and 4.4 split and joined), which takes no second launch to join (1,000 tokens, 32 heads:
-// 14.5 us in two launches, 10.3 in one).  Else workgroups of 4, as many a tile as give every compute unit one (two for float32,
+// wavefronts for a tile where that leaves each at most four pages, two of a list, which takes no second launch to join (1,000 tokens, 32
+// heads: 14.5 us in two launches, 10.3 in one; 8 tiles with lists of 16, 20 and 32 blocks, in a graph: 9.0, 9.7 and 12.3 us in one, 9.5,
+// 9.5 and 9.6 in two).  Else workgroups of 4, as many a tile as give every compute unit one (two for float32,
 // which is three times the products), but two pages (one) for every wavefront: parts cost their starts and ends, and joining them.
 // One workgroup a compute unit and two: one sequence of 65,536 tokens 27 us and 36, 32 of 4,096 to 8,192 with 8 heads of 8 47 and 53,
 // in float32 68 and 59.  Two pages a wavefront and one: 2 sequences of 16,384 19 us and 27.
@@ -170,11 +168,26 @@ int choose(const AttendArgs &a, int type, int64_t count, bool turned, int32_t *b
     return launch_select(s, type, stream);
 }
 
-// Whether attend_step_kernel takes a choice and the attention over it: few tokens, and for one workgroup not too many bytes.
+// What the single launch takes, in ns beside what both ways have in common: its workgroup works on one block after the other.
+int64_t step_takes(const AttendArgs &a, int type, int64_t count) {
+    const int64_t chosen = count * (40 + a.c.dim * 7 / 5);  // bfloat16
+    return a.t.blocks * (36 + a.c.dim) / 18 + (type == VL_BF16 ? chosen : type == VL_F16 ? chosen * 11 / 10 : chosen * 3 / 2);
+}
+// What several launches take: one or two more, a choice by a workgroup for a token or scores by many (0.13 ns each) and a choice from
+// them, and the chosen pages at about 6 TB/s.
+int64_t several_take(const AttendArgs &a, int64_t count) {
+    const int64_t items = (int64_t)a.t.rows * a.c.heads, pages = items * count * (kPage * (a.c.dim + a.c.dim / 16)) / 6000;
+    const int64_t choice = chosen_in_one(select_args(a, count)) ? a.t.blocks * (420 + a.c.dim) / 28 : 5000 + items * a.t.blocks * 13 / 100;
+    return 1500 + 12 * a.c.dim + choice + pages;
+}
+// Whether attend_step_kernel takes a choice and the attention over it.  us in one launch and in several, next to where the rule changes
+// sides, for 8 tokens times heads (bfloat16 of 128): 32 of 256 blocks 20.4 and 21.3, 64 of 256 26.9 and 21.2, 64 of 1,024 33.1 and 35.0, 128
+// of 1,024 45.8 and 35.4, 16 of 1,024 23.8 and 33.6, 16 of 1,040 24.3 and 21.6; for 64: 64 of 300 28.2 and 25.2, of 1,000 34.8 and 38.5, of
+// 2,000 43.5 and 36.2, 16 of 2,000 33.0 and 32.3; for 128: 256 of 300 67.1 and 61.3, of 1,000 73.5 and 74.4.  64 and 256 dimensions, half
+// precision and float32 change sides as the figures above have it, to 2 us of 20 to 50.
 bool in_one_step(const AttendArgs &a, int type, int64_t count) {
-    const int64_t items = (int64_t)a.t.rows * a.c.heads, bytes = (int64_t)a.t.blocks * 2 * a.c.dim + count * kPage * (a.c.dim + a.c.dim / 16);
-    return step_built(a.c.dim, type) && a.group <= 16 && a.t.blocks <= 16384 && count <= 2048 && items <= kStepItems &&
-           (bytes <= kStepBytes || items >= kStepFull);
+    return step_built(a.c.dim, type) && a.group <= 16 && a.t.blocks <= 16384 && count <= 2048 && (int64_t)a.t.rows * a.c.heads <= kStepItems &&
+           step_takes(a, type, count) <= several_take(a, count);
 }
 
 }  // namespace

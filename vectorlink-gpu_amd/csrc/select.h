@@ -13,5 +13,7 @@ struct SelectArgs {
     int32_t *out;    // [rows, c.heads, count]
     uint32_t *keys;  // [rows, c.heads, t.blocks]: scores, in an order that unsigned numbers have
 };
+// One workgroup a token scores and chooses where that fills the GPU or the blocks are few; else they are scored by many.
+bool chosen_in_one(const SelectArgs &a);
 int64_t select_workspace_bytes(const SelectArgs &a);
 int launch_select(const SelectArgs &a, int type, hipStream_t stream);

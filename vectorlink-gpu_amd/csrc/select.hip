@@ -11,8 +11,6 @@ int tokens_together(const SelectArgs &a) {
     const int fit = kLdsKeys / (a.t.blocks > 1 ? a.t.blocks : 1), T = tokens_a_tile(a.group);
     return fit < T ? fit : T;
 }
-// One workgroup a token scores and chooses where that fills the GPU or the blocks are few; else they are scored by many.
-bool in_one(const SelectArgs &a) { return tokens_together(a) > 0 && (a.t.blocks <= 1024 || (int64_t)a.t.rows * a.c.heads >= kComputeUnits); }
 
 // What a workgroup of choose_kernel has of LDS beside the scores
 struct ChooseKernelLds {
@@ -67,7 +65,7 @@ __global__ __launch_bounds__(512) void select_kernel(SelectArgs a) {
 template <int NS, bool WHOLE>
 int launch(const SelectArgs &a, hipStream_t stream) {
     hipError_t e = hipSuccess;
-    if (in_one(a)) {
+    if (chosen_in_one(a)) {
         const int T = tokens_together(a);
         const int64_t tiles = a.t.offsets ? a.t.rows / T + sequences_with_rows(a.t) : a.t.rows;
         VL_REQUIRE(tiles <= 4 * kMaxBlocks, "more rows than one call takes: %lld", (long long)tiles);
@@ -93,8 +91,10 @@ int launch(const SelectArgs &a, hipStream_t stream) {
 
 }  // namespace
 
+bool chosen_in_one(const SelectArgs &a) { return tokens_together(a) > 0 && (a.t.blocks <= 1024 || (int64_t)a.t.rows * a.c.heads >= kComputeUnits); }
+
 int64_t select_workspace_bytes(const SelectArgs &a) {
-    return in_one(a) ? 0 : ((int64_t)a.t.rows * a.c.heads * a.t.blocks * 4 + 255) / 256 * 256;
+    return chosen_in_one(a) ? 0 : ((int64_t)a.t.rows * a.c.heads * a.t.blocks * 4 + 255) / 256 * 256;
 }
 
 int launch_select(const SelectArgs &a, int type, hipStream_t stream) {
