@@ -37,7 +37,7 @@ int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
                 attend_few_kernel<D, NS, 4, C><<<dim3(groups, heads), 256, sizeof(JoinLds<4>), stream>>>(a, (int)tiles);
             }
         });
-        launch_join<D, NS>(a, stream);
+        if (e == hipSuccess) launch_join<D, NS>(a, stream);
     });
     VL_HIP(e);
     VL_LAUNCH_CHECK("attend_few_kernel");

@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheView c, Tokens t,
     uint8_t *const ks = c.key_scales + unit * (kPage * D / 32), *const vs = c.value_scales + unit * (kPage * D / 32);
 
     const int seg = threadIdx.x % T, at = threadIdx.x / T;
-    const uint64_t mine = T == 64 ? ~0ull : ((1ull << T) - 1) << ((threadIdx.x & 63) / T * T);  // lanes of my token
+    const uint64_t mine = ((1ull << T) - 1) << ((threadIdx.x & 63) / T * T);  // lanes of my token
     float hi[8], lo[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
