@@ -173,12 +173,12 @@ int64_t step_takes(const AttendArgs &a, int type, int64_t count) {
     const int64_t chosen = count * (40 + a.c.dim * 7 / 5);  // bfloat16
     return a.t.blocks * (36 + a.c.dim) / 18 + (type == VL_BF16 ? chosen : type == VL_F16 ? chosen * 11 / 10 : chosen * 3 / 2);
 }
-// What several launches take: one or two more, a choice by a workgroup for a token or scores by many (0.13 ns each) and a choice from
-// them, and the chosen pages at about 6 TB/s.
+// What several launches take: one or two more, and 1 us because fewer are to be had for the same; a choice by a workgroup for a token,
+// or scores by many (0.13 ns each) and a choice from them; the chosen pages at about 6 TB/s.
 int64_t several_take(const AttendArgs &a, int64_t count) {
     const int64_t items = (int64_t)a.t.rows * a.c.heads, pages = items * count * (kPage * (a.c.dim + a.c.dim / 16)) / 6000;
     const int64_t choice = chosen_in_one(select_args(a, count)) ? a.t.blocks * (420 + a.c.dim) / 28 : 5000 + items * a.t.blocks * 13 / 100;
-    return 1500 + 12 * a.c.dim + choice + pages;
+    return 2500 + 12 * a.c.dim + choice + pages;
 }
 // Whether attend_step_kernel takes a choice and the attention over it.  us in one launch and in several, next to where the rule changes
 // sides, for 8 tokens times heads (bfloat16 of 128): 32 of 256 blocks 20.4 and 21.3, 64 of 256 26.9 and 21.2, 64 of 1,024 33.1 and 35.0, 128
