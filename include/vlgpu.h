@@ -556,7 +556,7 @@ typedef struct vl_queries {
     const void *queries;
     void *out;
     float *lse;
-    double scale; /* scores are scale * <query, key> */
+    double scale; /* scores are scale * <query, key>; finite, as a float32 too */
     int32_t type; /* VL_BF16, VL_F16, VL_F32 */
     int32_t causal; /* 0: every row sees all lengths[b] tokens; else those up to its own place */
     int64_t form; /* of vl_attend: 0, or VL_ATTEND_FEW or VL_ATTEND_MANY whatever the sizes, for tests and measurements */
@@ -578,12 +578,14 @@ int vl_attend_form(const vl_cache *cache, const vl_tokens *tokens, const vl_quer
 
 /* blocks [rows, cache.heads, count]: for every row and head of the cache the
  * block of the row's own token and the others up to it with the best scores,
- * ascending, then VL_MAXINT.  The score of a block is an upper bound of the
- * largest <query, key> in it: with u the queries of the row that share the head
+ * ascending, then VL_MAXINT.  With u the queries of the row that share the head
  * rounded to 8 bits with one power of two (largest magnitude in [64, 128), cut
- * to 127), the largest over these queries of sum_j max(u_j, 0) hi_j +
- * min(u_j, 0) lo_j, hi and lo the block's bounds; whole numbers times a power
- * of two, so that no order of the sum changes one.  Blocks without bounds (127)
+ * to 127; the power is 2^-100 at least), the score of a block is the largest
+ * over these queries of sum_j max(u_j, 0) hi_j + min(u_j, 0) lo_j, hi and lo the
+ * block's bounds: no <u, key> in the block is above it (a <query, key> may be,
+ * by what the rounding of the query took).  Scores are whole numbers times a
+ * power of two, so that no order of the sum changes one, and are compared
+ * exactly.  Blocks without bounds (127)
  * come before all others, ties go to the lower block; queries that are not
  * finite count as zeros.  A row before the first token has no blocks.
  * queries->out, lse, scale and causal are not looked at. */

@@ -4,8 +4,8 @@
 // What bounds it is the cache's bytes: D + D / 16 a token and head, against 4 D operations for each of the queries that share
 // the head.  So a wavefront takes whole pages, 64 tokens at a time, every byte read once in 16-byte pieces, and keeps the
 // rest in registers; a maximum and a sum that run along (x -> exp2(x - max), both rescaled where the maximum grows) make one
-// pass of it.  Measured: 4 tokens over 131,072, 32 heads on 8 of 128, 570 MB in 101 us (5.6 TB/s; a sum of 2 GiB reads 6.2); 64
-// over 4,096 to 8,192 429 MB in 86 us, where the longest sequences' workgroups are waited for.
+// pass of it.  Measured: 4 tokens over 131,072, 32 heads on 8 of 128, 570 MB in 100 us (5.7 TB/s; a sum of 2 GiB reads 6.1 to 6.2) and
+// 5 us to join; 64 over 4,096 to 8,192 429 MB in 84 to 90 us, where the longest sequences' workgroups are waited for.
 //
 // S^T = K Q^T: A = 16 tokens x 32 dimensions, B = 32 dimensions x 16 rows (row = lane % 16 = r, quad = lane / 16 = c).  Which
 // token stands in which row of A and which dimension at which place of the sum is free, as long as both operands agree:

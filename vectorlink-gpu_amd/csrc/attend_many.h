@@ -5,8 +5,8 @@
 // share the head, one after the other - and takes a page of 64 tokens at a time: all wavefronts turn its bytes into bfloat16
 // in LDS once, then each reads all of it for 32 rows of its own.  PAGES pages a round, two sets of buffers, one barrier a round:
 // the next pages' bytes are on their way while these are worked on, and are turned into the other buffers after them.  Measured:
-// 2,048 rows over 16,384 tokens, 32 heads on 8 of 128, 490 us (1,050 TFLOP/s; a large library product of bfloat16 1,216), matrix
-// units busy 42 % and vector units 45 % of the time; in half precision, twice the products, 1,180 TFLOP/s of them.
+// 2,048 rows over 16,384 tokens, 32 heads on 8 of 128, 478 us (1,080 TFLOP/s; a large library product of bfloat16 1,216 to 1,248),
+// matrix units busy 46 % and vector units 49 % of the time; some cards take 500.
 //
 // S^T = K Q^T in tiles of 32 tokens x 32 rows: lane l holds row l % 32, and of a tile the tokens 8 (i / 4) + 4 (l / 32) + i % 4.
 // out^T = V^T P^T takes P^T as it lies, 16 tokens a step: of half l / 32 the tokens 16 s + 4 (l / 32) + j and those 8 further, so
@@ -152,8 +152,10 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
     typedef Images<D> I;
     typedef typename ElementOf<NS>::type E;
     constexpr int kRows = 32 * WAVES, kBuffer = I::kBytes + kPage;
-    // Parts of a weight, as many as of a query: a bfloat16 result's error is then sqrt(2) times that of its own rounding at most, and
-    // a second part would make half as many products again (half precision and float32 keep 16 and 24 bits).
+    // Parts of a weight, as many as of a query (half precision and float32 keep 16 and 24 bits).  A bfloat16 weight is off by up to
+    // 2^-8 of itself, the sum that it is divided by is not: over 16,384 tokens the result's error is 1.16 times that of its own
+    // rounding (root of the mean square, 5.00e-4 and 4.30e-4), and more where values cancel.  A second part makes half as many products
+    // again and takes that away, for 661 us instead of 494; dividing by the sum of the rounded weights leaves 4.95e-4 for 506.
     constexpr int NW = NS;
     extern __shared__ __attribute__((aligned(16))) char lds[];
 

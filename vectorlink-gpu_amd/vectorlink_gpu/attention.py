@@ -146,7 +146,8 @@ def attend(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, offs
     dim], heads a multiple of the cache's; scale defaults to dim ** -0.5.  The rows of a sequence are its last tokens and see
     what stands before them and themselves, or with causal=False everything.  A row that sees nothing gives zeros.  With
     return_lse also the logarithms of the sums of exponentials [rows, heads], by which parts of an attention are joined.
-    form: the library chooses one by the sizes; "few" or "many" ask for it, for tests and measurements."""
+    form: the library chooses one by the sizes; "few" or "many" ask for it, for tests and measurements.  Of bfloat16 "many" rounds the
+    weights to bfloat16 as well, "few" holds 16 bits of them."""
     assert form is None or form in nv.ATTEND_FORMS, f"unknown form {form!r}: expected one of {sorted(nv.ATTEND_FORMS)}"
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
@@ -164,7 +165,7 @@ def attend(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, offs
 def select_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, count: int,
                   offsets: Optional[Tensor] = None) -> Tensor:
     """For every row and head of the cache `count` blocks of its sequence, ascending: the row's own and those with the highest
-    upper bound on a score in them, by queries and bounds of 8 bits; MAXINT where there are no more.  [rows, cache.heads, count]"""
+    bound on a score in them, of queries rounded to 8 bits and keys' bounds of 8 bits; MAXINT where there are no more.  [rows, cache.heads, count]"""
     assert count >= 1, f"count: {count}"
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
