@@ -307,7 +307,8 @@ def _plain_write(state):
 
 def _plain_evict(state):
     """Tokens are ranked: the latest `recent` positions before all others, then by weight, of equal ones the earlier place.  The best
-    `keep` stay; those of them that stand behind the first `keep` places move, in their order, to the places there that got free."""
+    `keep` stay; those of them that stand behind the first `keep` places move, in their order, to the places there that got free.  What
+    stands behind the first `keep` places is left as it is, also on the page where they end, whose power may have grown."""
     (case, cache) = (state["case"], state["tensors"])
     (keep, batch, heads) = (case["keep"], case["batch"], case["heads"])
     cache["weights"].copy_(state["weights"])  # as another part of the program left them
@@ -327,6 +328,10 @@ def _plain_evict(state):
     (page, token) = (at[b, to // PAGE], to % PAGE)
     (page0, token0) = (at[b, source // PAGE], source % PAGE)
     unit = page * heads + h
+    stands = torch.full((cache["keys"].size(0),), PAGE, device=DEV)  # tokens of a page before the first `keep` places end
+    if keep < weights.size(2):
+        stands[at[:, keep // PAGE]] = keep % PAGE
+    token_of = {"keys": torch.arange(PAGE, device=DEV)[:, None], "values": torch.arange(PAGE, device=DEV).view(16, 1, 4)}
     for (which, name) in ((0, "keys"), (1, "values")):
         x = cache[name][page0, h, token0] if which == 0 else cache[name][page0, h, token0 // 4, :, token0 % 4]
         x = _decoded(x, cache["scales"][page0, h, which])
@@ -334,7 +339,9 @@ def _plain_evict(state):
         e = was.scatter_reduce(0, unit, _least_exponent(x.abs().amax(-1)), "amax")  # of every page and head
         grown = (e > was).nonzero()[:, 0]
         flat = cache[name].flatten(0, 1)
-        flat[grown] = _coded(_decoded(flat[grown].flatten(1), was[grown] + 127), e[grown][:, None]).view_as(flat[grown])
+        old = flat[grown]
+        again = _coded(_decoded(old.flatten(1), was[grown] + 127), e[grown][:, None]).view_as(old)
+        flat[grown] = torch.where(token_of[name] < stands[grown // heads].view(-1, *[1] * (old.dim() - 1)), again, old)
         cache["scales"][..., which] = (e + 127).view(-1, heads).to(torch.uint8)
         if which:
             cache[name][page, h, token // 4, :, token % 4] = _coded(x, e[unit][:, None])
@@ -516,7 +523,9 @@ def _exact_evict(state, lengths):
                 e = exponent[:, h, which].scatter_reduce(0, page1, need, "amax")
                 grown = (e > exponent[:, h, which]).nonzero()[:, 0]
                 was = torch.exp2(exponent[grown, h, which].double())[:, None, None]
+                before = codes[which][page[keep // PAGE], h, keep % PAGE:].clone()
                 codes[which][grown, h] = _nearest(codes[which][grown, h] * was, e[grown][:, None, None])
+                codes[which][page[keep // PAGE], h, keep % PAGE:] = before  # behind what stays nothing changes
                 exponent[:, h, which] = e
                 codes[which][page1, h, to % PAGE] = _nearest(x, e[page1][:, None])
             weights[page1, h, to % PAGE] = w[source]
