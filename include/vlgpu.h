@@ -609,6 +609,72 @@ int64_t vl_attend_selected_workspace_bytes(const vl_cache *cache, const vl_token
 int vl_attend_selected(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries, int64_t count,
                        int32_t *blocks, void *workspace, int64_t workspace_bytes, void *stream);
 
+/* ---- a key/value cache in 8 bits, its tokens' weights, and eviction ------ */
+/* No counterpart in the reference.  The same pages, tables and tokens with
+ * twice the bytes and a quarter of the rounding, for contexts that are bounded
+ * the other way: what was looked at least leaves the cache.
+ *
+ * An element is a code of 8 bits (E4M3: sign, four bits of exponent, three of
+ * mantissa, largest 448, no infinity) times a power of two that the 64 tokens of
+ * a page share, one for the keys and one for the values of each head.
+ *   keys       [pages, heads, 64, dim]
+ *   values     [pages, heads, 16, dim, 4]  token / 4, dim, token % 4
+ *   scales     [pages, heads, 4]           exponent + 127 of the keys' power and of the values'; 1 if a token of the
+ *                                          page may not be finite; 0
+ *   weights    [pages, heads, 64]          accumulated weights; or NULL, and positions with it: a cache that nothing
+ *   positions  [pages, heads, 64]          is evicted from needs neither
+ * dim: 32, 64, 96, 128, 192 or 256.  All pointers on 16-byte boundaries. */
+typedef struct vl_cache8 {
+    int64_t pages, heads, dim;
+    uint8_t *keys, *values, *scales;
+    float *weights;
+    int32_t *positions;
+} vl_cache8;
+
+/* vl_cache_write for such a cache.  The power of a block that is written into is
+ * the least 2^e, -117 <= e <= 119, whose 448-fold is not below any new element
+ * (magnitudes over 448 * 2^119 become that); if the block holds tokens already it is the old power at least, and where it grows
+ * they are rounded to it again.  Codes are the nearest ones, of two as near the
+ * even one.  A token with an element that is not finite reads as NaN, and its
+ * elements do not count for the power.  New tokens have weight 0 and position
+ * positions[row], NULL: their place in the sequence.  Two sequences must not
+ * share a page that is written into. */
+int vl_cache8_write(const vl_cache8 *cache, const vl_tokens *tokens, int type,
+                    const void *keys, int64_t key_row, int64_t key_head,
+                    const void *values, int64_t value_row, int64_t value_head,
+                    const int32_t *positions, void *stream);
+int vl_cache8_read(const vl_cache8 *cache, const vl_tokens *tokens, int type,
+                   void *keys, void *values, void *stream);
+
+/* vl_attend over such a cache.  accumulate: every token's weight grows by the
+ * sum of the softmax weights that it gets, over all rows and the queries that
+ * share its head; a row with a score or a sum that is not finite adds nothing.
+ * The sum is made in 32 bits and in one order, so that no weight depends on
+ * chance; no two sequences may share a page then. */
+int64_t vl_attend8_workspace_bytes(const vl_cache8 *cache, const vl_tokens *tokens, const vl_queries *queries, int accumulate);
+int vl_attend8(const vl_cache8 *cache, const vl_tokens *tokens, const vl_queries *queries, int accumulate,
+               void *workspace, int64_t workspace_bytes, void *stream);
+int vl_attend8_form(const vl_cache8 *cache, const vl_tokens *tokens, const vl_queries *queries);
+
+/* Cuts every sequence down to `keep` tokens.  tokens: rows == sequences, offsets
+ * NULL, lengths: what the sequences hold.  In each head of a sequence of more
+ * than `keep` tokens they are ranked: those whose position is one of the last
+ * `recent` (above the largest position of the head minus recent) before all
+ * others, then by weight, NaN last, of equal ones the earlier place first.  The
+ * best `keep` stay.  Those of them behind the first `keep` places move, in their
+ * order, into the places before that got free, with weight and position: heads
+ * differ in what they keep and in its order, which attention does not depend on.
+ * A page that tokens move to has its power raised to what they need and its
+ * tokens rounded to it.  Places from the new length on are left as they are.
+ * Tokens on no page leave first: new_lengths[b] is the smaller of keep and the
+ * tokens on pages, of a sequence of at most keep tokens its length (cut to what
+ * its table can name); what would move to a place on no page is lost.  0 <=
+ * recent <= keep.  No two sequences may share a page.  new_lengths must not be
+ * lengths. */
+int64_t vl_cache8_evict_workspace_bytes(const vl_cache8 *cache, const vl_tokens *tokens, int64_t keep);
+int vl_cache8_evict(const vl_cache8 *cache, const vl_tokens *tokens, int64_t keep, int64_t recent,
+                    int32_t *new_lengths, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,7 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 OUT = os.path.join(HERE, "vectorlink_gpu", "libvlgpu.so")
 
-SOURCES = ["error.cpp", "dist.hip", "queue.hip", "seed.hip", "prune.hip", "beam.hip", "beam_unaligned.hip", "beam_table.hip", "pair_table.hip", "knn.hip", "knn_few.hip", "knn_filter.hip", "graphopt.hip", "sketch.hip", "cache.hip", "select.hip", "attend.hip", "attend_bf16.hip", "attend_f16.hip", "attend_f32.hip"]
+SOURCES = ["error.cpp", "dist.hip", "queue.hip", "seed.hip", "prune.hip", "beam.hip", "beam_unaligned.hip", "beam_table.hip", "pair_table.hip", "knn.hip", "knn_few.hip", "knn_filter.hip", "graphopt.hip", "sketch.hip", "cache.hip", "select.hip", "attend.hip", "attend_bf16.hip", "attend_f16.hip", "attend_f32.hip", "cache8.hip", "attend8_bf16.hip", "attend8_f16.hip", "attend8_f32.hip", "weigh.hip", "evict.hip"]
 
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",

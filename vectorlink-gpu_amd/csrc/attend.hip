@@ -12,9 +12,13 @@ constexpr int64_t kStepItems = 256;
 
 float in_powers_of_two(double scale) { return (float)(fabs(scale) * 1.4426950408889634); }
 
-int attend_args(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *q, bool data, AttendArgs *a) {
+int cache_of(const vl_cache *cache, CacheView *out) { return vl_cache_of(cache, out); }
+int cache_of(const vl_cache8 *cache, CacheView *out) { return vl_cache8_of(cache, out); }
+
+template <class Cache>
+int attend_args(const Cache *cache, const vl_tokens *tokens, const vl_queries *q, bool data, AttendArgs *a) {
     *a = {};
-    int rc = vl_cache_of(cache, &a->c);
+    int rc = cache_of(cache, &a->c);
     if (rc == VL_OK) rc = vl_tokens_of(tokens, &a->t);
     if (rc != VL_OK) return rc;
     VL_REQUIRE(q != nullptr, "queries is null");
@@ -128,6 +132,7 @@ int check_workspace(int64_t need, const void *workspace, int64_t bytes) {
     return VL_OK;
 }
 
+template <int BITS = 4>
 int attend_few(AttendArgs &a, int type, void *workspace, int64_t bytes, hipStream_t stream) {
     const int64_t tiles = few_tiles(a);
     const Shares shares = shares_for(a, type, tiles);
@@ -136,16 +141,35 @@ int attend_few(AttendArgs &a, int type, void *workspace, int64_t bytes, hipStrea
     const int rc = check_workspace(part_bytes(a, a.splits), workspace, bytes);
     if (rc != VL_OK) return rc;
     a.part = (float *)workspace;
-    return type == VL_BF16 ? launch_attend_few<1>(a, tiles, stream) : type == VL_F16 ? launch_attend_few<2>(a, tiles, stream) : launch_attend_few<3>(a, tiles, stream);
+    return type == VL_BF16 ? launch_attend_few<1, BITS>(a, tiles, stream) : type == VL_F16 ? launch_attend_few<2, BITS>(a, tiles, stream)
+                                                                                         : launch_attend_few<3, BITS>(a, tiles, stream);
 }
 
+template <int BITS = 4>
 int attend_many(AttendArgs &a, int type, void *workspace, int64_t bytes, hipStream_t stream) {
     const int64_t tiles = many_tiles(a);
     a.splits = many_splits(a);
     const int rc = check_workspace(part_bytes(a, a.splits), workspace, bytes);
     if (rc != VL_OK) return rc;
     a.part = (float *)workspace;
-    return type == VL_BF16 ? launch_attend_many<1>(a, tiles, stream) : type == VL_F16 ? launch_attend_many<2>(a, tiles, stream) : launch_attend_many<3>(a, tiles, stream);
+    return type == VL_BF16 ? launch_attend_many<1, BITS>(a, tiles, stream) : type == VL_F16 ? launch_attend_many<2, BITS>(a, tiles, stream)
+                                                                                          : launch_attend_many<3, BITS>(a, tiles, stream);
+}
+
+// What a call over a cache in 8 bits has of its workspace: parts, and where weights are added up the rows' ends and, of single tokens
+// whose queries are one tile, their scores.
+struct Space {
+    int64_t part, ends, scores;
+    int64_t bytes() const { return part + ends + scores; }
+};
+Space space_of(const AttendArgs &a, const vl_queries *q, bool accumulate) {
+    auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+    const bool many = takes_many(a, q);
+    Space s = {part_bytes(a, many ? many_splits(a) : shares_for(a, q->type, few_tiles(a)).splits), 0, 0};
+    if (!accumulate) return s;
+    s.ends = up((int64_t)a.t.rows * a.heads_q * 8);
+    if (!many && !a.t.offsets && a.group <= 16) s.scores = up((int64_t)a.t.rows * a.heads_q * a.t.blocks * kPage * 4);
+    return s;
 }
 
 int check_count(int64_t count) {
@@ -213,6 +237,37 @@ VL_EXPORT int vl_attend(const vl_cache *cache, const vl_tokens *tokens, const vl
     if (rc != VL_OK || a.t.rows == 0) return rc;
     return takes_many(a, queries) ? attend_many(a, queries->type, workspace, workspace_bytes, (hipStream_t)stream)
                                         : attend_few(a, queries->type, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+VL_EXPORT int vl_attend8_form(const vl_cache8 *cache, const vl_tokens *tokens, const vl_queries *queries) {
+    AttendArgs a;
+    const int rc = attend_args(cache, tokens, queries, false, &a);
+    return rc != VL_OK ? rc : takes_many(a, queries) ? VL_ATTEND_MANY : VL_ATTEND_FEW;
+}
+
+VL_EXPORT int64_t vl_attend8_workspace_bytes(const vl_cache8 *cache, const vl_tokens *tokens, const vl_queries *queries, int accumulate) {
+    AttendArgs a;
+    const int rc = attend_args(cache, tokens, queries, false, &a);
+    return rc != VL_OK ? rc : space_of(a, queries, accumulate != 0).bytes();
+}
+
+VL_EXPORT int vl_attend8(const vl_cache8 *cache, const vl_tokens *tokens, const vl_queries *queries, int accumulate, void *workspace,
+                         int64_t workspace_bytes, void *stream) {
+    AttendArgs a;
+    int rc = attend_args(cache, tokens, queries, true, &a);
+    if (rc != VL_OK || a.t.rows == 0) return rc;
+    VL_REQUIRE(!accumulate || a.c.weights || a.c.pages == 0, "the cache has no weights");
+    const Space space = space_of(a, queries, accumulate != 0);
+    rc = check_workspace(space.bytes(), workspace, workspace_bytes);
+    if (rc != VL_OK) return rc;
+    if (space.ends) a.ends = (float *)((uint8_t *)workspace + space.part);
+    if (space.scores) a.scores = (float *)((uint8_t *)workspace + space.part + space.ends);
+    const hipStream_t s = (hipStream_t)stream;
+    const int type = queries->type;
+    rc = takes_many(a, queries) ? attend_many<8>(a, type, workspace, space.part, s) : attend_few<8>(a, type, workspace, space.part, s);
+    if (rc != VL_OK || !accumulate) return rc;
+    if (a.scores) return launch_weigh_scores(a, s);
+    return type == VL_BF16 ? launch_weigh_rows<1>(a, s) : type == VL_F16 ? launch_weigh_rows<2>(a, s) : launch_weigh_rows<3>(a, s);
 }
 
 VL_EXPORT int64_t vl_select_blocks_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,

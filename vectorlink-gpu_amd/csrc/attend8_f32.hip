@@ -1,0 +1,7 @@
+// Attention over a cache in 8 bits with queries of type f32.
+#include "attend_launch.h"
+#include "weigh.h"
+
+template int launch_attend_few<3, 8>(const AttendArgs &, int64_t, hipStream_t);
+template int launch_attend_many<3, 8>(const AttendArgs &, int64_t, hipStream_t);
+template int launch_weigh_rows<3>(const AttendArgs &, hipStream_t);

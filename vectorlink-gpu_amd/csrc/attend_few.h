@@ -22,15 +22,21 @@
 #pragma once
 #include "attend.h"
 
-template <int D>
+template <int D, int BITS = 4>
 struct Parts {  // D = parts of 128, then 64, then 32
     static constexpr int k128 = D / 128, k64 = D % 128 / 64, k32 = D % 64 / 32, kCount = k128 + k64 + k32;
     static constexpr int width(int p) { return p < k128 ? 128 : p == k128 && k64 ? 64 : 32; }
     static constexpr int base(int p) { return p <= k128 ? 128 * p : 128 * k128 + 64; }
 };
+template <int D>
+struct Parts<D, 8> {  // D = parts of 64, then 32: 16 bytes are half as many dimensions
+    static constexpr int k64 = D / 64, k32 = D % 64 / 32, kCount = k64 + k32;
+    static constexpr int width(int p) { return p < k64 ? 64 : 32; }
+    static constexpr int base(int p) { return 64 * p; }
+};
 
 // one page of a head, as a lane holds it
-template <int D>
+template <int D, int BITS = 4>
 struct PageRegs {
     static constexpr int P = Parts<D>::kCount;
     uint32_t k[P][4][4];  // [part][tile m][word]
@@ -75,6 +81,40 @@ __device__ inline void load_page(PageRegs<D> &g, const CacheView &c, int64_t pag
     }
 }
 
+// A page in 8 bits: the same tokens and dimensions of parts of 64 (32).  A word of values is a dimension's codes of four tokens, so
+// two halves of it turn into the pairs of tokens that the second product takes, without permutations.
+template <int D>
+struct PageRegs<D, 8> {
+    static constexpr int P = Parts<D, 8>::kCount;
+    u32x4 k[P][4];          // [part][tile m]: of 64 dimensions the 16 from q * 16 on
+    u32x4 v[P][4];          // [part][4 tokens m], a word a dimension: 4 r + j, or 2 r + j
+    float key_scale, value_scale;
+};
+template <int D>
+__device__ inline void load_page(PageRegs<D, 8> &g, const CacheView &c, int64_t page, int h) {
+    typedef Parts<D, 8> PT;
+    const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
+    const int64_t unit = page * c.heads + h;
+    const uint8_t *const kc = c.keys + unit * (kPage * D), *const vc = c.values + unit * (kPage * D);
+    const int token = (r >> 2) * 16 + (r & 3);
+    auto load = [](u32x4 &to, const uint8_t *at, int width) {
+        if (width == 64) {
+            to = *reinterpret_cast<const u32x4 *>(at);
+        } else {
+            const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
+            to[0] = x[0], to[1] = x[1];
+        }
+    };
+#pragma unroll
+    for (int m = 0; m < 4; m++)
+#pragma unroll
+        for (int p = 0; p < PT::kCount; p++) load(g.k[p][m], kc + (token + m * 4) * D + PT::base(p) + q * (PT::width(p) / 4), PT::width(p));
+#pragma unroll
+    for (int m = 0; m < 4; m++)
+#pragma unroll
+        for (int p = 0; p < PT::kCount; p++) load(g.v[p][m], vc + ((q * 4 + m) * D + PT::base(p) + r * (PT::width(p) / 16)) * 4, PT::width(p));
+}
+
 // NS bfloat16 values that add up to x (to 8 NS bits of it): the first NS - 1 cut off, so that what is left is exact.
 template <int NS>
 __device__ inline void split_into(float x, __bf16 (&out)[NS]) {
@@ -108,9 +148,9 @@ template <int D, int NS>
 struct QueryLoads {
     Eight<NS> x[D / 32];
 };
-template <int D, int NS>
+template <int D, int NS, int BITS = 4>
 __device__ inline void load_queries(QueryLoads<D, NS> &l, const AttendArgs &a, bool real, int64_t row, int head) {
-    typedef Parts<D> PT;
+    typedef Parts<D, BITS> PT;
     typedef typename ElementOf<NS>::type E;
     const int q = (threadIdx.x & 63) >> 4;
     const E *const at = (const E *)a.queries + (real ? row * a.q_row + head * a.q_head : 0);
@@ -191,10 +231,11 @@ __device__ inline float over_copies(float x, F f) {
 
 // A page's 64 tokens: this lane's row (r % C) sees the first `sees` of them, `written` hold something; edge: some row does not see
 // some token, or some token may not be finite.  Spoilt tokens (scale 255) turn the rows that see them into NaN, and no others.
-template <int D, int NS, int C>
-__device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryRegs<D, NS> &f, float scale, bool edge, int sees,
-                                 int written) {
-    typedef Parts<D> PT;
+// to: where this lane's row of scores goes, from the page's first token on, or null.
+template <int D, int NS, int C, int BITS>
+__device__ inline void take_page(RowState<D> &st, PageRegs<D, BITS> &g, const QueryRegs<D, NS> &f, float scale, bool edge, int sees,
+                                 int written, float *to) {
+    typedef Parts<D, BITS> PT;
     constexpr int NW = NS < 2 ? 2 : NS;  // parts of a weight
     constexpr int M = C / 4;             // tiles of 4 tokens of this lane
     const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
@@ -208,13 +249,18 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryReg
 #pragma unroll
     for (int p = 0; p < PT::kCount; p++) {
         float ks[4];
+        if constexpr (BITS == 4) {
 #pragma unroll
-        for (int m = 0; m < 4; m++) ks[m] = __builtin_bit_cast(float, __builtin_amdgcn_alignbit(g.ks[p][m], g.ks[p][m], turn));
+            for (int m = 0; m < 4; m++) ks[m] = __builtin_bit_cast(float, __builtin_amdgcn_alignbit(g.ks[p][m], g.ks[p][m], turn));
+        }
 #pragma unroll
         for (int j = 0; j < PT::width(p) / 32; j++) {
             bf16x8 k[4];
 #pragma unroll
-            for (int m = 0; m < 4; m++) k[m] = eight_values(g.k[p][m][j], ks[m]);
+            for (int m = 0; m < 4; m++) {
+                if constexpr (BITS == 4) k[m] = eight_values(g.k[p][m][j], ks[m]);
+                else k[m] = eight_of_bytes(g.k[p][m][2 * j], g.k[p][m][2 * j + 1], g.key_scale);
+            }
 #pragma unroll
             for (int n = 0; n < NS; n++)
 #pragma unroll
@@ -232,26 +278,53 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryReg
     spread_scores<C>(s, t);
     if (edge) {
         const int m0 = M * (r / C);
+        // of 4 tokens m a word whose bytes tell which are spoilt
+        auto marks = [&](int m) {
+            if constexpr (BITS == 4) return (uint32_t)g.vs[0][m];
+            else return g.v[0][m][0];
+        };
+        auto is_spoilt = [](uint32_t word, int e) {
+            if constexpr (BITS == 4) return (word >> (8 * e) & 255) == kNotFinite;
+            else return (word >> (8 * e) & 127) == kByteNaN;
+        };
 #pragma unroll
         for (int k = 0; k < M; k++) {
-            uint32_t word = g.vs[0][k];
-            if constexpr (C == 4) word = r < 4 ? g.vs[0][0] : r < 8 ? g.vs[0][1] : r < 12 ? g.vs[0][2] : g.vs[0][3];
-            if constexpr (C == 8) word = r < 8 ? g.vs[0][k] : g.vs[0][2 + k];
+            uint32_t word = marks(k);
+            if constexpr (C == 4) word = r < 4 ? marks(0) : r < 8 ? marks(1) : r < 12 ? marks(2) : marks(3);
+            if constexpr (C == 8) word = r < 8 ? marks(k) : marks(2 + k);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                if ((word >> (8 * e) & 255) == kNotFinite) t[k][e] = NAN;
+                if (is_spoilt(word, e)) t[k][e] = NAN;
                 if (q * 16 + (m0 + k) * 4 + e >= sees) t[k][e] = -INFINITY;
             }
         }
         // values of a token that is spoilt or not there: its weight is 0 or NaN whatever it holds, so any finite value will do
 #pragma unroll
-        for (int m = 0; m < 4; m++)
+        for (int m = 0; m < 4; m++) {
+            if constexpr (BITS == 4) {
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if ((g.vs[0][m] >> (8 * e) & 255) == kNotFinite || q * 16 + m * 4 + e >= written) {
+                for (int e = 0; e < 4; e++)
+                    if (is_spoilt(marks(m), e) || q * 16 + m * 4 + e >= written) {
 #pragma unroll
-                    for (int p = 0; p < PT::kCount; p++) g.vs[p][m] = (g.vs[p][m] & ~(255u << (8 * e))) | (127u << (8 * e));
-                }
+                        for (int p = 0; p < PT::kCount; p++) g.vs[p][m] = (g.vs[p][m] & ~(255u << (8 * e))) | (127u << (8 * e));
+                    }
+            } else {
+                uint32_t keep = ~0u;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (is_spoilt(marks(m), e) || q * 16 + m * 4 + e >= written) keep &= ~(255u << (8 * e));
+#pragma unroll
+                for (int p = 0; p < PT::kCount; p++)
+#pragma unroll
+                    for (int j = 0; j < PT::width(p) / 16; j++) g.v[p][m][j] &= keep;
+            }
+        }
+    }
+    if constexpr (BITS == 8) {
+        if (to) {
+#pragma unroll
+            for (int k = 0; k < M; k++) *reinterpret_cast<f32x4 *>(to + q * 16 + (M * (r / C) + k) * 4) = f32x4{t[k][0], t[k][1], t[k][2], t[k][3]};
+        }
     }
     float top = t[0][0];
 #pragma unroll
@@ -298,6 +371,17 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryReg
 #pragma unroll
         for (int p = 0; p < PT::kCount; p++) {
             const int W = PT::width(p), t0 = PT::base(p) / 16;
+            if constexpr (BITS == 8) {
+                bf16x8 a[4];
+#pragma unroll
+                for (int j = 0; j < W / 16; j++) a[j] = eight_of_bytes(g.v[p][2 * h][j], g.v[p][2 * h + 1][j], g.value_scale);
+#pragma unroll
+                for (int n = 0; n < NW; n++)
+#pragma unroll
+                    for (int j = 0; j < W / 16; j++) st.acc[t0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j], w[n], st.acc[t0 + j], 0, 0, 0);
+                continue;
+            }
+            if constexpr (BITS == 4) {
             uint32_t word[8];
             float vs[8];
 #pragma unroll
@@ -334,6 +418,7 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D> &g, const QueryReg
                 two_tiles(std::integral_constant<int, 3>(), a[1]);
                 products(t0 + 4, a, 4);
             }
+            }
         }
     }
 }
@@ -351,9 +436,9 @@ struct Blocks {
 // tokens over 4,096 to 8,192 and 8 heads; 128: 94 and 92; 96, and 128 of float32, spill); behind the last one the same page is loaded once more instead
 // of a branch, over which the compiler would have to wait for all loads.  The queries' loads are waited for with the first
 // page's.
-template <int D, int NS, int C>
+template <int D, int NS, int C, int BITS = 4>
 __device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const QueryLoads<D, NS> &queries, bool real, Blocks l, int b,
-                                   int h, int sees, int least, int most, int length) {
+                                   int h, int sees, int least, int most, int length, float *scores = nullptr) {
     const int lane = threadIdx.x & 63;
     QueryRegs<D, NS> f;
     bool first = true;
@@ -367,29 +452,38 @@ __device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const Q
         }
         uint64_t left = __ballot(page >= 0), edges = 0;
         if (!left) continue;
-        const int bound = a.c.bound_scales[(int64_t)max(page, 0) * a.c.heads + h];  // there is a page
+        const int64_t unit = (int64_t)max(page, 0) * a.c.heads + h;  // there is a page
+        int bound = 0;
+        uint32_t scales = 0;
+        if constexpr (BITS == 4) bound = a.c.bound_scales[unit];
+        else scales = a.c.scales[unit];
         int at = 0;
-        auto next = [&](PageRegs<D> &g) {  // the next page's loads
+        auto next = [&](PageRegs<D, BITS> &g) {  // the next page's loads
             if (left) {
                 at = __builtin_ctzll(left);
                 left &= left - 1;
             }
             load_page<D>(g, a.c, __builtin_amdgcn_readlane(page, at), h);
         };
-        auto take = [&](PageRegs<D> &g, int at) {
+        auto take = [&](PageRegs<D, BITS> &g, int at) {
             const int first = __builtin_amdgcn_readlane(block, at) * kPage;
-            take_page<D, NS, C>(st, g, f, a.scale, edges >> at & 1, sees - first, length - first);
+            if constexpr (BITS == 8) {
+                const uint32_t word = __builtin_amdgcn_readlane(scales, at);
+                g.key_scale = scale_of_keys(word);
+                g.value_scale = scale_of_values(word);
+            }
+            take_page<D, NS, C, BITS>(st, g, f, a.scale, edges >> at & 1, sees - first, length - first, scores ? scores + first : nullptr);
         };
         auto look = [&] {  // after the first page's loads
-            edges = __ballot(page >= 0 && ((block + 1) * kPage > least || bound == kBoundless));
+            edges = __ballot(page >= 0 && ((block + 1) * kPage > least || (BITS == 4 ? bound == kBoundless : is_marked(scales))));
             if (first) take_queries<D, NS>(f, queries, real, a.turn);
             first = false;
         };
-        PageRegs<D> x;
+        PageRegs<D, BITS> x;
         next(x);
         look();
-        if constexpr (D == 64 || (D == 128 && NS < 3)) {
-            PageRegs<D> y;
+        if constexpr (BITS == 4 ? D == 64 || (D == 128 && NS < 3) : D <= 64) {
+            PageRegs<D, BITS> y;
             for (;;) {
                 int here = at;
                 bool last = !left;
@@ -445,8 +539,9 @@ __device__ inline void put_sums(const AttendArgs &a, int64_t out_row, int split,
         float *const to = a.part + (int64_t)a.t.rows * a.heads_q * a.splits * D + (out_row * a.splits + split) * 2;
         to[0] = top;
         to[1] = total;
-    } else if (a.lse) {
-        a.lse[out_row] = (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+    } else {
+        if (a.lse) a.lse[out_row] = (top + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+        if (a.ends) *reinterpret_cast<f32x2 *>(a.ends + out_row * 2) = f32x2{top, total};
     }
 }
 
@@ -458,9 +553,9 @@ struct JoinLds {
     float sum[WAVES][16 * kJoinPad];
     float top[WAVES][16], all[WAVES][16];
 };
-template <int D, int NS, int WAVES, int C, class F>
+template <int D, int NS, int WAVES, int C, int BITS = 4, class F>
 __device__ inline void join_waves(const RowState<D> &st, JoinLds<WAVES> &s, const AttendArgs &a, int split, F out_row) {
-    typedef Parts<D> PT;
+    typedef Parts<D, BITS> PT;
     const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15, wave = threadIdx.x >> 6;
     const float sum = sum_of_row<C>(st.sum);
     if (q == 0) {
@@ -505,9 +600,9 @@ __device__ inline void join_waves(const RowState<D> &st, JoinLds<WAVES> &s, cons
 // A tile is 16 rows of one head: of the queries of one token where there is a list, of all tokens of a sequence otherwise.
 // The WAVES wavefronts of a workgroup share a tile's blocks and are joined; 1: each of four has a tile of its own.  C: the most
 // rows that a tile has, 16 unless its rows are one token's, which see the same.
-template <int D, int NS, int WAVES, int C>
+template <int D, int NS, int WAVES, int C, int BITS = 4>
 __global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 : 1) void attend_few_kernel(AttendArgs a, int tiles) {
-    typedef Parts<D> PT;
+    typedef Parts<D, BITS> PT;
     constexpr bool JOIN = WAVES > 1;
     const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -546,13 +641,17 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 
     least = __builtin_amdgcn_readfirstlane(least);
 
     QueryLoads<D, NS> f;
-    load_queries<D, NS>(f, a, real, row0 + (int64_t)token, head);
+    load_queries<D, NS, BITS>(f, a, real, row0 + (int64_t)token, head);
     RowState<D> st;
     start_rows<D>(st);
     const int entries = a.list ? a.count : (most + kPage - 1) / kPage;
     const int from = (int)((int64_t)entries * split / a.splits), to = (int)((int64_t)entries * (split + 1) / a.splits);
     const int32_t *const list = a.list ? a.list + ((row0 + (int64_t)token0) * a.c.heads + h) * a.count : nullptr;
-    take_blocks<D, NS, C>(st, a, f, real, {list, JOIN ? from + wave : from, WAVES, to}, b, h, C < 16 ? most : sees, least, most, length);
+    float *scores = nullptr;
+    if constexpr (BITS == 8) {  // of one token's queries, all in one tile
+        if (a.scores && r % C < a.group) scores = a.scores + ((row0 + (int64_t)token0) * a.heads_q + h * a.group + r % C) * ((int64_t)a.t.blocks * kPage);
+    }
+    take_blocks<D, NS, C, BITS>(st, a, f, real, {list, JOIN ? from + wave : from, WAVES, to}, b, h, C < 16 ? most : sees, least, most, length, scores);
 
     auto out_row = [&](int r) {
         const int i = w.piece * 16 + r;
@@ -560,7 +659,7 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 
     };
     if constexpr (JOIN) {
         extern __shared__ __attribute__((aligned(16))) char lds[];  // a JoinLds<WAVES>
-        join_waves<D, NS, WAVES, C>(st, *reinterpret_cast<JoinLds<WAVES> *>(lds), a, split, out_row);
+        join_waves<D, NS, WAVES, C, BITS>(st, *reinterpret_cast<JoinLds<WAVES> *>(lds), a, split, out_row);
     } else {
         const float total = sum_of_row<C>(st.sum);
         const int64_t to = out_row(r);
@@ -626,4 +725,5 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
         for (int k = 0; k < kEach; k++) ((E *)a.out)[row * D + at + k] = (E)(x[k] * by);
     }
     if (lane == 0 && a.lse) a.lse[row] = (most + __builtin_amdgcn_logf(total)) * 0.6931471805599453f;
+    if (lane == 0 && a.ends) *reinterpret_cast<f32x2 *>(a.ends + row * 2) = f32x2{most, total};
 }

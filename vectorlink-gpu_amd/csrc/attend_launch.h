@@ -17,7 +17,7 @@ void launch_join(const AttendArgs &a, hipStream_t stream) {
     if (a.splits > 1) attend_join_kernel<D, NS><<<(unsigned)(((int64_t)a.t.rows * a.heads_q + 3) / 4), 256, 0, stream>>>(a);
 }
 
-template <int NS>
+template <int NS, int BITS>
 int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
     VL_REQUIRE(tiles * a.splits <= 4 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)tiles);
     hipError_t e = hipSuccess;
@@ -27,14 +27,14 @@ int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
         for_rows(a.list || !a.t.offsets ? a.group : 16, [&](auto c) {
             constexpr int C = decltype(c)::value;
             if (a.waves == 1) {
-                attend_few_kernel<D, NS, 1, C><<<dim3((unsigned)((tiles + 3) / 4), heads), 256, 0, stream>>>(a, (int)tiles);
+                attend_few_kernel<D, NS, 1, C, BITS><<<dim3((unsigned)((tiles + 3) / 4), heads), 256, 0, stream>>>(a, (int)tiles);
             } else if (a.waves == 8) {
                 if constexpr (D <= 128) {
-                    e = vl_allow_lds(attend_few_kernel<D, NS, 8, C>, sizeof(JoinLds<8>));
-                    if (e == hipSuccess) attend_few_kernel<D, NS, 8, C><<<dim3(groups, heads), 512, sizeof(JoinLds<8>), stream>>>(a, (int)tiles);
+                    e = vl_allow_lds(attend_few_kernel<D, NS, 8, C, BITS>, sizeof(JoinLds<8>));
+                    if (e == hipSuccess) attend_few_kernel<D, NS, 8, C, BITS><<<dim3(groups, heads), 512, sizeof(JoinLds<8>), stream>>>(a, (int)tiles);
                 }
             } else {
-                attend_few_kernel<D, NS, 4, C><<<dim3(groups, heads), 256, sizeof(JoinLds<4>), stream>>>(a, (int)tiles);
+                attend_few_kernel<D, NS, 4, C, BITS><<<dim3(groups, heads), 256, sizeof(JoinLds<4>), stream>>>(a, (int)tiles);
             }
         });
         if (e == hipSuccess) launch_join<D, NS>(a, stream);
@@ -44,7 +44,7 @@ int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
     return VL_OK;
 }
 
-template <int NS>
+template <int NS, int BITS>
 int launch_attend_many(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
     const int64_t groups = tiles * a.splits * a.c.heads;
     VL_REQUIRE(groups <= 2 * kMaxBlocks, "more rows than one call takes: %lld tiles", (long long)groups);
@@ -53,9 +53,9 @@ int launch_attend_many(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
         constexpr int D = decltype(d)::value, W = many_waves(D), P = many_pages(D);
         if constexpr (many_built(D, NS)) {
             constexpr size_t lds = 2 * P * (Images<D>::kBytes + kPage);
-            e = vl_allow_lds(attend_many_kernel<D, NS, W, P>, lds);
+            e = vl_allow_lds(attend_many_kernel<D, NS, W, P, BITS>, lds);
             if (e != hipSuccess) return;
-            attend_many_kernel<D, NS, W, P><<<(unsigned)groups, W * 64, lds, stream>>>(a, (int)tiles);
+            attend_many_kernel<D, NS, W, P, BITS><<<(unsigned)groups, W * 64, lds, stream>>>(a, (int)tiles);
             launch_join<D, NS>(a, stream);
         }
     });

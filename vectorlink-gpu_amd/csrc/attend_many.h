@@ -29,16 +29,25 @@ struct Images {
 };
 
 // What a thread brings of a page: keys of D / 4 dimensions of a token, values of 8 dimensions of 4 tokens.
-template <int D>
+template <int D, int BITS = 4>
 struct KeyPart {
     uint32_t w[D / 32];
     uint8_t scale[D / 32];
 };
-template <int D>
+template <int D, int BITS = 4>
 struct ValuePart {
     static constexpr int kUnits = D <= 128 ? 1 : 2;
     u32x4 w[kUnits];
     uint32_t scale[kUnits];
+};
+template <int D>
+struct KeyPart<D, 8> {
+    uint32_t w[D / 16];
+};
+template <int D>
+struct ValuePart<D, 8> {
+    static constexpr int kUnits = D <= 128 ? 1 : 2;
+    u32x4 w[kUnits][2];  // a word a dimension
 };
 
 template <int D>
@@ -134,6 +143,74 @@ __device__ inline void store_values(const ValuePart<D> &g, char *lds, uint8_t *s
     }
 }
 
+template <int D>
+__device__ inline void fetch_keys(KeyPart<D, 8> &g, const CacheView &c, int64_t unit, int id) {
+    const int token = (id >> 6) * 16 + (id & 15), q = id >> 4 & 3;
+    const uint8_t *const at = c.keys + unit * (kPage * D) + token * D + q * (D / 4);
+    if constexpr (D % 64 == 0) {
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) {
+            const u32x4 x = reinterpret_cast<const u32x4 *>(at)[i];
+#pragma unroll
+            for (int k = 0; k < 4; k++) g.w[4 * i + k] = x[k];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+            const u32x2 x = reinterpret_cast<const u32x2 *>(at)[i];
+            g.w[2 * i] = x[0];
+            g.w[2 * i + 1] = x[1];
+        }
+    }
+}
+template <int D>
+__device__ inline void store_keys(const KeyPart<D, 8> &g, char *lds, int id, float scale) {
+    typedef Images<D> I;
+    const int token = (id >> 6) * 16 + (id & 15), q = id >> 4 & 3;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++)
+        *reinterpret_cast<bf16x8 *>(lds + I::key(token, q * (D / 32) + i)) = eight_of_bytes(g.w[2 * i], g.w[2 * i + 1], scale);
+}
+template <int D>
+__device__ inline void fetch_values(ValuePart<D, 8> &g, const CacheView &c, int64_t unit, int id) {
+    const int four = id & 15;
+    const uint8_t *const vc = c.values + unit * (kPage * D);
+#pragma unroll
+    for (int u = 0; u < ValuePart<D, 8>::kUnits; u++) {
+        const int seg = (id >> 4) + u * 16;
+        if (seg < D / 8) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) g.w[u][k] = reinterpret_cast<const u32x4 *>(vc + (four * D + seg * 8) * 4)[k];
+        }
+    }
+}
+template <int D>
+__device__ inline void store_values(const ValuePart<D, 8> &g, char *lds, uint8_t *spoilt, int id, bool edge, int written, float scale) {
+    typedef Images<D> I;
+    const int four = id & 15;
+    const int chunk = (four >> 2) * 2 + (four & 1), half = four >> 1 & 1;  // as above
+#pragma unroll
+    for (int u = 0; u < ValuePart<D, 8>::kUnits; u++) {
+        const int seg = (id >> 4) + u * 16;
+        if (seg >= D / 8) continue;
+        uint32_t keep = ~0u;
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const bool bad = (g.w[u][0][0] >> (8 * i) & 127) == kByteNaN;
+                if (seg == 0) spoilt[four * 4 + i] = bad;
+                if (bad || four * 4 + i >= written) keep &= ~(255u << (8 * i));  // see take_page
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < 8; d++) {
+            const uint32_t word = g.w[u][d >> 2][d & 3] & keep;
+            *reinterpret_cast<u32x2 *>(lds + I::value(seg * 8 + d, chunk) + half * 8) =
+                u32x2{two_of_bytes<false>(word, scale), two_of_bytes<true>(word, scale)};
+        }
+    }
+}
+
 __device__ inline float max_of_halves(float x) {
     const uint32_t u = __builtin_bit_cast(uint32_t, x);
     const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
@@ -147,7 +224,7 @@ __device__ inline float sum_of_halves(float x) {
     return __builtin_bit_cast(float, a0) + __builtin_bit_cast(float, a1);
 }
 
-template <int D, int NS, int WAVES, int PAGES>
+template <int D, int NS, int WAVES, int PAGES, int BITS = 4>
 __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, int tiles) {
     typedef Images<D> I;
     typedef typename ElementOf<NS>::type E;
@@ -202,18 +279,23 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
         for (int i = 0; i < 16; i++) acc[d][i] = 0;
     float top = -INFINITY, sum = 0;
 
-    KeyPart<D> kp[PAGES];
-    ValuePart<D> vp[PAGES];
+    KeyPart<D, BITS> kp[PAGES];
+    ValuePart<D, BITS> vp[PAGES];
     const int id = threadIdx.x & 255;
     const bool brings_keys = WAVES == 4 || wave < 4, brings_values = WAVES == 4 || wave >= 4;
     auto fetch = [&](int k, int page) {
         if (brings_keys) fetch_keys<D>(kp[k], a.c, (int64_t)page * a.c.heads + h, id);
         if (brings_values) fetch_values<D>(vp[k], a.c, (int64_t)page * a.c.heads + h, id);
     };
-    auto store = [&](int k, int buffer, int block, bool edge) {
+    auto store = [&](int k, int buffer, int block, bool edge, uint32_t scales) {
         char *const to = lds + buffer * kBuffer;
-        if (brings_keys) store_keys<D>(kp[k], to, id);
-        if (brings_values) store_values<D>(vp[k], to, (uint8_t *)to + I::kBytes, id, edge, length - block * kPage);
+        if constexpr (BITS == 4) {
+            if (brings_keys) store_keys<D>(kp[k], to, id);
+            if (brings_values) store_values<D>(vp[k], to, (uint8_t *)to + I::kBytes, id, edge, length - block * kPage);
+        } else {
+            if (brings_keys) store_keys<D>(kp[k], to, id, scale_of_keys(scales));
+            if (brings_values) store_values<D>(vp[k], to, (uint8_t *)to + I::kBytes, id, edge, length - block * kPage, scale_of_values(scales));
+        }
     };
 
     const int blocks = (most + kPage - 1) / kPage;
@@ -221,15 +303,21 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
     // 64 blocks' pages are looked up at once, a lane each, and handed out as scalars: a lookup of the next page would be waited for
     // at the head of every round
     int pages = -1;
+    uint32_t scales = 0;  // of a cache in 8 bits
     uint64_t edges = 0;
     auto look_up = [&](int block) {
         block += lane;
         pages = block < to ? (int)page_of(a.t, a.c, b, block) : -1;
-        edges = __ballot(pages >= 0 && ((block + 1) * kPage > least || a.c.bound_scales[(int64_t)pages * a.c.heads + h] == kBoundless));
+        if constexpr (BITS == 4) {
+            edges = __ballot(pages >= 0 && ((block + 1) * kPage > least || a.c.bound_scales[(int64_t)pages * a.c.heads + h] == kBoundless));
+        } else {
+            scales = pages >= 0 ? a.c.scales[(int64_t)pages * a.c.heads + h] : 0;
+            edges = __ballot(pages >= 0 && ((block + 1) * kPage > least || is_marked(scales)));
+        }
     };
     look_up(from);
     int page[PAGES], next[PAGES];
-    uint32_t edge = 0, next_edge = 0;
+    uint32_t edge = 0, next_edge = 0, next_scales[PAGES] = {};
 #pragma unroll
     for (int k = 0; k < PAGES; k++) {
         page[k] = __builtin_amdgcn_readlane(pages, k);
@@ -238,7 +326,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
     edge = (uint32_t)edges & ((1u << PAGES) - 1);
 #pragma unroll
     for (int k = 0; k < PAGES; k++)
-        if (page[k] >= 0) store(k, k, from + k, edge >> k & 1);
+        if (page[k] >= 0) store(k, k, from + k, edge >> k & 1, __builtin_amdgcn_readlane(scales, k));
     __syncthreads();
     for (int round = from, turn = 0; round < to; round += PAGES, turn ^= 1) {
         const int at = round + PAGES - from & 63;
@@ -247,6 +335,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
 #pragma unroll
         for (int k = 0; k < PAGES; k++) {
             next[k] = __builtin_amdgcn_readlane(pages, at + k);  // -1 behind the last
+            if constexpr (BITS == 8) next_scales[k] = __builtin_amdgcn_readlane(scales, at + k);
             if (next[k] >= 0) fetch(k, next[k]);
         }
 #pragma unroll
@@ -343,7 +432,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
         }
 #pragma unroll
         for (int k = 0; k < PAGES; k++) {
-            if (next[k] >= 0) store(k, (turn ^ 1) * PAGES + k, round + PAGES + k, next_edge >> k & 1);
+            if (next[k] >= 0) store(k, (turn ^ 1) * PAGES + k, round + PAGES + k, next_edge >> k & 1, next_scales[k]);
             page[k] = next[k];
         }
         edge = next_edge;
@@ -376,4 +465,5 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
             *reinterpret_cast<e4 *>(out + d * 32 + i * 8 + hi * 4) =
                 e4{(E)(acc[d][4 * i] * by), (E)(acc[d][4 * i + 1] * by), (E)(acc[d][4 * i + 2] * by), (E)(acc[d][4 * i + 3] * by)};
     if (hi == 0 && a.lse) a.lse[out_row] = (top + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+    if (hi == 0 && a.ends) *reinterpret_cast<f32x2 *>(a.ends + out_row * 2) = f32x2{top, sum};
 }

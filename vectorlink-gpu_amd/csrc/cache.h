@@ -34,6 +34,10 @@ struct CacheView {
     int heads, dim;
     uint8_t *keys, *key_scales, *values, *value_scales;
     int8_t *bounds, *bound_scales;
+    // of a cache in 8 bits (cache8.h), which has none of the scales and bounds above
+    uint32_t *scales;
+    float *weights;
+    int32_t *positions;
 };
 
 // The tokens of a call: rows [offsets[b], offsets[b + 1]) are new tokens of sequence b (offsets == nullptr: row b alone), whose

@@ -28,6 +28,11 @@ class Cache(C.Structure):
         "keys", "key_scales", "values", "value_scales", "bounds", "bound_scales")]
 
 
+class Cache8(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("pages", "heads", "dim")] + [(n, C.c_void_p) for n in (
+        "keys", "values", "scales", "weights", "positions")]
+
+
 class Tokens(C.Structure):
     _fields_ = [(n, C.c_int64) for n in ("rows", "sequences", "blocks", "table_stride")] + [
         (n, C.c_void_p) for n in ("table", "lengths", "offsets")]
@@ -100,6 +105,13 @@ _SIGNATURES = {
     "vl_attend_workspace_bytes": (C.c_int64, [_ptr, _ptr, _ptr]),
     "vl_attend_form": (C.c_int, [_ptr, _ptr, _ptr]),
     "vl_attend": (C.c_int, [_ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
+    "vl_cache8_write": (C.c_int, [_ptr, _ptr, C.c_int, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr]),
+    "vl_cache8_read": (C.c_int, [_ptr, _ptr, C.c_int, _ptr, _ptr, _ptr]),
+    "vl_attend8_workspace_bytes": (C.c_int64, [_ptr, _ptr, _ptr, C.c_int]),
+    "vl_attend8_form": (C.c_int, [_ptr, _ptr, _ptr]),
+    "vl_attend8": (C.c_int, [_ptr, _ptr, _ptr, C.c_int, _ptr, _i64, _ptr]),
+    "vl_cache8_evict_workspace_bytes": (C.c_int64, [_ptr, _ptr, _i64]),
+    "vl_cache8_evict": (C.c_int, [_ptr, _ptr, _i64, _i64, _ptr, _ptr, _i64, _ptr]),
     "vl_select_blocks_workspace_bytes": (C.c_int64, [_ptr, _ptr, _ptr, _i64]),
     "vl_select_blocks": (C.c_int, [_ptr, _ptr, _ptr, _i64, _ptr, _ptr, _i64, _ptr]),
     "vl_attend_blocks_workspace_bytes": (C.c_int64, [_ptr, _ptr, _ptr, _i64]),

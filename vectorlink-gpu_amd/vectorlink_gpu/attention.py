@@ -1,10 +1,14 @@
-"""Attention over a key/value cache held in 4 bits (no counterpart in the reference; include/vlgpu.h has the
+"""Attention over a key/value cache held in 4 or 8 bits (no counterpart in the reference; include/vlgpu.h has the
 formats and formulas).
 
     cache = KVCache.empty(pages, heads, dim)                  # pages of 64 tokens, for any number of sequences
     cache.write(keys, values, table, starts)                  # new tokens behind the `starts` tokens a sequence has
     out = attend(queries, cache, table, starts + 1)           # over everything
     out, blocks = attend_selected(queries, cache, table, starts + 1, count=32)   # over the 32 best blocks of each token
+
+    cache = KVCache8.empty(pages, heads, dim, weighted=True)  # twice the bytes, and weights of its tokens
+    out = attend(queries, cache, table, lengths, accumulate=True)     # adds the weights that the queries give the tokens
+    lengths = cache.evict(table, lengths, keep=4096, recent=256)      # the 4,096 that got most, and the latest, stay
 
 table [sequences, blocks] int32 names the page of each block of 64 tokens of a sequence.  Rows of keys, values and
 queries are tokens; offsets [sequences + 1] int32 says which rows are whose (None: one row a sequence).  Everything is
@@ -13,7 +17,7 @@ asks for one is refused.
 """
 import ctypes as C
 import struct
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -49,7 +53,7 @@ def _check_rows(t: Tensor, name: str, dim: int) -> int:
     assert t.dim() == 3 and t.shape[2] == dim, f"{name} must be [rows, heads, {dim}]"
     assert t.stride(2) == 1, f"the last dimension of {name} must be contiguous"
     assert t.dtype in nv.TYPES, f"{name} must be bfloat16, float16 or float32"
-    assert not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient, and there is none through a cache in 4 bits: call under no_grad"
+    assert not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient, and there is none through a cache in few bits: call under no_grad"
     return nv.TYPES[t.dtype]
 
 
@@ -122,7 +126,90 @@ class KVCache:
         return out
 
 
-def _queries(queries: Tensor, cache: KVCache, scale: Optional[float], causal: bool, out: Optional[Tensor],
+class KVCache8:
+    """Keys and values of 8 bits in pages of 64 tokens, with a power of two for each page and head, over tensors of the caller's (their
+    shapes are those of KVCache8.empty).  weights and positions are there for a cache that tokens are evicted from, or None.  Tokens
+    of a sequence differ from head to head once some have left; positions says which they are."""
+
+    def __init__(self, keys: Tensor, values: Tensor, scales: Tensor, weights: Optional[Tensor] = None, positions: Optional[Tensor] = None):
+        assert keys.dim() == 4 and keys.size(2) == PAGE, "keys must be uint8 [pages, heads, 64, dim]"
+        (pages, heads, _, dim) = keys.size()
+        assert dim in DIMS, f"dim must be one of {DIMS}, got {dim}"
+        assert (weights is None) == (positions is None), "weights and positions are there together or not at all"
+        for (t, name, dtype, shape) in ((keys, "keys", torch.uint8, (pages, heads, PAGE, dim)),
+                                        (values, "values", torch.uint8, (pages, heads, PAGE // 4, dim, 4)),
+                                        (scales, "scales", torch.uint8, (pages, heads, 4)),
+                                        (weights, "weights", torch.float32, (pages, heads, PAGE)),
+                                        (positions, "positions", torch.int32, (pages, heads, PAGE))):
+            if t is None:
+                continue
+            assert t.dtype == dtype and tuple(t.shape) == shape, f"{name} must be {dtype} {shape}"
+            assert t.is_contiguous(), f"{name} must be contiguous"
+            assert not t.requires_grad, f"{name} requires a gradient, and the cache is written in place"
+        self.gpu = nv.require_one_gpu(keys, values, scales, weights, positions)
+        (self.keys, self.values, self.scales, self.weights, self.positions) = (keys, values, scales, weights, positions)
+        (self.pages, self.heads, self.dim) = (pages, heads, dim)
+        self._native = nv.Cache8(pages, heads, dim, *(0 if t is None else t.data_ptr() for t in (keys, values, scales, weights, positions)))
+        self._ref = C.byref(self._native)
+
+    @classmethod
+    def empty(cls, pages: int, heads: int, dim: int, device="cuda", weighted: bool = False) -> "KVCache8":
+        """A cache of `pages` pages; 2 dim bytes a token and head, 8 more if weighted, and 4 a page and head."""
+        assert dim in DIMS, f"dim must be one of {DIMS}, got {dim}"
+
+        def part(*shape, dtype=torch.uint8):
+            return torch.empty((pages, heads, *shape), dtype=dtype, device=device)
+
+        return cls(part(PAGE, dim), part(PAGE // 4, dim, 4), part(4), part(PAGE, dtype=torch.float32) if weighted else None,
+                   part(PAGE, dtype=torch.int32) if weighted else None)
+
+    def write(self, keys: Tensor, values: Tensor, table: Tensor, starts: Tensor, offsets: Optional[Tensor] = None,
+              positions: Optional[Tensor] = None):
+        """Round keys and values [rows, heads, dim] behind the `starts` [sequences] tokens that the sequences hold.  A page's power of
+        two grows with its largest element, and what it holds is rounded to it again.  In a weighted cache the new tokens have weight 0
+        and stand at positions [rows] of their texts (None: where they are written; say so once a sequence has had tokens evicted)."""
+        kind = _check_rows(keys, "keys", self.dim)
+        assert _check_rows(values, "values", self.dim) == kind and values.shape == keys.shape, "keys and values differ in type or size"
+        assert keys.shape[1] == self.heads, f"keys have {keys.shape[1]} heads, the cache {self.heads}"
+        at = 0
+        if positions is not None:
+            assert self.positions is not None, "the cache keeps no positions: weighted=True"
+            assert positions.dtype == torch.int32 and positions.shape == keys.shape[:1] and positions.is_contiguous(), \
+                f"positions must be a contiguous int32 tensor of {keys.shape[0]}"
+            at = positions.data_ptr()
+        tokens = _tokens(keys.shape[0], table, starts, offsets)
+        gpu = nv.require_one_gpu(keys, values, table, starts, offsets, positions)
+        nv.check(nv.lib().vl_cache8_write(self._ref, tokens, kind, keys.data_ptr(), keys.stride(0), keys.stride(1),
+                                          values.data_ptr(), values.stride(0), values.stride(1), at, nv.stream_on(gpu, self.gpu)))
+
+    def read(self, table: Tensor, starts: Tensor, rows: int, offsets: Optional[Tensor] = None,
+             dtype: torch.dtype = torch.bfloat16) -> Tuple[Tensor, Tensor]:
+        """KVCache.read of this cache."""
+        assert dtype in nv.TYPES, "dtype must be bfloat16, float16 or float32"
+        tokens = _tokens(rows, table, starts, offsets)
+        gpu = nv.require_one_gpu(table, starts, offsets)
+        keys = torch.empty((rows, self.heads, self.dim), dtype=dtype, device=self.keys.device)
+        values = torch.empty_like(keys)
+        nv.check(nv.lib().vl_cache8_read(self._ref, tokens, nv.TYPES[dtype], keys.data_ptr(), values.data_ptr(), nv.stream_on(gpu, self.gpu)))
+        return (keys, values)
+
+    def evict(self, table: Tensor, lengths: Tensor, keep: int, recent: int = 0) -> Tensor:
+        """Cut sequences of more than `keep` tokens down to that many, in each head those that count most: the `recent` latest positions,
+        then the largest weights, of equal ones the earlier.  Tokens that stay move into the places of those that leave, so that a
+        sequence's first places hold them, in no order that attention would depend on.  The lengths [sequences] that are left."""
+        assert self.weights is not None, "the cache keeps no weights: weighted=True"
+        assert 0 <= recent <= keep < 1 << 31, f"recent: {recent} of {keep} that stay"
+        tokens = _tokens(table.shape[0], table, lengths, None)
+        gpu = nv.require_one_gpu(table, lengths)
+        left = torch.empty_like(lengths)
+        lib = nv.lib()
+        need = lib.vl_cache8_evict_workspace_bytes(self._ref, tokens, keep)
+        ws = _workspace(need, table)
+        nv.check(lib.vl_cache8_evict(self._ref, tokens, keep, recent, left.data_ptr(), nv.ptr(ws), need, nv.stream_on(gpu, self.gpu)))
+        return left
+
+
+def _queries(queries: Tensor, cache: Union[KVCache, KVCache8], scale: Optional[float], causal: bool, out: Optional[Tensor],
              lse: Optional[Tensor], form: Optional[str] = None) -> bytes:
     (row, head, _) = queries.stride()
     return _QUERIES.pack(queries.shape[1], row, head, queries.data_ptr(), 0 if out is None else out.data_ptr(),
@@ -130,24 +217,30 @@ def _queries(queries: Tensor, cache: KVCache, scale: Optional[float], causal: bo
                          nv.TYPES[queries.dtype], causal, 0 if form is None else nv.ATTEND_FORMS[form])
 
 
-def _check_queries(queries: Tensor, cache: KVCache):
+def _check_queries(queries: Tensor, cache: Union[KVCache, KVCache8]):
     _check_rows(queries, "queries", cache.dim)
     heads = queries.shape[1]
     assert heads > 0 and heads % cache.heads == 0, f"{heads} heads of queries for {cache.heads} of the cache"
+
+
+def _require_bounds(cache: KVCache):
+    assert not isinstance(cache, KVCache8), "blocks are chosen by bounds, and a cache in 8 bits has none"
 
 
 def _workspace(need: int, beside: Tensor) -> Optional[Tensor]:
     return beside.new_empty(nv.check(need), dtype=torch.uint8) if need else None
 
 
-def attend(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, offsets: Optional[Tensor] = None,
-           scale: Optional[float] = None, causal: bool = True, return_lse: bool = False, form: Optional[str] = None):
+def attend(queries: Tensor, cache: Union[KVCache, KVCache8], table: Tensor, lengths: Tensor, offsets: Optional[Tensor] = None,
+           scale: Optional[float] = None, causal: bool = True, return_lse: bool = False, form: Optional[str] = None,
+           accumulate: bool = False):
     """softmax(scale * queries keys^T) values over the `lengths` [sequences] tokens that the cache holds.  queries [rows, heads,
     dim], heads a multiple of the cache's; scale defaults to dim ** -0.5.  The rows of a sequence are its last tokens and see
     what stands before them and themselves, or with causal=False everything.  A row that sees nothing gives zeros.  With
     return_lse also the logarithms of the sums of exponentials [rows, heads], by which parts of an attention are joined.
     form: the library chooses one by the sizes; "few" or "many" ask for it, for tests and measurements.  Of bfloat16 "many" rounds the
-    weights to bfloat16 as well, "few" holds 16 bits of them."""
+    weights to bfloat16 as well, "few" holds 16 bits of them.  accumulate, for a weighted KVCache8 whose pages no two of the sequences
+    share: the softmax weights that a token gets from all rows and the queries that share its head are added to its weight."""
     assert form is None or form in nv.ATTEND_FORMS, f"unknown form {form!r}: expected one of {sorted(nv.ATTEND_FORMS)}"
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
@@ -156,6 +249,13 @@ def attend(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, offs
     lse = queries.new_empty(queries.shape[:2], dtype=torch.float32) if return_lse else None
     q = _queries(queries, cache, scale, causal, out, lse, form)
     lib = nv.lib()
+    if isinstance(cache, KVCache8):
+        assert not accumulate or cache.weights is not None, "the cache keeps no weights: weighted=True"
+        need = lib.vl_attend8_workspace_bytes(cache._ref, tokens, q, accumulate)
+        ws = _workspace(need, queries)
+        nv.check(lib.vl_attend8(cache._ref, tokens, q, accumulate, nv.ptr(ws), need, nv.stream_on(gpu, cache.gpu)))
+        return (out, lse) if return_lse else out
+    assert not accumulate, "a cache in 4 bits keeps no weights"
     need = lib.vl_attend_workspace_bytes(cache._ref, tokens, q)
     ws = _workspace(need, queries)
     nv.check(lib.vl_attend(cache._ref, tokens, q, nv.ptr(ws), need, nv.stream_on(gpu, cache.gpu)))
@@ -166,6 +266,7 @@ def select_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tenso
                   offsets: Optional[Tensor] = None) -> Tensor:
     """For every row and head of the cache `count` blocks of its sequence, ascending: the row's own and those with the highest
     bound on a score in them, of queries rounded to 8 bits and keys' bounds of 8 bits; MAXINT where there are no more.  [rows, cache.heads, count]"""
+    _require_bounds(cache)
     assert count >= 1, f"count: {count}"
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
@@ -182,6 +283,7 @@ def select_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tenso
 def attend_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, blocks: Tensor,
                   offsets: Optional[Tensor] = None, scale: Optional[float] = None, return_lse: bool = False):
     """attend over the tokens of blocks [rows, cache.heads, count] alone, up to the row's own place."""
+    _require_bounds(cache)
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
     assert blocks.dtype == torch.int32 and blocks.is_contiguous(), "blocks must be contiguous int32"
@@ -202,6 +304,7 @@ def attend_blocks(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tenso
 def attend_selected(queries: Tensor, cache: KVCache, table: Tensor, lengths: Tensor, count: int,
                     offsets: Optional[Tensor] = None, scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
     """(attend_blocks(...), blocks) with the blocks of select_blocks (of the negated queries where scale is negative), in one call."""
+    _require_bounds(cache)
     assert count >= 1, f"count: {count}"
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
