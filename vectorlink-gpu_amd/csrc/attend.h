@@ -6,6 +6,7 @@
 // S = scale <query, key>, P = softmax of S over the tokens that a row sees, out = P values.
 struct AttendArgs {
     CacheView c;
+    int bits;               // 4 or 8
     Tokens t;
     const void *queries;
     int64_t q_row, q_head;  // strides in elements
@@ -21,7 +22,7 @@ struct AttendArgs {
     int waves;              // of attend_few_kernel: wavefronts of a workgroup that share a tile, 4 or 8; 1: four have one each
     // of a cache in 8 bits whose tokens' weights are added up
     float *ends;            // [rows, heads_q, 2] or null: the maximum of a row's scores and the sum of its weights
-    float *scores;          // [rows, heads_q, t.blocks * 64] or null: the scores of single tokens, unscaled
+    float *scores;          // [rows, c.heads, t.blocks, group, 64] or null: the scores of single tokens, unscaled
     float *part;            // splits > 1: [rows * heads_q, splits, D] sums, then [rows * heads_q, splits, 2] maxima and sums of weights
 };
 constexpr int kMaxSplits = 64;

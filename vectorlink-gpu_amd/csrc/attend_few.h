@@ -21,6 +21,7 @@
 // result's own rounding.
 #pragma once
 #include "attend.h"
+#include "weigh_scores.h"
 
 template <int D, int BITS = 4>
 struct Parts {  // D = parts of 128, then 64, then 32
@@ -45,7 +46,7 @@ struct PageRegs {
     u32x4 vs[P];          // scales of tokens c * 16 + 4 m + byte
 };
 
-template <int D>
+template <int D, int USE>
 __device__ inline void load_page(PageRegs<D> &g, const CacheView &c, int64_t page, int h) {
     typedef Parts<D> PT;
     const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
@@ -90,29 +91,50 @@ struct PageRegs<D, 8> {
     u32x4 v[P][4];          // [part][4 tokens m], a word a dimension: 4 r + j, or 2 r + j
     float key_scale, value_scale;
 };
-template <int D>
-__device__ inline void load_page(PageRegs<D, 8> &g, const CacheView &c, int64_t page, int h) {
+// What a call over a cache in 8 bits uses a page for.  One that a single wavefront reads - a token's queries are one tile - is asked for
+// without leaving a place in the caches to it: 4 tokens over 131,072 186 us with a place and 165 (6.5 TB/s) without, 64 over 4,096 to
+// 8,192 149 and 145.  Where several tiles share the pages the caches are what they share them by: 16 sequences of 5 tokens over 8,000
+// to 16,384 184 us with and 228 without.
+enum PageUse { kShared, kOnce, kOnceAndScores };
+template <int USE, class T>
+__device__ inline T load_of_page(const uint8_t *at) {
+    if constexpr (USE == kShared) return *reinterpret_cast<const T *>(at);
+    else return __builtin_nontemporal_load(reinterpret_cast<const T *>(at));
+}
+template <int USE>
+__device__ inline void load_codes(u32x4 &to, const uint8_t *at, int width) {  // of 64 dimensions, or 32
+    if (width == 64) {
+        to = load_of_page<USE, u32x4>(at);
+    } else {
+        const u32x2 x = load_of_page<USE, u32x2>(at);
+        to[0] = x[0], to[1] = x[1];
+    }
+}
+template <int D, int USE>
+__device__ inline void load_page_keys(PageRegs<D, 8> &g, const CacheView &c, int64_t page, int h) {
     typedef Parts<D, 8> PT;
     const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
-    const int64_t unit = page * c.heads + h;
-    const uint8_t *const kc = c.keys + unit * (kPage * D), *const vc = c.values + unit * (kPage * D);
+    const uint8_t *const kc = c.keys + (page * c.heads + h) * (kPage * D);
     const int token = (r >> 2) * 16 + (r & 3);
-    auto load = [](u32x4 &to, const uint8_t *at, int width) {
-        if (width == 64) {
-            to = *reinterpret_cast<const u32x4 *>(at);
-        } else {
-            const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
-            to[0] = x[0], to[1] = x[1];
-        }
-    };
 #pragma unroll
     for (int m = 0; m < 4; m++)
 #pragma unroll
-        for (int p = 0; p < PT::kCount; p++) load(g.k[p][m], kc + (token + m * 4) * D + PT::base(p) + q * (PT::width(p) / 4), PT::width(p));
+        for (int p = 0; p < PT::kCount; p++) load_codes<USE>(g.k[p][m], kc + (token + m * 4) * D + PT::base(p) + q * (PT::width(p) / 4), PT::width(p));
+}
+template <int D, int USE>
+__device__ inline void load_page_values(PageRegs<D, 8> &g, const CacheView &c, int64_t page, int h) {
+    typedef Parts<D, 8> PT;
+    const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
+    const uint8_t *const vc = c.values + (page * c.heads + h) * (kPage * D);
 #pragma unroll
     for (int m = 0; m < 4; m++)
 #pragma unroll
-        for (int p = 0; p < PT::kCount; p++) load(g.v[p][m], vc + ((q * 4 + m) * D + PT::base(p) + r * (PT::width(p) / 16)) * 4, PT::width(p));
+        for (int p = 0; p < PT::kCount; p++) load_codes<USE>(g.v[p][m], vc + ((q * 4 + m) * D + PT::base(p) + r * (PT::width(p) / 16)) * 4, PT::width(p));
+}
+template <int D, int USE>
+__device__ inline void load_page(PageRegs<D, 8> &g, const CacheView &c, int64_t page, int h) {
+    load_page_keys<D, USE>(g, c, page, h);
+    load_page_values<D, USE>(g, c, page, h);
 }
 
 // NS bfloat16 values that add up to x (to 8 NS bits of it): the first NS - 1 cut off, so that what is left is exact.
@@ -231,10 +253,19 @@ __device__ inline float over_copies(float x, F f) {
 
 // A page's 64 tokens: this lane's row (r % C) sees the first `sees` of them, `written` hold something; edge: some row does not see
 // some token, or some token may not be finite.  Spoilt tokens (scale 255) turn the rows that see them into NaN, and no others.
-// to: where this lane's row of scores goes, from the page's first token on, or null.
-template <int D, int NS, int C, int BITS>
+// Where the scores of single tokens go: a buffer of its own for a token and head, the byte of it that this lane's row of the page has -
+// of a lane without a row past its end, where a store is dropped.  A branch around the store would leave the compiler to guess
+// how many stores are on their way, and loads would wait for them.
+struct ScoresAt {
+    __amdgpu_buffer_rsrc_t buffer;
+    int lane, page;
+};
+
+// put: where scores go, of a call that keeps them.  between(): what is done once the keys have been
+// used and before the values are.
+template <int D, int NS, int C, int BITS, int USE, class F>
 __device__ inline void take_page(RowState<D> &st, PageRegs<D, BITS> &g, const QueryRegs<D, NS> &f, float scale, bool edge, int sees,
-                                 int written, float *to) {
+                                 int written, const ScoresAt &put, F between) {
     typedef Parts<D, BITS> PT;
     constexpr int NW = NS < 2 ? 2 : NS;  // parts of a weight
     constexpr int M = C / 4;             // tiles of 4 tokens of this lane
@@ -274,6 +305,7 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D, BITS> &g, const Qu
 #pragma unroll
         for (int m = 0; m < 4; m++) s[m] += small[m];
     }
+    between();
     float t[M][4];
     spread_scores<C>(s, t);
     if (edge) {
@@ -320,11 +352,10 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D, BITS> &g, const Qu
             }
         }
     }
-    if constexpr (BITS == 8) {
-        if (to) {
+    if constexpr (USE == kOnceAndScores) {
 #pragma unroll
-            for (int k = 0; k < M; k++) *reinterpret_cast<f32x4 *>(to + q * 16 + (M * (r / C) + k) * 4) = f32x4{t[k][0], t[k][1], t[k][2], t[k][3]};
-        }
+        for (int k = 0; k < M; k++)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{t[k][0], t[k][1], t[k][2], t[k][3]}), put.buffer, put.lane + k * 16, put.page, 0);
     }
     float top = t[0][0];
 #pragma unroll
@@ -382,42 +413,42 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D, BITS> &g, const Qu
                 continue;
             }
             if constexpr (BITS == 4) {
-            uint32_t word[8];
-            float vs[8];
+                uint32_t word[8];
+                float vs[8];
 #pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const int m = 2 * h + (u >> 2);
-                word[u] = g.v[p][m][u & 3];
-                if (W == 64) word[u] >>= 16 * (r & 1);
-                if (W == 32) word[u] >>= 8 * (r & 3);
-                vs[u] = scale_at(g.vs[p][m], u & 3);
-            }
-            // byte B of the words: dimensions of tiles 2 B and 2 B + 1
-            auto two_tiles = [&](auto byte, u32x4(&a)[2]) {
-                constexpr int B = decltype(byte)::value;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t x = two_values<B>(word[2 * i], vs[2 * i]), y = two_values<B>(word[2 * i + 1], vs[2 * i + 1]);
-                    a[0][i] = __builtin_amdgcn_perm(y, x, 0x05040100);
-                    a[1][i] = __builtin_amdgcn_perm(y, x, 0x07060302);
+                for (int u = 0; u < 8; u++) {
+                    const int m = 2 * h + (u >> 2);
+                    word[u] = g.v[p][m][u & 3];
+                    if (W == 64) word[u] >>= 16 * (r & 1);
+                    if (W == 32) word[u] >>= 8 * (r & 3);
+                    vs[u] = scale_at(g.vs[p][m], u & 3);
                 }
-            };
-            auto products = [&](int tile, const u32x4(&a)[2][2], int tiles) {
+                // byte B of the words: dimensions of tiles 2 B and 2 B + 1
+                auto two_tiles = [&](auto byte, u32x4(&a)[2]) {
+                    constexpr int B = decltype(byte)::value;
 #pragma unroll
-                for (int n = 0; n < NW; n++)
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t x = two_values<B>(word[2 * i], vs[2 * i]), y = two_values<B>(word[2 * i + 1], vs[2 * i + 1]);
+                        a[0][i] = __builtin_amdgcn_perm(y, x, 0x05040100);
+                        a[1][i] = __builtin_amdgcn_perm(y, x, 0x07060302);
+                    }
+                };
+                auto products = [&](int tile, const u32x4(&a)[2][2], int tiles) {
 #pragma unroll
-                    for (int k = 0; k < tiles; k++)
-                        st.acc[tile + k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[k >> 1][k & 1]), w[n], st.acc[tile + k], 0, 0, 0);
-            };
-            u32x4 a[2][2];
-            two_tiles(std::integral_constant<int, 0>(), a[0]);
-            if (W >= 64) two_tiles(std::integral_constant<int, 1>(), a[1]);
-            products(t0, a, W >= 64 ? 4 : 2);
-            if (W >= 128) {
-                two_tiles(std::integral_constant<int, 2>(), a[0]);
-                two_tiles(std::integral_constant<int, 3>(), a[1]);
-                products(t0 + 4, a, 4);
-            }
+                    for (int n = 0; n < NW; n++)
+#pragma unroll
+                        for (int k = 0; k < tiles; k++)
+                            st.acc[tile + k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[k >> 1][k & 1]), w[n], st.acc[tile + k], 0, 0, 0);
+                };
+                u32x4 a[2][2];
+                two_tiles(std::integral_constant<int, 0>(), a[0]);
+                if (W >= 64) two_tiles(std::integral_constant<int, 1>(), a[1]);
+                products(t0, a, W >= 64 ? 4 : 2);
+                if (W >= 128) {
+                    two_tiles(std::integral_constant<int, 2>(), a[0]);
+                    two_tiles(std::integral_constant<int, 3>(), a[1]);
+                    products(t0 + 4, a, 4);
+                }
             }
         }
     }
@@ -436,9 +467,9 @@ struct Blocks {
 // tokens over 4,096 to 8,192 and 8 heads; 128: 94 and 92; 96, and 128 of float32, spill); behind the last one the same page is loaded once more instead
 // of a branch, over which the compiler would have to wait for all loads.  The queries' loads are waited for with the first
 // page's.
-template <int D, int NS, int C, int BITS = 4>
+template <int D, int NS, int C, int BITS = 4, int USE = kShared>
 __device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const QueryLoads<D, NS> &queries, bool real, Blocks l, int b,
-                                   int h, int sees, int least, int most, int length, float *scores = nullptr) {
+                                   int h, int sees, int least, int most, int length, ScoresAt scores = {}) {
     const int lane = threadIdx.x & 63;
     QueryRegs<D, NS> f;
     bool first = true;
@@ -463,42 +494,55 @@ __device__ inline void take_blocks(RowState<D> &st, const AttendArgs &a, const Q
                 at = __builtin_ctzll(left);
                 left &= left - 1;
             }
-            load_page<D>(g, a.c, __builtin_amdgcn_readlane(page, at), h);
+            load_page<D, USE>(g, a.c, __builtin_amdgcn_readlane(page, at), h);
         };
-        auto take = [&](PageRegs<D, BITS> &g, int at) {
+        auto take = [&](PageRegs<D, BITS> &g, int at, auto between) {
             const int first = __builtin_amdgcn_readlane(block, at) * kPage;
             if constexpr (BITS == 8) {
                 const uint32_t word = __builtin_amdgcn_readlane(scales, at);
                 g.key_scale = scale_of_keys(word);
                 g.value_scale = scale_of_values(word);
             }
-            take_page<D, NS, C, BITS>(st, g, f, a.scale, edges >> at & 1, sees - first, length - first, scores ? scores + first : nullptr);
+            if constexpr (USE == kOnceAndScores) scores.page = first * a.group * 4;
+            take_page<D, NS, C, BITS, USE>(st, g, f, a.scale, edges >> at & 1, sees - first, length - first, scores, between);
         };
         auto look = [&] {  // after the first page's loads
             edges = __ballot(page >= 0 && ((block + 1) * kPage > least || (BITS == 4 ? bound == kBoundless : is_marked(scales))));
             if (first) take_queries<D, NS>(f, queries, real, a.turn);
             first = false;
         };
+        auto nothing = [] {};
         PageRegs<D, BITS> x;
         next(x);
         look();
-        if constexpr (BITS == 4 ? D == 64 || (D == 128 && NS < 3) : D <= 64) {
+        if constexpr (BITS == 8 && D > 64) {
+            // one page's registers: the next page's keys are asked for once this one's have been used, its values likewise
+            while (left) {
+                const int here = at;
+                at = __builtin_ctzll(left);
+                left &= left - 1;
+                const int64_t ahead = __builtin_amdgcn_readlane(page, at);
+                take(x, here, [&] { load_page_keys<D, USE>(x, a.c, ahead, h); });
+                load_page_values<D, USE>(x, a.c, ahead, h);
+            }
+            take(x, at, nothing);
+        } else if constexpr (BITS == 8 || D == 64 || (D == 128 && NS < 3)) {
             PageRegs<D, BITS> y;
             for (;;) {
                 int here = at;
                 bool last = !left;
                 next(y);
-                take(x, here);
+                take(x, here, nothing);
                 if (last) break;
                 here = at;
                 last = !left;
                 next(x);
-                take(y, here);
+                take(y, here, nothing);
                 if (last) break;
             }
         } else {
             for (;;) {
-                take(x, at);
+                take(x, at, nothing);
                 if (!left) break;
                 next(x);
             }
@@ -595,12 +639,18 @@ __device__ inline void join_waves(const RowState<D> &st, JoinLds<WAVES> &s, cons
         }
     }
     if (js == 0 && to >= 0) put_sums(a, to, split, D, top, total);
+    if constexpr (BITS == 8) {  // for those who come after: what the rows end with
+        if (js == 0 && threadIdx.x < 256) {
+            s.top[0][jr] = top;
+            s.all[0][jr] = total;
+        }
+    }
 }
 
 // A tile is 16 rows of one head: of the queries of one token where there is a list, of all tokens of a sequence otherwise.
 // The WAVES wavefronts of a workgroup share a tile's blocks and are joined; 1: each of four has a tile of its own.  C: the most
 // rows that a tile has, 16 unless its rows are one token's, which see the same.
-template <int D, int NS, int WAVES, int C, int BITS = 4>
+template <int D, int NS, int WAVES, int C, int BITS = 4, int USE = kShared>
 __global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 : 1) void attend_few_kernel(AttendArgs a, int tiles) {
     typedef Parts<D, BITS> PT;
     constexpr bool JOIN = WAVES > 1;
@@ -647,11 +697,13 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 
     const int entries = a.list ? a.count : (most + kPage - 1) / kPage;
     const int from = (int)((int64_t)entries * split / a.splits), to = (int)((int64_t)entries * (split + 1) / a.splits);
     const int32_t *const list = a.list ? a.list + ((row0 + (int64_t)token0) * a.c.heads + h) * a.count : nullptr;
-    float *scores = nullptr;
-    if constexpr (BITS == 8) {  // of one token's queries, all in one tile
-        if (a.scores && r % C < a.group) scores = a.scores + ((row0 + (int64_t)token0) * a.heads_q + h * a.group + r % C) * ((int64_t)a.t.blocks * kPage);
+    ScoresAt scores = {};
+    if constexpr (USE == kOnceAndScores) {  // of one token's queries, all in one tile
+        const int64_t wide = (int64_t)a.t.blocks * a.group * kPage * 4;  // bytes of a token and head
+        scores.buffer = __builtin_amdgcn_make_buffer_rsrc((char *)a.scores + ((int64_t)row0 * a.c.heads + h) * wide, 0, (int)wide, 0x00020000);
+        scores.lane = r % C < a.group ? (r % C * kPage + q * 16 + C / 4 * (r / C) * 4) * 4 : INT32_MIN;
     }
-    take_blocks<D, NS, C, BITS>(st, a, f, real, {list, JOIN ? from + wave : from, WAVES, to}, b, h, C < 16 ? most : sees, least, most, length, scores);
+    take_blocks<D, NS, C, BITS, USE>(st, a, f, real, {list, JOIN ? from + wave : from, WAVES, to}, b, h, C < 16 ? most : sees, least, most, length, scores);
 
     auto out_row = [&](int r) {
         const int i = w.piece * 16 + r;
@@ -659,10 +711,21 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 
     };
     if constexpr (JOIN) {
         extern __shared__ __attribute__((aligned(16))) char lds[];  // a JoinLds<WAVES>
-        join_waves<D, NS, WAVES, C, BITS>(st, *reinterpret_cast<JoinLds<WAVES> *>(lds), a, split, out_row);
+        JoinLds<WAVES> &s = *reinterpret_cast<JoinLds<WAVES> *>(lds);
+        join_waves<D, NS, WAVES, C, BITS>(st, s, a, split, out_row);
+        if constexpr (USE == kOnceAndScores) {
+            if (a.splits > 1) return;
+            __syncthreads();
+            weigh_places<C, 1024>(a, b, h, threadIdx.x * 4, length, [&](int g) { return row_ends(s.top[0][g], s.all[0][g]); });
+        }
     } else {
         const float total = sum_of_row<C>(st.sum);
         const int64_t to = out_row(r);
+        if constexpr (USE == kOnceAndScores)
+            weigh_places<C, 256>(a, b, h, lane * 4, length, [&](int g) {
+                const int top = __builtin_amdgcn_readlane(__builtin_bit_cast(int, st.top), g), all = __builtin_amdgcn_readlane(__builtin_bit_cast(int, total), g);
+                return row_ends(__builtin_bit_cast(float, top), __builtin_bit_cast(float, all));
+            });
         if (to < 0) return;
 #pragma unroll
         for (int p = 0; p < PT::kCount; p++) {

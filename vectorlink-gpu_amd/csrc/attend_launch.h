@@ -26,16 +26,24 @@ int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream) {
         const unsigned groups = (unsigned)(tiles * a.splits), heads = (unsigned)a.c.heads;
         for_rows(a.list || !a.t.offsets ? a.group : 16, [&](auto c) {
             constexpr int C = decltype(c)::value;
-            if (a.waves == 1) {
-                attend_few_kernel<D, NS, 1, C, BITS><<<dim3((unsigned)((tiles + 3) / 4), heads), 256, 0, stream>>>(a, (int)tiles);
-            } else if (a.waves == 8) {
-                if constexpr (D <= 128) {
-                    e = vl_allow_lds(attend_few_kernel<D, NS, 8, C, BITS>, sizeof(JoinLds<8>));
-                    if (e == hipSuccess) attend_few_kernel<D, NS, 8, C, BITS><<<dim3(groups, heads), 512, sizeof(JoinLds<8>), stream>>>(a, (int)tiles);
+            auto launch = [&](auto use) {
+                constexpr int S = decltype(use)::value;
+                if (a.waves == 1) {
+                    attend_few_kernel<D, NS, 1, C, BITS, S><<<dim3((unsigned)((tiles + 3) / 4), heads), 256, 0, stream>>>(a, (int)tiles);
+                } else if (a.waves == 8) {
+                    if constexpr (BITS == 4 && D <= 128) {
+                        e = vl_allow_lds(attend_few_kernel<D, NS, 8, C, BITS, S>, sizeof(JoinLds<8>));
+                        if (e == hipSuccess) attend_few_kernel<D, NS, 8, C, BITS, S><<<dim3(groups, heads), 512, sizeof(JoinLds<8>), stream>>>(a, (int)tiles);
+                    }
+                } else {
+                    attend_few_kernel<D, NS, 4, C, BITS, S><<<dim3(groups, heads), 256, sizeof(JoinLds<4>), stream>>>(a, (int)tiles);
                 }
-            } else {
-                attend_few_kernel<D, NS, 4, C, BITS><<<dim3(groups, heads), 256, sizeof(JoinLds<4>), stream>>>(a, (int)tiles);
+            };
+            if constexpr (BITS == 8) {
+                if (a.scores) return launch(std::integral_constant<int, kOnceAndScores>());
+                if (C < 16 || (!a.t.offsets && a.group <= 16)) return launch(std::integral_constant<int, kOnce>());
             }
+            if constexpr (BITS == 4 || C == 16) launch(std::integral_constant<int, kShared>());
         });
         if (e == hipSuccess) launch_join<D, NS>(a, stream);
     });

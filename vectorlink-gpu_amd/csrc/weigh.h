@@ -1,24 +1,8 @@
-// The weights that attention gave the tokens of a cache in 8 bits, added to those that it holds: w_t += sum over rows and the queries
-// that share a head of exp2(scale s_t - max) / sum, with each row's maximum and sum as attention left them.
+// The weights of weigh_scores.h from the keys once more.
 //
 // A page and head is one workgroup's (two pages of one sequence are two), so sums have one order and nothing is atomic.
 #pragma once
 #include "attend_few.h"
-
-// What a row's scores are turned into weights with: exp2(scale s - max) * by.  A row that saw nothing, or something that is not finite,
-// gives no weight to anything: exp2(s - inf) * 0, for scores that are finite.
-struct RowEnds {
-    float minus, by;
-    bool fine;
-};
-__device__ inline RowEnds row_ends(const float *ends, int64_t row) {
-    const f32x2 e = *reinterpret_cast<const f32x2 *>(ends + row * 2);
-    RowEnds r;
-    r.fine = e[0] > -INFINITY && e[0] < INFINITY && e[1] > 0 && e[1] < INFINITY;
-    r.minus = r.fine ? -e[0] : -INFINITY;
-    r.by = r.fine ? 1.0f / e[1] : 0.0f;
-    return r;
-}
 
 // Many rows, or several tokens of a sequence: the scores of a page are made once more.  A workgroup has one page of one head; its
 // wavefronts hold the page's keys in registers as bfloat16 (32 tokens a tile, two tiles) and take every fourth tile of 32 rows.
@@ -65,7 +49,8 @@ __global__ __launch_bounds__(256) void weigh_rows_kernel(AttendArgs a, int64_t u
             const int token = (int)(index / a.group), head = h * a.group + (int)(index % a.group);
             const bool real = index < rows;
             const int64_t row = row0 + (int64_t)token;
-            RowEnds ends = row_ends(a.ends, real ? row * a.heads_q + head : 0);
+            f32x2 top_and_total = *reinterpret_cast<const f32x2 *>(a.ends + (real ? row * a.heads_q + head : 0) * 2);
+            const RowEnds ends = row_ends(top_and_total[0], top_and_total[1]);
             const int sees = !real || !ends.fine ? 0 : a.causal ? min(max(place0 + token + 1, 0), length) : length;
             const E *const at = (const E *)a.queries + (real ? row * a.q_row + head * a.q_head : 0) + hi * 16;
             f32x16 s[2], small[2];
