@@ -80,7 +80,9 @@ def test_workspaces_are_checked(lib):
     assert lib.vl_cache8_evict(cache(), t, 64, 0, 256, 264, need, None) == -1
     # an eviction's lists are bounded by what stays and by half of what there is
     (one, all_) = (lib.vl_cache8_evict_workspace_bytes(cache(), t, keep) for keep in (1, (1 << 31) - 1))
-    assert one < need < all_ < 3 * 2 * (2 * 40_000 * 64 // 2 * 4 + 40_002 * 4 + 2048)
+    # two lists of 8 bytes an entry, the first hole of every block, and what workgroups that share a sequence and head tell each other
+    (entries, chunks) = (40_000 * 64 // 2, -(-40_000 // 128))
+    assert one < need < all_ < 3 * 2 * (2 * entries * 8 + 40_002 * 4 + chunks * (8 + 16 * 16) + 3 * 2048 * 4 + 2048)
 
 
 def test_calls_without_rows_succeed(lib):
