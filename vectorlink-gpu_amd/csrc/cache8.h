@@ -37,6 +37,19 @@ __device__ inline bf16x8 eight_of_bytes(uint32_t x, uint32_t y, float scale) {
     u32x4 v = {two_of_bytes<false>(x, scale), two_of_bytes<true>(x, scale), two_of_bytes<false>(y, scale), two_of_bytes<true>(y, scale)};
     return __builtin_bit_cast(bf16x8, v);
 }
+// the same as half precision, without the power: every code is exact there
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+template <bool UPPER>
+__device__ inline uint32_t two_halves(uint32_t word) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.0f, UPPER));
+}
+__device__ inline f16x8 eight_halves(uint32_t x, uint32_t y) {
+    u32x4 v = {two_halves<false>(x), two_halves<true>(x), two_halves<false>(y), two_halves<true>(y)};
+    return __builtin_bit_cast(f16x8, v);
+}
+// What scores of such keys are multiplied with: the call's scale and the keys' power, kept a normal number - 0 or infinite it would make
+// NaN of scores that are infinite or 0, where the true product is next to nothing or beyond everything all the same.
+__device__ inline float scale_with(float scale, float power) { return __builtin_amdgcn_fmed3f(scale * power, 0x1p-126f, 0x1.fffffep127f); }
 // the four codes of a word as numbers, and the way back: to the nearest code, of two as near the even one; magnitudes up to 448
 __device__ inline f32x4 four_numbers(uint32_t word) {
     const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
