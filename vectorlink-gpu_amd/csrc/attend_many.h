@@ -163,13 +163,14 @@ __device__ inline void fetch_keys(KeyPart<D, 8> &g, const CacheView &c, int64_t 
         }
     }
 }
-template <int D>
+template <int D, bool HALF>
 __device__ inline void store_keys(const KeyPart<D, 8> &g, char *lds, int id, float scale) {
     typedef Images<D> I;
     const int token = (id >> 6) * 16 + (id & 15), q = id >> 4 & 3;
 #pragma unroll
     for (int i = 0; i < D / 32; i++)
-        *reinterpret_cast<bf16x8 *>(lds + I::key(token, q * (D / 32) + i)) = eight_of_bytes(g.w[2 * i], g.w[2 * i + 1], scale);
+        if constexpr (HALF) *reinterpret_cast<f16x8 *>(lds + I::key(token, q * (D / 32) + i)) = eight_halves(g.w[2 * i], g.w[2 * i + 1]);
+        else *reinterpret_cast<bf16x8 *>(lds + I::key(token, q * (D / 32) + i)) = eight_of_bytes(g.w[2 * i], g.w[2 * i + 1], scale);
 }
 template <int D>
 __device__ inline void fetch_values(ValuePart<D, 8> &g, const CacheView &c, int64_t unit, int id) {
@@ -234,6 +235,12 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
     // rounding (root of the mean square, 5.00e-4 and 4.30e-4), and more where values cancel.  A second part makes half as many products
     // again and takes that away, for 661 us instead of 494; dividing by the sum of the rounded weights leaves 4.95e-4 for 506.
     constexpr int NW = NS;
+    // Half precision over a cache in 8 bits: its codes are half precision as well, so a score is one product and not two.  Keys are left
+    // without their power, which the scores are multiplied with (2,048 rows over 16,384 tokens, 32 heads on 8 of 128: 875 us with two,
+    // 703 with one; with weights and values of half precision too, where a page's fit it, 831: two ways through a page spill).
+    constexpr bool HALF = BITS == 8 && NS == 2;
+    constexpr int NQ = HALF ? 1 : NS;  // parts of a query
+    typedef typename std::conditional<HALF, f16x8, bf16x8>::type Operand;
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
     // all tiles of a head go to the same XCD where there are 8 heads; the last tiles, which see most, come first
@@ -255,7 +262,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
     const int least = a.causal ? min(max(place0 + first_token + 1, 0), length) : length;
     const int most = a.causal ? min(max(place0 + last_token + 1, 0), length) : length;
 
-    bf16x8 q[NS][D / 16];
+    Operand q[NQ][D / 16];
     {
         Eight<NS> x[D / 16];
         const E *const at = (const E *)a.queries + (real ? row * a.q_row + head * a.q_head : 0) + hi * 8;
@@ -265,10 +272,14 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
         for (int k = 0; k < D / 16; k++) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                __bf16 s[NS];
-                split_into<NS>((float)x[k][i] * a.turn, s);
+                if constexpr (HALF) {
+                    q[0][k][i] = x[k][i] * (E)a.turn;
+                } else {
+                    __bf16 s[NS];
+                    split_into<NS>((float)x[k][i] * a.turn, s);
 #pragma unroll
-                for (int n = 0; n < NS; n++) q[n][k][i] = s[n];
+                    for (int n = 0; n < NS; n++) q[n][k][i] = s[n];
+                }
             }
         }
     }
@@ -293,7 +304,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
             if (brings_keys) store_keys<D>(kp[k], to, id);
             if (brings_values) store_values<D>(vp[k], to, (uint8_t *)to + I::kBytes, id, edge, length - block * kPage);
         } else {
-            if (brings_keys) store_keys<D>(kp[k], to, id, scale_of_keys(scales));
+            if (brings_keys) store_keys<D, HALF>(kp[k], to, id, scale_of_keys(scales));
             if (brings_values) store_values<D>(vp[k], to, (uint8_t *)to + I::kBytes, id, edge, length - block * kPage, scale_of_values(scales));
         }
     };
@@ -317,7 +328,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
     };
     look_up(from);
     int page[PAGES], next[PAGES];
-    uint32_t edge = 0, next_edge = 0, next_scales[PAGES] = {};
+    uint32_t edge = 0, next_edge = 0, here_scales[PAGES] = {}, next_scales[PAGES] = {};
 #pragma unroll
     for (int k = 0; k < PAGES; k++) {
         page[k] = __builtin_amdgcn_readlane(pages, k);
@@ -325,8 +336,10 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
     }
     edge = (uint32_t)edges & ((1u << PAGES) - 1);
 #pragma unroll
-    for (int k = 0; k < PAGES; k++)
-        if (page[k] >= 0) store(k, k, from + k, edge >> k & 1, __builtin_amdgcn_readlane(scales, k));
+    for (int k = 0; k < PAGES; k++) {
+        here_scales[k] = __builtin_amdgcn_readlane(scales, k);
+        if (page[k] >= 0) store(k, k, from + k, edge >> k & 1, here_scales[k]);
+    }
     __syncthreads();
     for (int round = from, turn = 0; round < to; round += PAGES, turn ^= 1) {
         const int at = round + PAGES - from & 63;
@@ -343,6 +356,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
             if (page[k] < 0) continue;
             const int block = round + k;
             const char *const in = lds + (turn * PAGES + k) * kBuffer;
+            const float scale = HALF ? scale_with(a.scale, scale_of_keys(here_scales[k])) : a.scale;
             // of three parts of a query the second and third add to sums of their own, which rounds a score less often
             constexpr int kSums = NS == 3 ? 2 : 1;
             f32x16 sums[kSums][2];
@@ -355,15 +369,16 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
 #pragma unroll
             for (int c = 0; c < D / 16; c++) {
                 // products that add to the same sums do not follow each other: one waits for the other's result
-                bf16x8 x[2];
+                Operand x[2];
 #pragma unroll
-                for (int t = 0; t < 2; t++) x[t] = *reinterpret_cast<const bf16x8 *>(in + I::key(t * 32 + col, c * 2 + hi));
+                for (int t = 0; t < 2; t++) x[t] = *reinterpret_cast<const Operand *>(in + I::key(t * 32 + col, c * 2 + hi));
 #pragma unroll
-                for (int n = 0; n < NS; n++)
+                for (int n = 0; n < NQ; n++)
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
                         f32x16 &to = sums[n > 0 ? kSums - 1 : 0][t];
-                        to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[t], q[n][c], to, 0, 0, 0);
+                        if constexpr (HALF) to = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[t], q[n][c], to, 0, 0, 0);
+                        else to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[t], q[n][c], to, 0, 0, 0);
                     }
             }
             f32x16(&s)[2] = sums[0];
@@ -386,7 +401,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
             float most_here = s[0][0];
 #pragma unroll
             for (int i = 1; i < 32; i++) most_here = fmaxf(most_here, s[i >> 4][i & 15]);
-            most_here = max_of_halves(most_here) * a.scale;
+            most_here = max_of_halves(most_here) * scale;
             // The maximum that weights are measured from may lie up to 8 below the true one: weights up to 256 cost nothing, and
             // the sums are rescaled a few times a row instead of at every new maximum.  Each row's moves when that row passes it, so
             // that no result depends on the rows beside it.
@@ -406,7 +421,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
                 float part = 0;
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.scale, minus));
+                    s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], scale, minus));
                     part += s[t][i];
                 }
                 sum += part;
@@ -434,6 +449,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
         for (int k = 0; k < PAGES; k++) {
             if (next[k] >= 0) store(k, (turn ^ 1) * PAGES + k, round + PAGES + k, next_edge >> k & 1, next_scales[k]);
             page[k] = next[k];
+            here_scales[k] = next_scales[k];
         }
         edge = next_edge;
         __syncthreads();

@@ -37,7 +37,7 @@ __device__ inline bf16x8 eight_of_bytes(uint32_t x, uint32_t y, float scale) {
     u32x4 v = {two_of_bytes<false>(x, scale), two_of_bytes<true>(x, scale), two_of_bytes<false>(y, scale), two_of_bytes<true>(y, scale)};
     return __builtin_bit_cast(bf16x8, v);
 }
-// the same as half precision, without the power: every code is exact there
+// the same as half precision; without the power every code is exact there
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 template <bool UPPER>
 __device__ inline uint32_t two_halves(uint32_t word) {
