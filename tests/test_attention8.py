@@ -85,6 +85,13 @@ def test_workspaces_are_checked(lib):
     assert one < need < all_ < 3 * 2 * (2 * entries * 8 + 40_002 * 4 + chunks * (8 + 16 * 16) + 3 * 2048 * 4 + 2048)
 
 
+def test_scores_take_4_gib_at_most(lib):
+    """Tables of many blocks that mostly name nothing: weights are made from the keys once more."""
+    def need(blocks):
+        return lib.vl_attend8_workspace_bytes(cache(heads=8), tokens(rows=64, sequences=64, blocks=blocks, table_stride=blocks), queries(heads=32), 1)
+    assert 1 << 32 <= need(8_192) < (1 << 32) + (1 << 28) and need(8_193) < 1 << 28
+
+
 def test_calls_without_rows_succeed(lib):
     t = tokens(rows=0, sequences=0, table=None, lengths=None)
     assert lib.vl_cache8_write(cache(), t, 1, None, 0, 0, None, 0, 0, None, None) == 0

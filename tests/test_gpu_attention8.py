@@ -250,6 +250,61 @@ def test_split_over_workgroups(dtype):
     attend_and_check(cache, table, lengths, queries_for(43, 3, 64, gen, dtype), ends(counts))
 
 
+@pytest.mark.parametrize("dim, dtype, group", [(64, torch.bfloat16, 4), (128, torch.float16, 7), (96, torch.float32, 16), (192, torch.bfloat16, 1)])
+def test_many_short_sequences(dim, dtype, group):
+    """A tile of rows is one wavefront's, which adds its tokens' weights itself; of prompts four pages are a workgroup's."""
+    gen = torch.Generator().manual_seed(dim)
+    lengths = torch.randint(0, 67, (700,), generator=gen).tolist()
+    cache, table, held, gen = filled(lengths, 3, dim, dim, dtype, blocks=2)
+    table[17, 0] = -1
+    table[300:310, 1] = MAXINT
+    attend_and_check(cache, table, held, queries_for(700, 3 * group, dim, gen, dtype))
+    counts = [n % 3 for n in lengths]
+    q = queries_for(sum(counts) + 2, 6, dim, gen, dtype)
+    for form in forms_of(dim, dtype):
+        attend_and_check(cache, table, held, q, ends(counts), form=form)
+
+
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_weights_under_wide_tables(dim, dtype, causal):
+    """Tables of many blocks, most of which hold nothing: pages that are marked, that miss, that some rows see; no rows, no tokens, more
+    rows than tokens; as many rows as a step of the workgroup takes and one more."""
+    (counts, lengths) = ([70, 0, 64, 33, 9, 1, 22], [300, 50, 65, 20, 0, 129, 400])
+    cache, table, held, gen = filled(lengths, 2, dim, dim + 1, dtype)
+    (k, v) = torch.randn((2, 30, 2, dim), generator=gen, device=DEV).to(dtype)
+    k[9, 0, 3] = math.inf
+    v[20, 1, 5] = math.nan
+    cache.write(k, v, table, held - 30, whole(0, 30, 30, 30, 30, 30, 30, 30))
+    wide = torch.full((7, 160), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.size(1)] = table
+    wide[6, 2] = cache.pages
+    q = queries_for(sum(counts) + 3, 6, dim, gen, dtype)
+    q[150, 2, 7] = math.nan
+    for form in forms_of(dim, dtype):
+        attend_and_check(cache, wide, held, q, ends(counts), causal=causal, form=form)
+
+
+def test_tables_too_wide_for_scores():
+    """Single tokens whose scores would take more than 4 GiB under their table."""
+    cache, table, held, gen = filled([n % 150 for n in range(0, 64 * 7, 7)], 2, 32, 17)
+    wide = torch.full((64, 17_000), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.size(1)] = table
+    attend_and_check(cache, wide, held, queries_for(64, 16, 32, gen, torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [-0.4, 0.0, 7.0])
+def test_scales(dtype, scale):
+    """Scores that are turned round, that are all the same, and that leave one token all weight."""
+    cache, table, lengths, gen = filled([150, 64, 5], 2, 64, 21, dtype)
+    q = queries_for(60, 8, 64, gen, dtype)
+    for form in forms_of(64, dtype):
+        attend_and_check(cache, table, lengths, q, ends([40, 19, 1]), scale=scale, form=form)
+    attend_and_check(cache, table, lengths, q[:3], scale=scale)
+
+
 @pytest.mark.parametrize("form", [None, "many"])
 def test_tokens_that_are_not_finite_are_seen_by_later_rows_alone(form):
     cache, table, lengths, gen = filled([90, 200], 2, 64, 12)
@@ -368,6 +423,22 @@ def test_eviction_of_sequences_that_miss_pages():
     assert left.tolist() == [90, 90, 0, 90]
     table[3, 1:] = -1
     assert evict_and_check(cache, table, whole(MAXINT, 90, -4, 200), 89, 10).tolist() == [89, 89, 0, 0]
+
+
+@pytest.mark.parametrize("dim", [32, 128])
+@pytest.mark.parametrize("keep", [1_470, 1_535, 1_472])
+def test_eviction_of_few_of_many(dim, keep):
+    """Several pages are one workgroup's: sequences that keep all, that end early or miss pages among others; tokens of all sizes, so that
+    powers grow, and one that is not finite."""
+    lengths = [1_536, 1_500, 0, 1_536, keep, keep + 1, 700] + [1_536] * 17
+    cache, table, held, gen = filled(lengths, 4, dim, keep + dim, blocks=24)
+    (k, v) = torch.randn((2, 10 * 24, 4, dim), generator=gen, device=DEV) * 10.0 ** torch.randint(-2, 5, (2, 10 * 24, 4, 1), generator=gen, device=DEV)
+    k[3, 0, 5] = math.nan
+    cache.write(k, v, table, (held - 10).clamp(min=0), ends([10] * 24))
+    table[3, 5] = -1
+    table[8, 23] = MAXINT
+    weigh_at_random(cache, gen)
+    evict_and_check(cache, table, held, keep, 12)
 
 
 @pytest.mark.parametrize("length, keep, recent", [(20_000, 9_999, 500), (70_001, 1_000, 999), (70_001, 69_990, 0)])

@@ -186,8 +186,10 @@ Space space_of(const AttendArgs &a, const vl_queries *q, bool accumulate) {
     Space s = {part_bytes(a, many ? many_splits(a) : shares_for(a, q->type, few_tiles(a)).splits), 0, 0};
     if (!accumulate) return s;
     s.ends = up((int64_t)a.t.rows * a.heads_q * 8);
-    // the scores of a token and head are reached by 31 bits
-    if (!many && !a.t.offsets && a.group <= 16 && a.t.blocks <= 1 << 18) s.scores = up((int64_t)a.t.rows * a.heads_q * a.t.blocks * kPage * 4);
+    // the scores of a token and head are reached by 31 bits; where tables are so wide that they would take more than 4 GiB, they are
+    // made once more from the keys
+    const int64_t scores = up((int64_t)a.t.rows * a.heads_q * a.t.blocks * kPage * 4);
+    if (!many && !a.t.offsets && a.group <= 16 && a.t.blocks <= 1 << 18 && scores <= (int64_t)1 << 32) s.scores = scores;
     return s;
 }
 

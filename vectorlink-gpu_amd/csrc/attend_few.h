@@ -721,11 +721,13 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256, WAVES != 8 && D <= 128 ? 2 
     } else {
         const float total = sum_of_row<C>(st.sum);
         const int64_t to = out_row(r);
-        if constexpr (USE == kOnceAndScores)
+        if constexpr (USE == kOnceAndScores) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // the scores are other lanes' stores
             weigh_places<C, 256>(a, b, h, lane * 4, length, [&](int g) {
                 const int top = __builtin_amdgcn_readlane(__builtin_bit_cast(int, st.top), g), all = __builtin_amdgcn_readlane(__builtin_bit_cast(int, total), g);
                 return row_ends(__builtin_bit_cast(float, top), __builtin_bit_cast(float, all));
             });
+        }
         if (to < 0) return;
 #pragma unroll
         for (int p = 0; p < PT::kCount; p++) {
