@@ -650,10 +650,11 @@ int vl_cache8_read(const vl_cache8 *cache, const vl_tokens *tokens, int type,
  * sum of the softmax weights that it gets, over all rows and the queries that
  * share its head; a row with a score or a sum that is not finite adds nothing.
  * The sum is made in 32 bits and in one order, so that no weight depends on
- * chance; no two sequences may share a page then. */
+ * chance; no page may stand twice in the tables then. */
 int64_t vl_attend8_workspace_bytes(const vl_cache8 *cache, const vl_tokens *tokens, const vl_queries *queries, int accumulate);
 int vl_attend8(const vl_cache8 *cache, const vl_tokens *tokens, const vl_queries *queries, int accumulate,
                void *workspace, int64_t workspace_bytes, void *stream);
+/* VL_ATTEND_FEW or VL_ATTEND_MANY: the form that such a call takes */
 int vl_attend8_form(const vl_cache8 *cache, const vl_tokens *tokens, const vl_queries *queries);
 
 /* Cuts every sequence down to `keep` tokens.  tokens: rows == sequences, offsets
@@ -669,8 +670,8 @@ int vl_attend8_form(const vl_cache8 *cache, const vl_tokens *tokens, const vl_qu
  * Tokens on no page leave first: new_lengths[b] is the smaller of keep and the
  * tokens on pages, of a sequence of at most keep tokens its length (cut to what
  * its table can name); what would move to a place on no page is lost.  0 <=
- * recent <= keep.  No two sequences may share a page.  new_lengths must not be
- * lengths. */
+ * recent <= keep.  No page may stand twice in the tables.  new_lengths that
+ * overlap lengths are refused. */
 int64_t vl_cache8_evict_workspace_bytes(const vl_cache8 *cache, const vl_tokens *tokens, int64_t keep);
 int vl_cache8_evict(const vl_cache8 *cache, const vl_tokens *tokens, int64_t keep, int64_t recent,
                     int32_t *new_lengths, void *workspace, int64_t workspace_bytes, void *stream);

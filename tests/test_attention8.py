@@ -60,6 +60,8 @@ def test_evictions_are_checked(lib):
     for keep, recent in ((-1, 0), (1 << 31, 0), (64, -1), (64, 65)):
         assert lib.vl_cache8_evict(cache(), tokens(), keep, recent, 256, 256, MUCH, None) == -1
     assert lib.vl_cache8_evict(cache(), tokens(), 64, 0, None, 256, MUCH, None) == -1
+    for new in (1_024, 1_032, 1_016):  # three lengths of 4 bytes; other workgroups still read them
+        assert lib.vl_cache8_evict(cache(), tokens(lengths=1_024), 64, 0, new, 256, MUCH, None) == -1 and b"overlap" in lib.vl_last_error()
     assert lib.vl_cache8_evict(cache(), tokens(offsets=256), 64, 0, 256, 256, MUCH, None) == -1
     plain = cache(weights=None, positions=None)
     assert lib.vl_cache8_evict(plain, tokens(), 64, 0, 256, 256, MUCH, None) == -1 and b"weights" in lib.vl_last_error()

@@ -2,8 +2,8 @@
 //
 // What stays behind the new length moves into places before it that got free, so a step that gives up 64 tokens moves at most 64
 // a head, where closing the gaps in order would move nearly all of them; sources (behind the new length) and destinations
-// (before it) are apart, so pages are made in any order.  Two launches: one workgroup a sequence and head ranks its tokens and lists
-// free places and what moves there; one a page and head moves.
+// (before it) are apart, so pages are made in any order.  A workgroup for a sequence and head, or several in
+// six launches for a long one, ranks its tokens and lists free places and what moves there; a launch over pages and heads moves.
 #include "cache8.h"
 
 namespace {
@@ -559,6 +559,8 @@ VL_EXPORT int vl_cache8_evict(const vl_cache8 *cache, const vl_tokens *tokens, i
         return VL_ERR_WORKSPACE;
     }
     VL_REQUIRE(((uintptr_t)workspace & 15) == 0, "workspace not on a 16-byte boundary");
+    // workgroups of other heads still read the old ones
+    VL_REQUIRE(new_lengths + a.t.sequences <= a.t.lengths || a.t.lengths + a.t.sequences <= new_lengths, "new_lengths overlap lengths");
     uint8_t *const ws = (uint8_t *)workspace;
     a.recent = (int)recent;
     a.lengths = new_lengths;

@@ -195,7 +195,7 @@ class KVCache8:
 
     def evict(self, table: Tensor, lengths: Tensor, keep: int, recent: int = 0) -> Tensor:
         """Cut sequences of more than `keep` tokens down to that many, in each head those that count most: the `recent` latest positions,
-        then the largest weights, of equal ones the earlier.  Tokens that stay move into the places of those that leave, so that a
+        then the largest weights, of equal ones the earlier.  No page may stand twice in the table.  Tokens that stay move into the places of those that leave, so that a
         sequence's first places hold them, in no order that attention would depend on.  The lengths [sequences] that are left."""
         assert self.weights is not None, "the cache keeps no weights: weighted=True"
         assert 0 <= recent <= keep < 1 << 31, f"recent: {recent} of {keep} that stay"
@@ -239,8 +239,8 @@ def attend(queries: Tensor, cache: Union[KVCache, KVCache8], table: Tensor, leng
     what stands before them and themselves, or with causal=False everything.  A row that sees nothing gives zeros.  With
     return_lse also the logarithms of the sums of exponentials [rows, heads], by which parts of an attention are joined.
     form: the library chooses one by the sizes; "few" or "many" ask for it, for tests and measurements.  Of bfloat16 "many" rounds the
-    weights to bfloat16 as well, "few" holds 16 bits of them.  accumulate, for a weighted KVCache8 whose pages no two of the sequences
-    share: the softmax weights that a token gets from all rows and the queries that share its head are added to its weight."""
+    weights to bfloat16 as well, "few" holds 16 bits of them.  accumulate, for a weighted KVCache8 and a table in which no page stands
+    twice: the softmax weights that a token gets from all rows and the queries that share its head are added to its weight."""
     assert form is None or form in nv.ATTEND_FORMS, f"unknown form {form!r}: expected one of {sorted(nv.ATTEND_FORMS)}"
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
