@@ -234,15 +234,11 @@ __global__ __launch_bounds__(W * 64) void evict_choose_kernel(EvictArgs a) {
             if (s_bin[i]) atomicAdd(&bins[kDigits * kBins + i], s_bin[i]);
         return;
     }
-    // keys above `prefix` stay, and the first `need` of those equal to it: how many of both there are, before and behind the new length
-    uint64_t more[K], equal[K];
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-        more[k] = equal[k] = 0;
-        if (k >= n) continue;
-        more[k] = __ballot(there(k) && key[k] > prefix);
-        equal[k] = __ballot(there(k) && key[k] == prefix);
-    }
+    // keys above `prefix` stay, and the first `need` of those equal to it: how many of both there are, before and behind the new length.
+    // Asked of the keys both times: masks of 32 blocks fill more scalar registers than there are (one sequence of
+    // 9,000 40 us with both launches, 28 without them; with 16 blocks 1 us more).
+    auto more_of = [&](int k) { return __ballot(there(k) && key[k] > prefix); };
+    auto equal_of = [&](int k) { return __ballot(there(k) && key[k] == prefix); };
     auto front = [&](int block) {  // the places of a block before the new length
         const int before = min(max(kept - block * kPage, 0), kPage);
         return before == kPage ? ~0ull : (1ull << before) - 1;
@@ -251,11 +247,12 @@ __global__ __launch_bounds__(W * 64) void evict_choose_kernel(EvictArgs a) {
     if constexpr (whole || STAGE == kCount) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const uint64_t f = front(from + k);
-            count[0] += __popcll(more[k] & f);
-            count[1] += __popcll(more[k] & ~f);
-            count[2] += __popcll(equal[k] & f);
-            count[3] += __popcll(equal[k] & ~f);
+            if (k >= n) continue;
+            const uint64_t f = front(from + k), more = more_of(k), equal = equal_of(k);
+            count[0] += __popcll(more & f);
+            count[1] += __popcll(more & ~f);
+            count[2] += __popcll(equal & f);
+            count[3] += __popcll(equal & ~f);
         }
         int32_t *const to = whole ? s_count[wave] : a.counts + ((list * a.chunks + chunk) * W + wave) * 4;
         if (lane < 4) to[lane] = lane == 0 ? count[0] : lane == 1 ? count[1] : lane == 2 ? count[2] : count[3];
@@ -286,9 +283,10 @@ __global__ __launch_bounds__(W * 64) void evict_choose_kernel(EvictArgs a) {
 #pragma unroll
     for (int k = 0; k < K; k++) {
         if (k >= n) continue;
-        const int block = from + k, ties = __popcll(equal[k]);
-        uint64_t in = more[k] | equal[k];
-        if (tie + ties > need) in = more[k] | __ballot((equal[k] >> lane & 1) && tie + __popcll(equal[k] & before) < need);
+        const uint64_t more = more_of(k), equal = equal_of(k);
+        const int block = from + k, ties = __popcll(equal);
+        uint64_t in = more | equal;
+        if (tie + ties > need) in = more | __ballot((equal >> lane & 1) && tie + __popcll(equal & before) < need);
         tie += ties;
         const uint64_t f = front(block), hole = ~in & f, moving = in & ~f;
         if (lane == 0 && block < a.pages) starts[block] = free;
