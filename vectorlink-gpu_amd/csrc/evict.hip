@@ -24,12 +24,12 @@ struct EvictArgs {
     int64_t *border;          // [2] page and head that the new length lies in, and its scales before any change
     // where workgroups share one, per sequence and head:
     int32_t *latest;          // [chunks, 2] the latest position, tokens on pages
-    uint32_t *bins;           // [3, kBins]
+    uint32_t *bins;           // [kBinWords]: [3, kBins], and what was found with each of the three: prefix and need
     int32_t *counts;          // [chunks * kSharedWaves, 4]
 };
 
 constexpr int kDigit = 11;  // bits of a key that one pass over the weights tells apart
-constexpr int kBins = 1 << kDigit;
+constexpr int kBins = 1 << kDigit, kBinWords = 3 * kBins + 8;
 // wavefronts of a workgroup and blocks of a wavefront: where one workgroup has all of a short or a long sequence and head, and where several share
 constexpr int kShortWaves = 8, kShortBlocks = 16, kLongWaves = 16, kLongBlocks = 32, kSharedWaves = 16, kSharedBlocks = 8;
 constexpr int kChunkBlocks = kSharedWaves * kSharedBlocks;
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(W * 64) void evict_choose_kernel(EvictArgs a) {
     const int h = (int)(list % a.c.heads), b = (int)(list / a.c.heads);
     const int length = length_of(a.t, b);
     int32_t *const starts = a.starts + list * (a.pages + 1);
-    uint32_t *const bins = a.bins + list * (3 * kBins);
+    uint32_t *const bins = a.bins + list * kBinWords;
     const bool last_stage = whole || STAGE == kList;
     if (length <= a.keep) {
         if (last_stage && chunk == 0) {
@@ -201,9 +201,19 @@ __global__ __launch_bounds__(W * 64) void evict_choose_kernel(EvictArgs a) {
     int need = kept;
     uint32_t prefix = 0;
     constexpr int kBitsOf[3] = {kDigit, kDigit, 32 - 2 * kDigit};
-    if constexpr (!whole) {
-#pragma unroll
-        for (int d = 0; d < kDigits; d++) prefix = prefix << kBitsOf[d] | digit_of(bins + d * kBins, need, s_digit);
+    if constexpr (!whole && kDigits > 0) {
+        constexpr int told = STAGE == kList ? kDigits : kDigits - 1;  // by the launches before this one
+        if constexpr (told > 0) {
+            prefix = bins[3 * kBins + 2 * told - 2];
+            need = (int)bins[3 * kBins + 2 * told - 1];
+        }
+        if constexpr (told < kDigits) {
+            prefix = prefix << kBitsOf[told] | digit_of(bins + told * kBins, need, s_digit);
+            if (chunk == 0 && threadIdx.x == 0) {
+                bins[3 * kBins + 2 * kDigits - 2] = prefix;
+                bins[3 * kBins + 2 * kDigits - 1] = (uint32_t)need;
+            }
+        }
     }
     auto count_digit = [&](int d) {  // into the bins in LDS, which are 0
         const int bits = kBitsOf[d], low = d < 2 ? 32 - (d + 1) * kDigit : 0;
@@ -503,7 +513,7 @@ Layout layout_of(const CacheView &c, const Tokens &t, int64_t keep) {
     l.chunks = t.blocks <= kLongWaves * kLongBlocks ? 1 : (t.blocks + kChunkBlocks - 1) / kChunkBlocks;
     const int64_t shared = l.chunks > 1 ? lists : 0;
     l.bins = l.latest + up(shared * l.chunks * 8);
-    l.counts = l.bins + up(shared * 3 * kBins * 4);
+    l.counts = l.bins + up(shared * kBinWords * 4);
     l.bytes = l.counts + up(shared * l.chunks * kSharedWaves * 16);
     return l;
 }
