@@ -94,6 +94,14 @@ def test_scores_take_4_gib_at_most(lib):
     assert 1 << 32 <= need(8_192) < (1 << 32) + (1 << 28) and need(8_193) < 1 << 28
 
 
+def test_a_cache_without_pages_keeps_no_scores(lib):
+    """There would be no weights to add them to."""
+    (few, wide) = (tokens(), tokens(blocks=40_000, table_stride=40_000))
+    for t in (few, wide):
+        assert lib.vl_attend8_workspace_bytes(cache(pages=0), t, queries(), 1) == lib.vl_attend8_workspace_bytes(cache(pages=0), t, queries(), 0)
+        assert lib.vl_attend8_workspace_bytes(cache(), t, queries(), 1) > lib.vl_attend8_workspace_bytes(cache(), t, queries(), 0)
+
+
 def test_calls_without_rows_succeed(lib):
     t = tokens(rows=0, sequences=0, table=None, lengths=None)
     assert lib.vl_cache8_write(cache(), t, 1, None, 0, 0, None, 0, 0, None, None) == 0

@@ -545,6 +545,31 @@ def test_captured_steps():
         q.normal_(generator=gen)
 
 
+def test_nothing_to_look_at():
+    """Tables of no blocks, a cache of no pages, no sequences: zeros, and lengths that are cut to what there is."""
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    q = queries_for(2, 4, 64, gen, torch.bfloat16)
+    (kv, held) = (queries_for(2, 2, 64, gen, torch.bfloat16), whole(100, 7))
+    full = filled([100], 2, 64, 5)[0]
+    none = KVCache8.empty(0, 2, 64, weighted=True)
+    for cache, table, left in [(full, torch.empty((2, 0), dtype=torch.int32, device=DEV), [0, 0]), (none, whole(0, 1, 2, 3).view(2, 2), [0, 7]),
+                               (full, torch.full((2, 2), -1, dtype=torch.int32, device=DEV), [0, 7])]:
+        was = [t.clone() for t in (cache.keys, cache.values, cache.scales, cache.weights, cache.positions)]
+        for offsets in (None, whole(0, 1, 2), whole(0, 0, 0)):
+            cache.write(kv, kv, table, held, offsets)
+            assert not any(bool(t.any()) for t in cache.read(table, held, 2, offsets))
+            out = attend(q, cache, table, held, offsets, accumulate=True)
+            assert not bool(out[:0 if offsets is not None and not int(offsets[-1]) else None].any())
+        assert cache.evict(table, held, 10, 3).tolist() == left
+        assert cache.evict(table, held, 0).tolist() == [0, 0]
+        for a, b in zip(was, (cache.keys, cache.values, cache.scales, cache.weights, cache.positions)):
+            assert torch.equal(a.nan_to_num() if a.is_floating_point() else a, b.nan_to_num() if b.is_floating_point() else b)
+    nothing = torch.empty((0, 3), dtype=torch.int32, device=DEV)
+    full.write(kv[:0], kv[:0], nothing, held[:0])
+    assert attend(q[:0], full, nothing, held[:0], accumulate=True).shape == (0, 4, 64)
+    assert full.evict(nothing, held[:0], 5).shape == (0,)
+
+
 def test_two_streams():
     """Two caches worked on at once."""
     jobs = []

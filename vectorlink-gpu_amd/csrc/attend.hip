@@ -184,7 +184,7 @@ Space space_of(const AttendArgs &a, const vl_queries *q, bool accumulate) {
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     const bool many = takes_many(a, q);
     Space s = {part_bytes(a, many ? many_splits(a) : shares_for(a, q->type, few_tiles(a)).splits), 0, 0};
-    if (!accumulate) return s;
+    if (!accumulate || a.c.pages == 0) return s;  // without pages no token has a weight, nor are there any to read
     s.ends = up((int64_t)a.t.rows * a.heads_q * 8);
     // the scores of a token and head are reached by 31 bits; where tables are so wide that they would take more than 4 GiB, they are
     // made once more from the keys

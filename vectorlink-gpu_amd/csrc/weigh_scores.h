@@ -30,7 +30,7 @@ __device__ inline void weigh_places(const AttendArgs &a, int b, int h, int from,
 #pragma unroll
         for (int u = 0; u < U; u++) page[u] = from + u * STEP < sees ? page_of(a.t, a.c, b, (from + u * STEP) / kPage) : -1;
 #pragma unroll
-        for (int u = 0; u < U; u++) {  // of no page: loads of what is there, which nothing is made of
+        for (int u = 0; u < U; u++) {  // of no page: loads of the cache's first, which there is, and nothing is made of them
             const int place = min(from + u * STEP, (sees - 1) & ~3);
             const float *const at = scores + (int64_t)(place / kPage) * a.group * kPage + place % kPage;
 #pragma unroll
