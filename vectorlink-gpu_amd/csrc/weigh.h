@@ -27,12 +27,14 @@ __device__ inline void load_keys(PageKeys<D, NS> &g, const AttendArgs &a, int64_
     const uint32_t scales = a.c.scales[unit];
     g.marked = is_marked(scales);
     g.scale = (NS == 2 ? scale_with(a.scale, scale_of_keys(scales)) : a.scale) * (NS == 3 ? 1.0f : a.turn);
+    // Without a scale all scores are 0, and 0 times a product beyond float32 would be none: the keys are 0 then.  (Queries of float32 are.)
+    const uint32_t there = NS < 3 && a.turn == 0 ? 0 : ~0u;
 #pragma unroll
     for (int t = 0; t < 2; t++) {
         u32x4 x[D / 32];
         const uint8_t *const at = a.c.keys + unit * (kPage * D) + (t * 32 + col) * D + hi * 16;
 #pragma unroll
-        for (int c = 0; c < D / 32; c++) x[c] = *reinterpret_cast<const u32x4 *>(at + c * 32);
+        for (int c = 0; c < D / 32; c++) x[c] = *reinterpret_cast<const u32x4 *>(at + c * 32) & there;
 #pragma unroll
         for (int c = 0; c < D / 32; c++) {
             if constexpr (NS == 2) {
