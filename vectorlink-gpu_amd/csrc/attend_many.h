@@ -323,7 +323,7 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
             edges = __ballot(pages >= 0 && ((block + 1) * kPage > least || a.c.bound_scales[(int64_t)pages * a.c.heads + h] == kBoundless));
         } else {
             scales = pages >= 0 ? a.c.scales[(int64_t)pages * a.c.heads + h] : 0;
-            edges = __ballot(pages >= 0 && ((block + 1) * kPage > least || is_marked(scales)));
+            edges = __ballot(pages >= 0 && ((block + 1) * kPage > least || is_marked(scales) || (HALF && is_beyond(a.scale, scale_of_keys(scales)))));
         }
     };
     look_up(from);
@@ -389,10 +389,12 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
                     for (int i = 0; i < 16; i++) s[t][i] += sums[1][t][i];
             }
             if (edge >> k & 1) {
+                const float ahead = HALF ? power_ahead(a.scale, scale_of_keys(here_scales[k])) : 1.0f;
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
+                        if constexpr (HALF) s[t][i] *= ahead;
                         const int place = t * 32 + 8 * (i >> 2) + 4 * hi + (i & 3);
                         if (reinterpret_cast<const uint8_t *>(in)[I::kBytes + place]) s[t][i] = NAN;
                         if (block * kPage + place >= sees) s[t][i] = -INFINITY;

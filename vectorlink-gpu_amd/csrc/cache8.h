@@ -47,9 +47,12 @@ __device__ inline f16x8 eight_halves(uint32_t x, uint32_t y) {
     u32x4 v = {two_halves<false>(x), two_halves<true>(x), two_halves<false>(y), two_halves<true>(y)};
     return __builtin_bit_cast(f16x8, v);
 }
-// What scores of such keys are multiplied with: the call's scale and the keys' power, kept a normal number - 0 or infinite it would make
-// NaN of scores that are infinite or 0, where the true product is next to nothing or beyond everything all the same.
-__device__ inline float scale_with(float scale, float power) { return __builtin_amdgcn_fmed3f(scale * power, 0x1p-126f, 0x1.fffffep127f); }
+// What scores of such keys are multiplied with: the call's scale and the keys' power, kept a normal number - 0 would make NaN of scores
+// that are masked, where the true product leaves all scores next to nothing all the same.  Where it leaves float32 it is the scale
+// alone, and the scores take the power before (power_ahead): one of codes and half precision may be as little as 2^-33.
+__device__ inline bool is_beyond(float scale, float power) { return scale * power > 0x1.fffffep127f; }
+__device__ inline float scale_with(float scale, float power) { return is_beyond(scale, power) ? scale : fmaxf(scale * power, 0x1p-126f); }
+__device__ inline float power_ahead(float scale, float power) { return is_beyond(scale, power) ? power : 1.0f; }
 // the four codes of a word as numbers, and the way back: to the nearest code, of two as near the even one; magnitudes up to 448
 __device__ inline f32x4 four_numbers(uint32_t word) {
     const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);

@@ -18,14 +18,15 @@ constexpr int query_parts(int NS) { return NS == 3 ? 3 : 1; }
 template <int D, int NS>
 struct PageKeys {
     Operand<NS> k[2][D / 16];
-    float scale;  // of the scores
-    bool marked;
+    float ahead, scale;  // of the scores: see scale_with
+    bool apart;          // a token may not be finite, or ahead is not 1
 };
 template <int D, int NS>
 __device__ inline void load_keys(PageKeys<D, NS> &g, const AttendArgs &a, int64_t unit) {
     const int col = threadIdx.x & 31, hi = threadIdx.x >> 5 & 1;
     const uint32_t scales = a.c.scales[unit];
-    g.marked = is_marked(scales);
+    g.ahead = NS == 2 ? power_ahead(a.scale, scale_of_keys(scales)) : 1.0f;
+    g.apart = is_marked(scales) || g.ahead != 1.0f;
     g.scale = (NS == 2 ? scale_with(a.scale, scale_of_keys(scales)) : a.scale) * (NS == 3 ? 1.0f : a.turn);
     // Without a scale all scores are 0, and 0 times a product beyond float32 would be none: the keys are 0 then.  (Queries of float32 are.)
     const uint32_t there = NS < 3 && a.turn == 0 ? 0 : ~0u;
@@ -69,23 +70,23 @@ __device__ inline void weigh_tile(float (&sum)[32], const PageKeys<D, NS> &g, fl
                 else to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(g.k[t][c], q[n], to, 0, 0, 0);
             }
     }
-    auto weight = [&](int i) {
+    auto weight = [&](int i, float ahead) {
         const float score = NS == 3 ? s[i >> 4][i & 15] + small[i >> 4][i & 15] : s[i >> 4][i & 15];
-        return __builtin_amdgcn_exp2f(__builtin_fmaf(score, g.scale, minus));
+        return __builtin_amdgcn_exp2f(__builtin_fmaf(NS == 2 ? score * ahead : score, g.scale, minus));
     };
-    if (g.marked || __ballot(sees < kPage)) {
+    if (g.apart || __ballot(sees < kPage)) {
         const int mine = sees - 4 * (threadIdx.x >> 5 & 1);
 #pragma unroll
         for (int i = 0; i < 32; i++) {
             if (i % 8 == 0) __builtin_amdgcn_sched_barrier(0);
-            const float p = weight(i) * by;
+            const float p = weight(i, g.ahead) * by;
             sum[i] += (i >> 4) * 32 + 8 * (i >> 2 & 3) + (i & 3) < mine ? p : 0.0f;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 32; i++) {
             if (i % 8 == 0) __builtin_amdgcn_sched_barrier(0);  // a few exponentials at a time: all 32 at once take the registers
-            sum[i] = __builtin_fmaf(weight(i), by, sum[i]);
+            sum[i] = __builtin_fmaf(weight(i, 1.0f), by, sum[i]);
         }
     }
 }
