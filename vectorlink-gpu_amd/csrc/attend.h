@@ -27,6 +27,11 @@ struct AttendArgs {
 };
 constexpr int kMaxSplits = 64;
 
+// Weights are exp2(scale s - top) with one rounding, of the difference, where top is rounded: a largest score of 2^k finds itself up to
+// 2^(k - 24) above or below it, which its row's sum takes out again, until it leaves no float32 - the row would be NaN, or zeros.
+// Where top is beyond 2^28 (16 either way) the scores are rounded as it is.
+__device__ inline bool is_far(float top) { return __builtin_fabsf(top) > 0x1p28f; }
+
 // 16 rows at a time, the tokens split over wavefronts and workgroups
 template <int NS, int BITS = 4>
 int launch_attend_few(const AttendArgs &a, int64_t tiles, hipStream_t stream);

@@ -371,13 +371,19 @@ __device__ inline void take_page(RowState<D> &st, PageRegs<D, BITS> &g, const Qu
     }
     // scale s - top with one rounding: a product rounded on its own would be off by a share of the score, not of the difference
     const float minus = st.top > -INFINITY ? -st.top : 0.0f;  // a row that has seen nothing yet: all weights 0
+    float by = scale;
+    if (const bool far = is_far(minus); __ballot(far)) {
+#pragma unroll
+        for (int i = 0; i < 4 * M; i++) t[i >> 2][i & 3] = far ? t[i >> 2][i & 3] * scale : t[i >> 2][i & 3];
+        by = far ? 1.0f : scale;
+    }
     uint32_t weight[NW][2][4];  // [part][two tokens][tile]
     {
         uint32_t pair[NW][2][M];
 #pragma unroll
         for (int k = 0; k < M; k++) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) t[k][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[k][e], scale, minus));
+            for (int e = 0; e < 4; e++) t[k][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[k][e], by, minus));
             st.sum += (t[k][0] + t[k][1]) + (t[k][2] + t[k][3]);
 #pragma unroll
             for (int two = 0; two < 2; two++) {

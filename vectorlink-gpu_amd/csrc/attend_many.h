@@ -418,12 +418,18 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
                     for (int i = 0; i < 16; i++) acc[d][i] *= less;
             }
             const float minus = top > -INFINITY ? -top : 0.0f;
+            float by = scale;
+            if (const bool far = is_far(minus); __ballot(far)) {
+#pragma unroll
+                for (int i = 0; i < 32; i++) s[i >> 4][i & 15] = far ? s[i >> 4][i & 15] * scale : s[i >> 4][i & 15];
+                by = far ? 1.0f : scale;
+            }
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 float part = 0;
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], scale, minus));
+                    s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], by, minus));
                     part += s[t][i];
                 }
                 sum += part;

@@ -70,23 +70,25 @@ __device__ inline void weigh_tile(float (&sum)[32], const PageKeys<D, NS> &g, fl
                 else to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(g.k[t][c], q[n], to, 0, 0, 0);
             }
     }
-    auto weight = [&](int i, float ahead) {
-        const float score = NS == 3 ? s[i >> 4][i & 15] + small[i >> 4][i & 15] : s[i >> 4][i & 15];
-        return __builtin_amdgcn_exp2f(__builtin_fmaf(NS == 2 ? score * ahead : score, g.scale, minus));
-    };
-    if (g.apart || __ballot(sees < kPage)) {
+    auto score = [&](int i) { return NS == 3 ? s[i >> 4][i & 15] + small[i >> 4][i & 15] : s[i >> 4][i & 15]; };
+    auto weight = [&](float x, float scale) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, minus)); };
+    // These scores are sums in another order than attention's: beyond 2^16 the largest may be far above what the row ends with, and no
+    // weight is more than 1.
+    if (g.apart || __ballot(sees < kPage || __builtin_fabsf(minus) > 0x1p16f)) {
         const int mine = sees - 4 * (threadIdx.x >> 5 & 1);
+        const bool far = is_far(minus);
+        const float then = far ? g.scale : 1.0f, scale = far ? 1.0f : g.scale;
 #pragma unroll
         for (int i = 0; i < 32; i++) {
             if (i % 8 == 0) __builtin_amdgcn_sched_barrier(0);
-            const float p = weight(i, g.ahead) * by;
+            const float p = fminf(fmaxf(weight((NS == 2 ? score(i) * g.ahead : score(i)) * then, scale) * by, 0.0f), 1.0f);
             sum[i] += (i >> 4) * 32 + 8 * (i >> 2 & 3) + (i & 3) < mine ? p : 0.0f;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 32; i++) {
             if (i % 8 == 0) __builtin_amdgcn_sched_barrier(0);  // a few exponentials at a time: all 32 at once take the registers
-            sum[i] = __builtin_fmaf(weight(i, 1.0f), by, sum[i]);
+            sum[i] = __builtin_fmaf(weight(score(i), g.scale), by, sum[i]);
         }
     }
 }

@@ -45,8 +45,11 @@ __device__ inline void weigh_places(const AttendArgs &a, int b, int h, int from,
             for (int g = 0; g < G; g++) {
                 const RowEnds e = ends(min(g, a.group - 1));
                 if (g >= a.group || !e.fine) continue;
+                const bool far = is_far(e.minus);
+                const f32x4 x = far ? s[u][g] * a.scale : s[u][g];
+                const float by = far ? 1.0f : a.scale;
 #pragma unroll
-                for (int i = 0; i < 4; i++) sum[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][g][i], a.scale, e.minus)), e.by, sum[i]);
+                for (int i = 0; i < 4; i++) sum[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(x[i], by, e.minus)), e.by, sum[i]);
             }
             const int place = from + u * STEP;
 #pragma unroll
