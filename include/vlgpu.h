@@ -559,12 +559,16 @@ typedef struct vl_queries {
     double scale; /* scores are scale * <query, key>; finite, as a float32 too */
     int32_t type; /* VL_BF16, VL_F16, VL_F32 */
     int32_t causal; /* 0: every row sees all lengths[b] tokens; else those up to its own place */
-    int64_t form; /* of vl_attend: 0, or VL_ATTEND_FEW or VL_ATTEND_MANY whatever the sizes, for tests and measurements */
+    int64_t form; /* of vl_attend: 0, or VL_ATTEND_FEW or VL_ATTEND_MANY whatever the sizes */
 } vl_queries;
 
 /* Softmax attention over everything the cache holds of the sequences.  Sums and
  * softmax are held in 32 bits; keys, values and queries enter the products
- * exactly, the weights rounded to the queries' type or finer. */
+ * exactly, the weights rounded to the queries' type or finer: of bfloat16 to 8
+ * bits by the form for many rows, to 16 by the other, which can be asked for.
+ * Products of queries and keys, scores and sums of weights (up to 2^8 each)
+ * times values leave float32 where its range ends.  Beyond 2^28 scores are
+ * compared to 24 bits, and the largest has all weight. */
 int64_t vl_attend_workspace_bytes(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries);
 int vl_attend(const vl_cache *cache, const vl_tokens *tokens, const vl_queries *queries,
               void *workspace, int64_t workspace_bytes, void *stream);
@@ -633,12 +637,12 @@ typedef struct vl_cache8 {
 
 /* vl_cache_write for such a cache.  The power of a block that is written into is
  * the least 2^e, -117 <= e <= 119, whose 448-fold is not below any new element
- * (magnitudes over 448 * 2^119 become that); if the block holds tokens already it is the old power at least, and where it grows
- * they are rounded to it again.  Codes are the nearest ones, of two as near the
- * even one.  A token with an element that is not finite reads as NaN, and its
- * elements do not count for the power.  New tokens have weight 0 and position
- * positions[row], NULL: their place in the sequence.  Two sequences must not
- * share a page that is written into. */
+ * (magnitudes over 448 * 2^119 become that); if the block holds tokens already
+ * it is the old power at least, and where it grows they are rounded to it again.
+ * Codes are the nearest ones, of two as near the even one.  A token with an
+ * element that is not finite reads as NaN, and its elements do not count for the
+ * power.  New tokens have weight 0 and position positions[row], NULL: their place
+ * in the sequence.  Two sequences must not share a page that is written into. */
 int vl_cache8_write(const vl_cache8 *cache, const vl_tokens *tokens, int type,
                     const void *keys, int64_t key_row, int64_t key_head,
                     const void *values, int64_t value_row, int64_t value_head,
@@ -650,7 +654,9 @@ int vl_cache8_read(const vl_cache8 *cache, const vl_tokens *tokens, int type,
  * sum of the softmax weights that it gets, over all rows and the queries that
  * share its head; a row with a score or a sum that is not finite adds nothing.
  * The sum is made in 32 bits and in one order, so that no weight depends on
- * chance; no page may stand twice in the tables then. */
+ * chance; no page may stand twice in the tables then.  Rows of prompts have their
+ * scores made twice, in two orders: what 32 bits lose of a score may differ, and
+ * of scores beyond 2^28 the largest may be missed. */
 int64_t vl_attend8_workspace_bytes(const vl_cache8 *cache, const vl_tokens *tokens, const vl_queries *queries, int accumulate);
 int vl_attend8(const vl_cache8 *cache, const vl_tokens *tokens, const vl_queries *queries, int accumulate,
                void *workspace, int64_t workspace_bytes, void *stream);
@@ -661,8 +667,8 @@ int vl_attend8_form(const vl_cache8 *cache, const vl_tokens *tokens, const vl_qu
  * NULL, lengths: what the sequences hold.  In each head of a sequence of more
  * than `keep` tokens they are ranked: those whose position is one of the last
  * `recent` (above the largest position of the head minus recent) before all
- * others, then by weight, NaN last, of equal ones the earlier place first.  The
- * best `keep` stay.  Those of them behind the first `keep` places move, in their
+ * others, the earlier places first, whatever their weights; the others by weight,
+ * NaN last, of equal ones the earlier place first.  The best `keep` stay.  Those of them behind the first `keep` places move, in their
  * order, into the places before that got free, with weight and position: heads
  * differ in what they keep and in its order, which attention does not depend on.
  * A page that tokens move to has its power raised to what they need and its

@@ -251,8 +251,6 @@ __device__ inline float over_copies(float x, F f) {
     return x;
 }
 
-// A page's 64 tokens: this lane's row (r % C) sees the first `sees` of them, `written` hold something; edge: some row does not see
-// some token, or some token may not be finite.  Spoilt tokens (scale 255) turn the rows that see them into NaN, and no others.
 // Where the scores of single tokens go: a buffer of its own for a token and head, the byte of it that this lane's row of the page has -
 // of a lane without a row past its end, where a store is dropped.  A branch around the store would leave the compiler to guess
 // how many stores are on their way, and loads would wait for them.
@@ -261,8 +259,10 @@ struct ScoresAt {
     int lane, page;
 };
 
-// put: where scores go, of a call that keeps them.  between(): what is done once the keys have been
-// used and before the values are.
+// A page's 64 tokens: this lane's row (r % C) sees the first `sees` of them, `written` hold something; edge: some row does not see
+// some token, or some token may not be finite.  Spoilt tokens (scale 255, of 8 bits codes of NaN) turn the rows that see them into NaN, and
+// no others.  put: where scores go, of a call that keeps them.  between(): what is done once the keys have been used and before the
+// values are.
 template <int D, int NS, int C, int BITS, int USE, class F>
 __device__ inline void take_page(RowState<D> &st, PageRegs<D, BITS> &g, const QueryRegs<D, NS> &f, float scale, bool edge, int sees,
                                  int written, const ScoresAt &put, F between) {

@@ -233,7 +233,8 @@ __global__ __launch_bounds__(WAVES * 64) void attend_many_kernel(AttendArgs a, i
     // Parts of a weight, as many as of a query (half precision and float32 keep 16 and 24 bits).  A bfloat16 weight is off by up to
     // 2^-8 of itself, the sum that it is divided by is not: over 16,384 tokens the result's error is 1.16 times that of its own
     // rounding (root of the mean square, 5.00e-4 and 4.30e-4), and more where values cancel.  A second part makes half as many products
-    // again and takes that away, for 661 us instead of 494; dividing by the sum of the rounded weights leaves 4.95e-4 for 506.
+    // again and takes that away, for 661 us instead of 494; dividing by the sum of the rounded weights leaves 4.95e-4 for 506.  A caller
+    // who wants 16 bits of every weight asks for the form for few rows.
     constexpr int NW = NS;
     // Half precision over a cache in 8 bits: its codes are half precision as well, so a score is one product and not two.  Keys are left
     // without their power, which the scores are multiplied with (2,048 rows over 16,384 tokens, 32 heads on 8 of 128: 875 us with two,

@@ -246,8 +246,9 @@ __global__ __launch_bounds__(W * 64) void evict_choose_kernel(EvictArgs a) {
         return;
     }
     // keys above `prefix` stay, and the first `need` of those equal to it: how many of both there are, before and behind the new length.
-    // Asked of the keys both times: masks of 32 blocks fill more scalar registers than there are (one sequence of
-    // 9,000 40 us with both launches, 28 without them; with 16 blocks 1 us more).
+    // Asked of the keys both times: masks of 32 blocks held from the counts to the lists spill vector registers too (one sequence of 9,000
+    // 40 us with both launches, 28 without them; with 16 blocks 1 us more).  As it is none spills, but the blocks' pages and ends are scalars of
+    // unrolled loops, of which the compiler keeps 216 (with 16 blocks 88) in lanes of vector registers.
     auto more_of = [&](int k) { return __ballot(there(k) && key[k] > prefix); };
     auto equal_of = [&](int k) { return __ballot(there(k) && key[k] == prefix); };
     auto front = [&](int block) {  // the places of a block before the new length

@@ -3,7 +3,8 @@
 
 namespace {
 
-// 2,048 places of a sequence and head a workgroup
+// 2,048 places of a sequence and head a workgroup: one round of 256 threads with 8 queries a head, two with more; of 4 or fewer half of a
+// round's loads lie behind the piece's end
 template <int G>
 __global__ __launch_bounds__(256) void weigh_scores_kernel(AttendArgs a, int64_t units, int pieces) {
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {

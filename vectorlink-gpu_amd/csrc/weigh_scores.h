@@ -19,7 +19,7 @@ __device__ inline RowEnds row_ends(float top, float total) {
 }
 
 // Places from, from + STEP, ... < sees of a sequence and head, four at a time: the scores of the queries that share the head (at most G)
-// are asked for all at once, and for two turns.  ends(g): (max, sum) of query g.
+// are asked for all at once, and for U turns, 16 loads of scores.  ends(g): (max, sum) of query g.
 template <int G, int STEP, class F>
 __device__ inline void weigh_places(const AttendArgs &a, int b, int h, int from, int sees, F ends) {
     constexpr int U = 16 / G;

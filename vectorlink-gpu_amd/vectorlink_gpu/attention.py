@@ -195,8 +195,9 @@ class KVCache8:
 
     def evict(self, table: Tensor, lengths: Tensor, keep: int, recent: int = 0) -> Tensor:
         """Cut sequences of more than `keep` tokens down to that many, in each head those that count most: the `recent` latest positions,
-        then the largest weights, of equal ones the earlier.  No page may stand twice in the table.  Tokens that stay move into the places of those that leave, so that a
-        sequence's first places hold them, in no order that attention would depend on.  The lengths [sequences] that are left."""
+        then the largest weights, of equal ones the earlier.  Tokens that stay move into the places of those that leave, so that a
+        sequence's first places hold them, in no order that attention would depend on.  No page may stand twice in the table, and every
+        block before the new length needs one: what would move to a place on no page is lost.  The lengths [sequences] that are left."""
         assert self.weights is not None, "the cache keeps no weights: weighted=True"
         assert 0 <= recent <= keep < 1 << 31, f"recent: {recent} of {keep} that stay"
         tokens = _tokens(table.shape[0], table, lengths, None)
@@ -238,9 +239,11 @@ def attend(queries: Tensor, cache: Union[KVCache, KVCache8], table: Tensor, leng
     dim], heads a multiple of the cache's; scale defaults to dim ** -0.5.  The rows of a sequence are its last tokens and see
     what stands before them and themselves, or with causal=False everything.  A row that sees nothing gives zeros.  With
     return_lse also the logarithms of the sums of exponentials [rows, heads], by which parts of an attention are joined.
-    form: the library chooses one by the sizes; "few" or "many" ask for it, for tests and measurements.  Of bfloat16 "many" rounds the
-    weights to bfloat16 as well, "few" holds 16 bits of them.  accumulate, for a weighted KVCache8 and a table in which no page stands
-    twice: the softmax weights that a token gets from all rows and the queries that share its head are added to its weight."""
+    form: the library chooses one by the sizes, "many" where enough rows of a sequence share its pages (over 8 bits, of 32 heads on 8,
+    from about 10 on); "few" or "many" ask for it.  Of bfloat16 "many" rounds the weights to bfloat16 as well, which makes the
+    result's error 1.2 times that of its own rounding; "few" holds 16 bits of them, and takes longer for many rows.
+    accumulate, for a weighted KVCache8 and a table in which no page stands twice: the softmax weights that a token gets from all
+    rows and the queries that share its head are added to its weight."""
     assert form is None or form in nv.ATTEND_FORMS, f"unknown form {form!r}: expected one of {sorted(nv.ATTEND_FORMS)}"
     tokens = _tokens(queries.shape[0], table, lengths, offsets)
     _check_queries(queries, cache)
