@@ -132,7 +132,9 @@ bool takes_many(const AttendArgs &a, const vl_queries *q) {
     // Of 8 bits a page is twice the bytes for every tile that reads it, and what it takes to turn it into bfloat16 no more: 8 sequences of
     // 8,192, 32 heads on 8 of 128, us few and many: 8 rows each 57 and 68, 16 rows 103 and 70, 32 rows 160 and 77; one sequence 15 and 19,
     // 24 and 21, 29 and 25; 16 of 1,024 tokens with 16 rows 25 and 30, with 32 44 and 36.  64 dimensions change sides at 16 rows (54 and
-    // 53), 32 at 24; half precision takes 91 for the 70, and changes sides at 14 and at 24 rows of 64; float32 of 64 at 50.
+    // 53), 32 at 24; half precision takes 91 for the 70, and changes sides at 14 and at 24 rows of 64; float32 of 64 at 50.  One figure does
+    // for all longer rows: 8 sequences of 8,192 with 12 rows each and with 16, of 96 dimensions 46 and 60, 77 and 62, of 192 89 and 95, 122
+    // and 96, of 256 115 and 115, 163 and 117; 10 rows, which are three tiles as 12 are, 98 and 94 of 192, 129 and 115 of 256.
     if (a.bits == 8) {
         const int at = a.c.dim <= 32 ? 0 : a.c.dim <= 64 ? 1 : 2;
         const int quarters[3][3] = {{24, 16, 12}, {28, 20, 14}, {44, 44, 44}};  // of such a unit, a page of the form for many rows

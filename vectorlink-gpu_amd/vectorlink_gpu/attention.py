@@ -240,7 +240,7 @@ def attend(queries: Tensor, cache: Union[KVCache, KVCache8], table: Tensor, leng
     what stands before them and themselves, or with causal=False everything.  A row that sees nothing gives zeros.  With
     return_lse also the logarithms of the sums of exponentials [rows, heads], by which parts of an attention are joined.
     form: the library chooses one by the sizes, "many" where enough rows of a sequence share its pages (over 8 bits, of 32 heads on 8,
-    from about 10 on); "few" or "many" ask for it.  Of bfloat16 "many" rounds the weights to bfloat16 as well, which makes the
+    more than about 12); "few" or "many" ask for it.  Of bfloat16 "many" rounds the weights to bfloat16 as well, which makes the
     result's error 1.2 times that of its own rounding; "few" holds 16 bits of them, and takes longer for many rows.
     accumulate, for a weighted KVCache8 and a table in which no page stands twice: the softmax weights that a token gets from all
     rows and the queries that share its head are added to its weight."""
